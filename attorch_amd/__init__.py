@@ -11,6 +11,7 @@ hand-written gfx950 HIP kernels behind the C ABI declared in include/attorch_hip
 from .act_layers import (CELU, ELU, GELU, SELU, ActFuncAutoGrad, Dropout, DropoutAutoGrad, Hardshrink,
                          Hardsigmoid, Hardswish, Hardtanh, LeakyReLU, LogSigmoid, Mish, ReLU, ReLU6,
                          Sigmoid, SiLU, Softplus, Softshrink, Softsign, Tanh, Tanhshrink)
+from .attention import WindowAttention, WindowAttentionAutoGrad
 from .batch_norm import BatchNorm1d, BatchNorm2d, BatchNormAutoGrad
 from .conv import Conv1d, Conv2d, Conv2dAutoGrad
 from .cross_entropy import CrossEntropyLoss, CrossEntropyLossAutoGrad
@@ -20,6 +21,7 @@ from .nll_loss import NLLLoss, NLLLossAutoGrad
 from .p_loss import HuberLoss, L1Loss, MSELoss, PLossAutoGrad, SmoothL1Loss
 from .pooling import AvgPool1d, AvgPool2d
 from .norms import LayerNorm, LayerNormAutoGrad, RMSNorm, RMSNormAutoGrad
+from .rotary import Rotary, RotaryAutoGrad
 from .softmax import LogSoftmax, Softmax, SoftmaxAutoGrad, Softmin
 from .utils import get_output_dtype
 
@@ -29,7 +31,8 @@ __all__ = [
     'Dropout', 'DropoutAutoGrad', 'ELU', 'GELU', 'GLU', 'GLUAutoGrad', 'Hardshrink', 'Hardsigmoid',
     'Hardswish', 'Hardtanh', 'HuberLoss', 'L1Loss', 'LayerNorm', 'LayerNormAutoGrad', 'LeakyReLU',
     'Linear', 'LinearAutoGrad', 'LogSigmoid', 'LogSoftmax', 'MSELoss', 'Mish', 'NLLLoss',
-    'NLLLossAutoGrad', 'PLossAutoGrad', 'RMSNorm', 'RMSNormAutoGrad', 'ReLU', 'ReLU6', 'SELU', 'SiLU',
-    'Sigmoid', 'SmoothL1Loss', 'Softmax', 'SoftmaxAutoGrad', 'Softmin', 'Softplus', 'Softshrink',
-    'Softsign', 'Tanh', 'Tanhshrink', 'get_output_dtype',
+    'NLLLossAutoGrad', 'PLossAutoGrad', 'RMSNorm', 'RMSNormAutoGrad', 'ReLU', 'ReLU6', 'Rotary',
+    'RotaryAutoGrad', 'SELU', 'SiLU', 'Sigmoid', 'SmoothL1Loss', 'Softmax', 'SoftmaxAutoGrad',
+    'Softmin', 'Softplus', 'Softshrink', 'Softsign', 'Tanh', 'Tanhshrink', 'WindowAttention',
+    'WindowAttentionAutoGrad', 'get_output_dtype',
 ]

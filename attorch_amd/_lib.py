@@ -78,6 +78,13 @@ PROTOTYPES = {
     'at_act_dropout_fwd': (I, [P, P, L, I, F, F, U, I, P]),
     'at_act_dropout_bwd': (I, [P, P, P, L, I, F, F, U, I, P]),
     'at_batch_norm_bwd': (I, [P, P, P, P, P, P, P, P, P, P, P, L, L, L, L, I, F, I, I, P]),
+    # the first argument of these is a ctypes structure, passed by reference (attention.py, rotary.py)
+    'at_attention_row_pitch': (L, [L, L, L]),
+    'at_attention_fwd_workspace_bytes': (L, [P]),
+    'at_attention_fwd': (I, [P, P, P, P, P, P, P, P, L, P]),
+    'at_attention_bwd_workspace_bytes': (L, [P]),
+    'at_attention_bwd': (I, [P, P, P, P, P, P, P, P, P, P, P, P, L, P]),
+    'at_rotary': (I, [P, P, P, P, P, P, P, P, P]),
 }
 
 _lib: Optional[ctypes.CDLL] = None

@@ -1,0 +1,274 @@
+// Building blocks shared by the attention kernels: arguments, the visibility rule, LDS tiles and
+// matrix-core fragments.
+//
+// Rows.  The query heads that share a key head are folded into one list of rows: row r of a
+// key head is token r / group of query head r % group.  The rows of a tile then span few
+// tokens, so a window or a causal edge wastes little of a tile, and one pass over the keys
+// serves every query head that shares them.
+//
+// Visibility.  A sequence has `len` tokens; its first row is token `start`, and `live` rows are
+// tokens of it (the others are padding).  Row of token p sees key j < len when j lies in
+// [p - left, p + right] or j is one of the first `sinks` (and j <= p where causal).
+#pragma once
+
+#include "at_mfma.h"
+
+namespace at_hip {
+
+constexpr float kLog2E = 1.4426950408889634f;
+constexpr int kFar = 1 << 30;          // more than any distance between two tokens
+
+struct Strided {                       // [batch, head, token, dim] tensor; strides in bytes
+  char* p;
+  int64_t batch, head, token;
+};
+
+struct AttentionArgs {
+  Strided q, k, v, out, dout, dq, dk, dv;
+  char* rest;                          // nullable; out before its rounding minus out, in out's layout and type
+  float* lse;                          // [batch * kv_heads][row_pitch]: log2 of the row's sum of exponentials
+  float* delta;                        // backward, same layout: sum over dim of output * output_grad
+  float* part;                         // forward in splits: unreduced outputs [split][batch * kv_heads][rows][dim], fp32
+  float* part_lse;                     // and their log2 sums [split][batch * kv_heads][row_pitch]
+  const void* lengths;                 // tokens of each sequence, or null: `keys` of all
+  const void* query_lengths;           // live rows of each sequence, or null: `rows` of all
+  int lengths64, causal;
+  int batch, kv_heads, group, rows, keys, dim;
+  int row_pitch, tiles, splits;
+  int left, right, sinks;
+  float scale, scale_log2;
+};
+
+struct Sequence {
+  int len, start, live;
+};
+
+__device__ __forceinline__ int clamp_length(const void* p, int is64, int b, int limit) {
+  if (!p) return limit;
+  const int64_t n = is64 ? reinterpret_cast<const int64_t*>(p)[b] : (int64_t)reinterpret_cast<const int*>(p)[b];
+  return (int)(n < 0 ? 0 : n > limit ? limit : n);
+}
+
+__device__ __forceinline__ Sequence sequence_of(const AttentionArgs& a, int b) {
+  Sequence s;
+  s.len = clamp_length(a.lengths, a.lengths64, b, a.keys);
+  const int rows = clamp_length(a.query_lengths, a.lengths64, b, a.rows);
+  s.start = s.len > rows ? s.len - rows : 0;
+  s.live = s.len < rows ? s.len : rows;
+  return s;
+}
+
+// Keys that some row of the tokens [first, last] sees: [lo, hi) and the first `sinks`.
+struct KeyRange {
+  int lo, hi, sinks;
+  __device__ __forceinline__ bool has(int key) const { return (key >= lo && key < hi) || key < sinks; }
+};
+
+__device__ __forceinline__ KeyRange keys_of(const AttentionArgs& a, const Sequence& s, int first, int last) {
+  KeyRange r;
+  r.lo = max(first - a.left, 0);
+  r.hi = min(last + a.right + 1, s.len);
+  r.sinks = min(a.sinks, a.causal ? last + 1 : s.len);
+  return r;
+}
+
+// ---- matrix-core fragments --------------------------------------------------------------------
+// A fragment holds 8 contraction elements of one row (lane % 32) per lane.  In "row" order they are
+// the elements 8 h .. 8 h + 7 of a step of 16 (h = lane / 32); in "accumulator" order they are
+// the elements 4 h .. 4 h + 3 and 8 + 4 h .. 8 + 4 h + 3, which is how a 32 x 32 result leaves the
+// matrix cores: a result whose rows are contracted next is then an operand as it stands, and only
+// the other operand's reads have to follow the order (a contraction may be summed in any order).
+template <typename T> struct Frag {
+  typedef uint4 type;
+  static __device__ __forceinline__ type zero() { return make_uint4(0u, 0u, 0u, 0u); }
+  static __device__ __forceinline__ type load(const char* p) { return *reinterpret_cast<const uint4*>(p); }
+  static __device__ __forceinline__ type pack(const float (&f)[8]) { return pack16<T>(f); }
+  static __device__ __forceinline__ void unpack(const type& x, float (&f)[8]) { unpack16<T>(x, f); }
+  static __device__ __forceinline__ f32x16 mma(const type& x, const type& y, f32x16 c) { return Mfma16<T>::run(x, y, c); }
+};
+struct Frag32 { float e[8]; };
+template <> struct Frag<float> {
+  typedef Frag32 type;
+  static __device__ __forceinline__ type zero() { return type{{0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f}}; }
+  static __device__ __forceinline__ type load(const char* p) {
+    const float4 a = reinterpret_cast<const float4*>(p)[0], b = reinterpret_cast<const float4*>(p)[1];
+    return type{{a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w}};
+  }
+  static __device__ __forceinline__ type pack(const float (&f)[8]) {
+    return type{{f[0], f[1], f[2], f[3], f[4], f[5], f[6], f[7]}};
+  }
+  static __device__ __forceinline__ void unpack(const type& x, float (&f)[8]) {
+#pragma unroll
+    for (int j = 0; j < 8; ++j) f[j] = x.e[j];
+  }
+  // eight steps of two elements each: element j of either half, in whatever order the fragments are
+  static __device__ __forceinline__ f32x16 mma(const type& x, const type& y, f32x16 c) {
+#pragma unroll
+    for (int j = 0; j < 8; ++j) c = __builtin_amdgcn_mfma_f32_32x32x2f32(x.e[j], y.e[j], c, 0, 0, 0);
+    return c;
+  }
+};
+
+// Probabilities of fp16 inputs are multiplied by 2^15 before they are rounded to fp16 (they are at
+// most 1, so nothing overflows): without it those of a long flat row would be subnormal numbers.
+// bf16 has fp32's exponents and needs no such factor.
+template <typename T> struct ProbShift { static constexpr float value = 0.f; };
+template <> struct ProbShift<f16_t> { static constexpr float value = 15.f; };
+
+__device__ __forceinline__ f32x16 zero_acc() {
+  f32x16 z;
+#pragma unroll
+  for (int e = 0; e < 16; ++e) z[e] = 0.f;
+  return z;
+}
+
+// Value of the lane whose number differs by 32, combined with this lane's.
+__device__ __forceinline__ float half_max(float v) {
+  const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+  return fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1]));
+}
+__device__ __forceinline__ float half_sum(float v) {
+  const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+  return __uint_as_float(r[0]) + __uint_as_float(r[1]);
+}
+
+// Row of a 32 x 32 result that register e of this lane holds.
+__device__ __forceinline__ int acc_row(int e, int half) { return (e >> 2) * 8 + half * 4 + (e & 3); }
+
+// ---- tiles in LDS -------------------------------------------------------------------------
+// [ROWS][dim] tile, dim padded with zeros to DT * 32 elements, rows of 64 (DT <= 2) or 128 elements.
+// The 16-byte chunks of a row are permuted by an XOR with spread(row) so that both kinds of
+// fragment reads touch all banks: 8 consecutive rows at one chunk (row order) as well as 4
+// consecutive rows at two neighbouring chunks (transposed reads).
+template <typename T, int DT> struct Tile {
+  static constexpr int kPitch = (DT <= 2 ? 64 : 128) * (int)sizeof(T);
+  static constexpr int kChunks = kPitch / 16;
+  static constexpr int kSteps = 2 * DT;             // contraction steps of 16 over dim
+
+  static __device__ __forceinline__ int spread(int row) {
+    return ((row & 3) << 1) | ((row >> 2) & 1) | (kChunks >= 16 ? (row & 8) : 0);
+  }
+  static __device__ __forceinline__ int at(int row, int chunk) { return row * kPitch + ((chunk ^ spread(row)) << 4); }
+
+  // Rows `row_base` + lane % 32, elements 16 step .. 16 step + 15, row order.
+  static __device__ __forceinline__ typename Frag<T>::type rows_frag(const char* tile, int row_base, int step) {
+    const int lane = threadIdx.x & 63, row = lane & 31, half = lane >> 5;
+    const char* base = tile + row_base * kPitch;
+    if constexpr (sizeof(T) == 2) {
+      return *reinterpret_cast<const uint4*>(base + at(row, step * 2 + half));
+    } else {
+      const float4 a = *reinterpret_cast<const float4*>(base + at(row, step * 4 + half * 2));
+      const float4 b = *reinterpret_cast<const float4*>(base + at(row, step * 4 + half * 2 + 1));
+      return Frag32{{a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w}};
+    }
+  }
+
+  // Elements (columns) 32 dt + lane % 32 as rows, tile rows `row_base` .. + 15 as contraction in
+  // accumulator order.  16-bit elements are transposed by the reads themselves
+  // (ds_read_b64_tr_b16: within 16 lanes, result[l][e] = source[4 e + l / 4][l % 4]).
+  static __device__ __forceinline__ typename Frag<T>::type cols_frag(const char* tile, int row_base, int dt) {
+    const int lane = threadIdx.x & 63, half = lane >> 5;
+    const char* base = tile + row_base * kPitch;
+    if constexpr (sizeof(T) == 2) {
+      const int i = lane & 15;
+      const int chunk = dt * 4 + ((lane >> 4) & 1) * 2 + ((i & 3) >> 1);
+      const int row = half * 4 + (i >> 2);
+      const char* p0 = base + at(row, chunk) + (i & 1) * 8;
+      const char* p1 = base + at(row + 8, chunk) + (i & 1) * 8;
+      typedef __attribute__((address_space(3))) s16x4 lds_s16x4;
+      const uint2 a = __builtin_bit_cast(uint2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)p0));
+      const uint2 b = __builtin_bit_cast(uint2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)p1));
+      return make_uint4(a.x, a.y, b.x, b.y);
+    } else {
+      const int col = dt * 32 + (lane & 31);
+      Frag32 f;
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        const int row = (j < 4 ? 0 : 8) + half * 4 + (j & 3);
+        f.e[j] = *reinterpret_cast<const float*>(base + at(row, col >> 2) + (col & 3) * 4);
+      }
+      return f;
+    }
+  }
+
+  // Asynchronous copy of ROWS rows into `tile`, shared among NW waves.  offset(row) is the row's byte
+  // offset from the resource's base, negative for a row that is to be zeros.
+  template <int ROWS, int NW, typename Offset>
+  static __device__ __forceinline__ void fetch(const i32x4& rsrc, int dim_bytes, char* tile, Offset&& offset) {
+    constexpr int kLoads = ROWS * kPitch / 1024;
+    static_assert(kLoads % NW == 0, "every wave issues the same number of loads");
+    const int lane = threadIdx.x & 63;
+    const int wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
+#pragma unroll
+    for (int n = 0; n < kLoads / NW; ++n) {
+      const int load = n * NW + wave;
+      const int index = load * 64 + lane;
+      const int row = index / kChunks;
+      const int byte = ((index % kChunks) ^ spread(row)) << 4;
+      const int off = offset(row);
+      lds_dma_16(rsrc, off >= 0 && byte < dim_bytes ? off + byte : kOobOffset, tile + load * 1024);
+    }
+  }
+};
+
+// Resource of everything from `base` on; rows that must not be read get kOobOffset.
+__device__ __forceinline__ i32x4 open_rsrc(const char* base) {
+  i32x4 r = make_buffer_rsrc(base, 0x7fffffff);
+  r.x = __builtin_amdgcn_readfirstlane(r.x);
+  r.y = __builtin_amdgcn_readfirstlane(r.y);
+  return r;
+}
+
+// ---- host side ----------------------------------------------------------------------------
+constexpr int kRowAlign = 64;          // rows of lse and delta are padded to whole tiles
+
+inline bool grid_fits(int64_t workgroups) { return workgroups < ((int64_t)1 << 24); }   // 256 threads each, 32-bit grid
+
+// Checks the shape and fills the arguments that do not depend on the pointers.
+inline int attention_args(const at_attention_t* s, AttentionArgs& a) {
+  if (!s) return AT_ERR_NULL;
+  if (!dtype_valid(s->dtype)) return AT_ERR_DTYPE;
+  const int64_t limit = (int64_t)1 << 29;
+  if (s->batch < 0 || s->batch > 65535 || s->kv_heads <= 0 || s->kv_heads > 65535 || s->heads <= 0 || s->heads > 65535 ||
+      s->heads % s->kv_heads != 0 || s->rows < 0 || s->keys < s->rows || s->keys > limit || s->dim <= 0 || s->dim > 128 ||
+      s->window < 0 || s->sinks < 0)
+    return AT_ERR_DIM;
+  if (!(s->scale > 0.f) || s->scale > 3e38f) return AT_ERR_DIM;
+  if (s->dim % 8 != 0) return AT_ERR_ALIGN;
+  a = AttentionArgs{};
+  a.batch = (int)s->batch;
+  a.kv_heads = (int)s->kv_heads;
+  a.group = (int)(s->heads / s->kv_heads);
+  a.rows = (int)s->rows;
+  a.keys = (int)s->keys;
+  a.dim = (int)s->dim;
+  if (s->rows * a.group > limit) return AT_ERR_DIM;
+  a.row_pitch = (int)(cdiv64(s->rows * a.group, kRowAlign) * kRowAlign);
+  const int64_t reach = s->window > 0 && s->window - 1 < s->keys ? s->window - 1 : s->keys;
+  a.left = (int)reach;
+  a.right = s->causal ? 0 : (int)reach;
+  a.sinks = (int)(s->sinks < s->keys ? s->sinks : s->keys);
+  a.causal = s->causal != 0;
+  a.scale = s->scale;
+  a.scale_log2 = s->scale * kLog2E;
+  a.lengths = s->lengths;
+  a.query_lengths = s->query_lengths;
+  a.lengths64 = s->lengths_int64;
+  const int size = dtype_size(s->dtype);
+  Strided* const views[8] = {&a.q, &a.k, &a.v, &a.out, &a.dout, &a.dq, &a.dk, &a.dv};
+  for (int n = 0; n < 8; ++n) {
+    const int64_t* st = s->strides[n];
+    for (int j = 0; j < 3; ++j) {
+      if (st[j] < 0 || st[j] > ((int64_t)1 << 56)) return AT_ERR_DIM;
+      if (st[j] * size % 16 != 0) return AT_ERR_ALIGN;
+    }
+    *views[n] = Strided{nullptr, st[0] * size, st[1] * size, st[2] * size};
+    // a tile is read with 32-bit offsets from its first token
+    const bool heads_in_tile = n == 0 || n == 4;
+    const double span = 160.0 * (double)(st[2] * size) + (heads_in_tile ? (double)(a.group - 1) * (double)(st[1] * size) : 0.0);
+    if (n < 3 || n == 4) { if (span >= 2147483000.0) return AT_ERR_DIM; }
+  }
+  return AT_OK;
+}
+
+}  // namespace at_hip

@@ -1,0 +1,387 @@
+// Attention over a sliding window with first tokens that stay visible: backward pass.
+//
+//   p_ij  = exp(s_ij - lse_i)             dv_j = sum_i p_ij do_i
+//   ds_ij = p_ij (do_i . v_j - delta_i)   delta_i = do_i . out_i
+//   dq_i  = scale sum_j ds_ij k_j         dk_j = scale sum_i ds_ij q_i
+//
+// Two kernels, each of which owns what it sums: the first walks over the keys for a tile of rows (dq, and
+// delta for the second), the second over the rows for a tile of keys (dk, dv).  The scores are formed
+// twice, and no sum crosses workgroups: results do not depend on the order in which they run.
+//
+// delta is taken from the output before its rounding (the forward pass keeps what the rounding left
+// over): an error of delta is common to a whole row of ds, and with the rounded output it was the largest
+// one in dq and dk (bf16, 512 tokens: 2.0e-3 of them against 1.7e-3 for rounding ds).
+#include "attention.h"
+
+namespace at_hip {
+namespace {
+
+constexpr int kWaves = 4;
+constexpr int kTileRows = 32 * kWaves;   // rows (dq) or keys (dk, dv) that a workgroup owns
+constexpr int kStep = 64;                // keys or rows of a tile it walks over
+
+template <typename T, int DT>
+__global__ __launch_bounds__(kWaves * 64, sizeof(T) == 2 ? 2 : 1) void attention_dq_kernel(AttentionArgs a) {
+  typedef Tile<T, DT> L;
+  typedef typename Frag<T>::type F;
+  constexpr int kTileBytes = kStep * L::kPitch;
+  __shared__ __attribute__((aligned(1024))) char lds[4 * kTileBytes];   // two stages of keys | values
+
+  const int lane = threadIdx.x & 63, half = lane >> 5;
+  const int wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
+  const int tile_id = a.tiles - 1 - (int)(blockIdx.x % a.tiles);
+  const int bh = blockIdx.x / a.tiles;
+  const int b = bh / a.kv_heads, h = bh - b * a.kv_heads;
+  const Sequence seq = sequence_of(a, b);
+  const int live_rows = seq.live * a.group, all_rows = a.rows * a.group;
+  const int row0 = tile_id * kTileRows;
+
+  const int row = row0 + wave * 32 + (lane & 31);
+  const int i = row / a.group, g = row - i * a.group;
+  const bool valid = row < live_rows;
+  const int head = h * a.group + g;
+
+  F qf[L::kSteps], df[L::kSteps];
+  float delta = 0.f;
+  {
+    const char* qp = a.q.p + b * a.q.batch + head * a.q.head + i * a.q.token;
+    const char* dp = a.dout.p + b * a.dout.batch + head * a.dout.head + i * a.dout.token;
+    const int64_t at = b * a.out.batch + head * a.out.head + i * a.out.token;
+    const char *op = a.out.p + at, *rp = a.rest + at;
+#pragma unroll
+    for (int s = 0; s < L::kSteps; ++s) {
+      const int d = s * 16 + half * 8;
+      const bool in = valid && d < a.dim;
+      qf[s] = in ? Frag<T>::load(qp + d * sizeof(T)) : Frag<T>::zero();
+      df[s] = in ? Frag<T>::load(dp + d * sizeof(T)) : Frag<T>::zero();
+      const F of = in ? Frag<T>::load(op + d * sizeof(T)) : Frag<T>::zero();
+      float x[8], y[8];
+      Frag<T>::unpack(df[s], x);
+      Frag<T>::unpack(of, y);
+#pragma unroll
+      for (int e = 0; e < 8; ++e) delta = fmaf(x[e], y[e], delta);
+      if (sizeof(T) == 2 && a.rest) {
+        Frag<T>::unpack(in ? Frag<T>::load(rp + d * sizeof(T)) : Frag<T>::zero(), y);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) delta = fmaf(x[e], y[e], delta);
+      }
+    }
+  }
+  delta = half_sum(delta);
+  float lse = INFINITY;
+  if (row < a.row_pitch) {
+    lse = a.lse[(int64_t)bh * a.row_pitch + row];
+    if (half == 0) a.delta[(int64_t)bh * a.row_pitch + row] = delta;
+  }
+
+  f32x16 dq[DT];
+#pragma unroll
+  for (int dt = 0; dt < DT; ++dt) dq[dt] = zero_acc();
+
+  const int p = seq.start + i;
+  const int see_lo = valid ? p - a.left : 1, see_hi = valid ? min(p + a.right, seq.len - 1) : 0;
+  const int see_sinks = valid ? min(a.sinks, a.causal ? p + 1 : seq.len) : 0;
+  const int wrow0 = row0 + wave * 32;
+  const int first = seq.start + wrow0 / a.group;
+  const int last = wrow0 < live_rows ? seq.start + (min(wrow0 + 32, live_rows) - 1) / a.group : first - 1;
+  const KeyRange mine = keys_of(a, seq, first, last);
+
+  int tiles_lo = 0, sink_tiles = 0, tiles = 0;
+  KeyRange range = {0, 0, 0};
+  if (row0 < live_rows) {
+    range = keys_of(a, seq, seq.start + row0 / a.group, seq.start + (min(row0 + kTileRows, live_rows) - 1) / a.group);
+    tiles_lo = range.lo / kStep;
+    sink_tiles = min((range.sinks + kStep - 1) / kStep, tiles_lo);
+    tiles = sink_tiles + (max(range.hi, range.sinks) + kStep - 1) / kStep - tiles_lo;
+  }
+  const char* kb = a.k.p + b * a.k.batch + h * a.k.head;
+  const char* vb = a.v.p + b * a.v.batch + h * a.v.head;
+  const int dim_bytes = a.dim * (int)sizeof(T);
+  auto first_key = [&](int t) { return (t < sink_tiles ? t : t - sink_tiles + tiles_lo) * kStep; };
+  auto fetch = [&](int t, char* stage) {
+    const int k0 = first_key(t);
+    L::template fetch<kStep, kWaves>(open_rsrc(kb + k0 * a.k.token), dim_bytes, stage,
+                                     [&](int r) { return range.has(k0 + r) ? r * (int)a.k.token : -1; });
+    L::template fetch<kStep, kWaves>(open_rsrc(vb + k0 * a.v.token), dim_bytes, stage + kTileBytes,
+                                     [&](int r) { return range.has(k0 + r) ? r * (int)a.v.token : -1; });
+  };
+
+  if (tiles > 0) fetch(0, lds);
+  for (int t = 0; t < tiles; ++t) {
+    char* stage = lds + (t & 1) * 2 * kTileBytes;
+    lds_dma_wait_all();
+    __syncthreads();
+    if (t + 1 < tiles) fetch(t + 1, lds + ((t + 1) & 1) * 2 * kTileBytes);
+    const int k0 = first_key(t);
+    if (!((k0 < mine.hi && k0 + kStep > mine.lo) || k0 < mine.sinks) || last < first) continue;
+    const bool whole = k0 >= last - a.left && k0 + kStep - 1 <= min(first + a.right, seq.len - 1);
+
+#pragma unroll
+    for (int n = 0; n < kStep / 32; ++n) {
+      f32x16 s = zero_acc(), dp = zero_acc();
+#pragma unroll
+      for (int ks = 0; ks < L::kSteps; ++ks) {
+        s = Frag<T>::mma(L::rows_frag(stage, n * 32, ks), qf[ks], s);
+        dp = Frag<T>::mma(L::rows_frag(stage + kTileBytes, n * 32, ks), df[ks], dp);
+      }
+#pragma unroll
+      for (int e = 0; e < 16; ++e) {
+        const int key = k0 + n * 32 + acc_row(e, half);
+        const bool seen = whole || (key >= see_lo && key <= see_hi) || key < see_sinks;
+        const float pr = __builtin_amdgcn_exp2f(fmaf(s[e], a.scale_log2, -lse));
+        s[e] = seen ? pr * (dp[e] - delta) : 0.f;
+      }
+#pragma unroll
+      for (int t16 = 0; t16 < 2; ++t16) {
+        float x[8];
+#pragma unroll
+        for (int e = 0; e < 8; ++e) x[e] = s[t16 * 8 + e];
+        const F ds = Frag<T>::pack(x);
+#pragma unroll
+        for (int dt = 0; dt < DT; ++dt)
+          dq[dt] = Frag<T>::mma(L::cols_frag(stage, n * 32 + t16 * 16, dt), ds, dq[dt]);
+      }
+    }
+  }
+
+  if (row >= all_rows) return;
+  char* gp = a.dq.p + b * a.dq.batch + head * a.dq.head + i * a.dq.token;
+#pragma unroll
+  for (int dt = 0; dt < DT; ++dt)
+#pragma unroll
+    for (int q = 0; q < 4; ++q) {
+      const int d = dt * 32 + q * 8 + half * 4;
+      const float v[4] = {dq[dt][q * 4] * a.scale, dq[dt][q * 4 + 1] * a.scale, dq[dt][q * 4 + 2] * a.scale,
+                          dq[dt][q * 4 + 3] * a.scale};
+      if (d < a.dim) store_f32<T, 4>(reinterpret_cast<T*>(gp) + d, v);
+    }
+}
+
+__device__ __forceinline__ int wave_min(int v) {
+  for (int o = 32; o > 0; o >>= 1) v = min(v, __shfl_xor(v, o, kWave));
+  return __builtin_amdgcn_readfirstlane(v);
+}
+
+template <typename T, int DT>
+__global__ __launch_bounds__(kWaves * 64, sizeof(T) == 2 ? 2 : 1) void attention_dkv_kernel(AttentionArgs a) {
+  typedef Tile<T, DT> L;
+  typedef typename Frag<T>::type F;
+  constexpr int kTileBytes = kStep * L::kPitch;
+  constexpr int kStage = 2 * kTileBytes + 2048;                       // queries | output gradients | lse | delta
+  __shared__ __attribute__((aligned(1024))) char lds[2 * kStage];
+
+  const int lane = threadIdx.x & 63, half = lane >> 5;
+  const int wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
+  const int tile_id = (int)(blockIdx.x % a.tiles);     // the first keys of a causal sequence are seen by the most rows
+  const int bh = blockIdx.x / a.tiles;
+  const int b = bh / a.kv_heads, h = bh - b * a.kv_heads;
+  const Sequence seq = sequence_of(a, b);
+  const int live_rows = seq.live * a.group;
+  const int key0 = tile_id * kTileRows;
+
+  const int key = key0 + wave * 32 + (lane & 31);
+  const bool valid = key < seq.len;
+  F kf[L::kSteps], vf[L::kSteps];
+  {
+    const char* kp = a.k.p + b * a.k.batch + h * a.k.head + key * a.k.token;
+    const char* vp = a.v.p + b * a.v.batch + h * a.v.head + key * a.v.token;
+#pragma unroll
+    for (int s = 0; s < L::kSteps; ++s) {
+      const int d = s * 16 + half * 8;
+      const bool in = valid && d < a.dim;
+      kf[s] = in ? Frag<T>::load(kp + d * sizeof(T)) : Frag<T>::zero();
+      vf[s] = in ? Frag<T>::load(vp + d * sizeof(T)) : Frag<T>::zero();
+    }
+  }
+  f32x16 dk[DT], dv[DT];
+#pragma unroll
+  for (int dt = 0; dt < DT; ++dt) dk[dt] = dv[dt] = zero_acc();
+
+  // rows [row_lo, row_hi] that see this lane's key
+  int row_lo = 1 << 30, row_hi = -1;
+  if (valid) {
+    const bool sink = key < a.sinks;
+    const int tok_lo = !a.causal && sink ? seq.start : max(key - a.right, seq.start);
+    const int tok_hi = sink ? seq.len - 1 : min(key + a.left, seq.len - 1);
+    if (tok_lo <= tok_hi) {
+      row_lo = (tok_lo - seq.start) * a.group;
+      row_hi = min((tok_hi - seq.start) * a.group + a.group, live_rows) - 1;
+    }
+  }
+  // rows that some key of the wave, and that every key of it, is seen by
+  const int any_lo = wave_min(row_lo), any_hi = -wave_min(-row_hi);
+  const int all_lo = -wave_min(-row_lo), all_hi = wave_min(row_hi);
+  __shared__ int ranges[2 * kWaves];
+  if (lane == 0) {
+    ranges[wave] = any_lo;
+    ranges[kWaves + wave] = any_hi;
+  }
+  __syncthreads();
+  int begin = ranges[0], end = ranges[kWaves];
+#pragma unroll
+  for (int w = 1; w < kWaves; ++w) {
+    begin = min(begin, ranges[w]);
+    end = max(end, ranges[kWaves + w]);
+  }
+  begin = __builtin_amdgcn_readfirstlane(begin / kStep);
+  end = __builtin_amdgcn_readfirstlane(end < 0 ? begin : end / kStep + 1);
+
+  const char* qb = a.q.p + b * a.q.batch + (int64_t)h * a.group * a.q.head;
+  const char* db = a.dout.p + b * a.dout.batch + (int64_t)h * a.group * a.dout.head;
+  const float* lse = a.lse + (int64_t)bh * a.row_pitch;
+  const float* delta = a.delta + (int64_t)bh * a.row_pitch;
+  const int dim_bytes = a.dim * (int)sizeof(T);
+  const float per_group = 1.f / (float)a.group;
+  auto fetch = [&](int t, char* stage) {
+    const int r0 = t * kStep;
+    const int i0 = r0 / a.group, rest = r0 - i0 * a.group;
+    // rest + r is small, and the quotient's error far below the 0.5 / group that would change it
+    auto offset = [&](int r, const Strided& x) {
+      const int n = rest + r, token = (int)(((float)n + 0.5f) * per_group);
+      return r0 + r < live_rows ? token * (int)x.token + (n - token * a.group) * (int)x.head : -1;
+    };
+    L::template fetch<kStep, kWaves>(open_rsrc(qb + i0 * a.q.token), dim_bytes, stage,
+                                     [&](int r) { return offset(r, a.q); });
+    L::template fetch<kStep, kWaves>(open_rsrc(db + i0 * a.dout.token), dim_bytes, stage + kTileBytes,
+                                     [&](int r) { return offset(r, a.dout); });
+    if (wave < 2)   // 64 values each: lanes 0..15 move 16 bytes, the others write zeros behind them
+      lds_dma_16(open_rsrc((const char*)((wave == 0 ? lse : delta) + r0)), lane < 16 ? lane * 16 : kOobOffset,
+                 stage + 2 * kTileBytes + wave * 1024);
+  };
+
+  if (begin < end) fetch(begin, lds);
+  for (int t = begin; t < end; ++t) {
+    char* stage = lds + ((t - begin) & 1) * kStage;
+    lds_dma_wait_all();
+    __syncthreads();
+    if (t + 1 < end) fetch(t + 1, lds + ((t + 1 - begin) & 1) * kStage);
+    const float* stats = reinterpret_cast<const float*>(stage + 2 * kTileBytes);
+#pragma unroll
+    for (int n = 0; n < kStep / 32; ++n) {
+      const int r0 = t * kStep + n * 32;
+      if (r0 > any_hi || r0 + 31 < any_lo) continue;
+      const bool whole = r0 >= all_lo && r0 + 31 <= all_hi;
+      f32x16 s = zero_acc(), dp = zero_acc();
+#pragma unroll
+      for (int ks = 0; ks < L::kSteps; ++ks) {
+        s = Frag<T>::mma(L::rows_frag(stage, n * 32, ks), kf[ks], s);
+        dp = Frag<T>::mma(L::rows_frag(stage + kTileBytes, n * 32, ks), vf[ks], dp);
+      }
+#pragma unroll
+      for (int q = 0; q < 4; ++q) {
+        const float4 l4 = *reinterpret_cast<const float4*>(stats + n * 32 + q * 8 + half * 4);
+        const float4 d4 = *reinterpret_cast<const float4*>(stats + 256 + n * 32 + q * 8 + half * 4);
+        const float ls[4] = {l4.x, l4.y, l4.z, l4.w}, de[4] = {d4.x, d4.y, d4.z, d4.w};
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          const int e = q * 4 + j;
+          const int r = r0 + q * 8 + half * 4 + j;
+          const bool seen = whole || (r >= row_lo && r <= row_hi);
+          const float pr = seen ? __builtin_amdgcn_exp2f(fmaf(s[e], a.scale_log2, ProbShift<T>::value - ls[j])) : 0.f;
+          s[e] = pr;
+          dp[e] = seen ? pr * (dp[e] - de[j]) : 0.f;
+        }
+      }
+#pragma unroll
+      for (int t16 = 0; t16 < 2; ++t16) {
+        float x[8], y[8];
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+          x[e] = s[t16 * 8 + e];
+          y[e] = dp[t16 * 8 + e];
+          if (ProbShift<T>::value != 0.f) y[e] *= 1.f / 32768.f;
+        }
+        const F pf = Frag<T>::pack(x), ds = Frag<T>::pack(y);
+#pragma unroll
+        for (int dt = 0; dt < DT; ++dt) {
+          dv[dt] = Frag<T>::mma(L::cols_frag(stage + kTileBytes, n * 32 + t16 * 16, dt), pf, dv[dt]);
+          dk[dt] = Frag<T>::mma(L::cols_frag(stage, n * 32 + t16 * 16, dt), ds, dk[dt]);
+        }
+      }
+    }
+  }
+
+  if (key >= a.keys) return;
+  const float unshift = ProbShift<T>::value != 0.f ? 1.f / 32768.f : 1.f;
+  char* kp = a.dk.p + b * a.dk.batch + h * a.dk.head + key * a.dk.token;
+  char* vp = a.dv.p + b * a.dv.batch + h * a.dv.head + key * a.dv.token;
+#pragma unroll
+  for (int dt = 0; dt < DT; ++dt)
+#pragma unroll
+    for (int q = 0; q < 4; ++q) {
+      const int d = dt * 32 + q * 8 + half * 4;
+      float x[4], y[4];
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        x[j] = dk[dt][q * 4 + j] * a.scale;
+        y[j] = dv[dt][q * 4 + j] * unshift;
+      }
+      if (d < a.dim) {
+        store_f32<T, 4>(reinterpret_cast<T*>(kp) + d, x);
+        store_f32<T, 4>(reinterpret_cast<T*>(vp) + d, y);
+      }
+    }
+}
+
+template <typename T, int DT>
+int launch(AttentionArgs a, hipStream_t stream) {
+  const int64_t heads = (int64_t)a.batch * a.kv_heads;
+  if (!grid_fits(cdiv64((int64_t)a.rows * a.group, kTileRows) * heads) || !grid_fits(cdiv64(a.keys, kTileRows) * heads))
+    return AT_ERR_DIM;
+  if (a.rows > 0) {
+    a.tiles = (int)cdiv64((int64_t)a.rows * a.group, kTileRows);
+    hipLaunchKernelGGL((attention_dq_kernel<T, DT>), dim3((unsigned)(a.tiles * heads)), dim3(kWaves * 64), 0, stream, a);
+    const int rc = launch_status();
+    if (rc != AT_OK) return rc;
+  }
+  a.tiles = (int)cdiv64(a.keys, kTileRows);
+  hipLaunchKernelGGL((attention_dkv_kernel<T, DT>), dim3((unsigned)(a.tiles * heads)), dim3(kWaves * 64), 0, stream, a);
+  return launch_status();
+}
+
+template <typename T>
+int launch_dim(const AttentionArgs& a, hipStream_t stream) {
+  switch ((a.dim + 31) / 32) {
+    case 1: return launch<T, 1>(a, stream);
+    case 2: return launch<T, 2>(a, stream);
+    case 3: return launch<T, 3>(a, stream);
+    default: return launch<T, 4>(a, stream);
+  }
+}
+
+}  // namespace
+}  // namespace at_hip
+
+using namespace at_hip;
+
+extern "C" {
+
+int64_t at_attention_bwd_workspace_bytes(const at_attention_t* shape) {
+  AttentionArgs a;
+  if (attention_args(shape, a) != AT_OK) return 0;
+  return (int64_t)a.batch * a.kv_heads * a.row_pitch * 4;
+}
+
+int at_attention_bwd(const at_attention_t* shape, const void* output_grad, const void* q, const void* k, const void* v,
+                     const void* out, const void* out_rest, const float* lse, void* dq, void* dk, void* dv,
+                     void* workspace, int64_t workspace_bytes, at_stream_t stream) {
+  AttentionArgs a;
+  const int rc = attention_args(shape, a);
+  if (rc != AT_OK) return rc;
+  if (a.batch == 0 || a.keys == 0) return AT_OK;
+  if (!k || !v || !dk || !dv || (a.rows > 0 && (!output_grad || !q || !out || !lse || !dq))) return AT_ERR_NULL;
+  if (!aligned16(q) || !aligned16(k) || !aligned16(v) || !aligned16(out) || !aligned16(output_grad) || !aligned16(dq) ||
+      !aligned16(dk) || !aligned16(dv) || !aligned16(lse) || !aligned16(workspace) || !aligned16(out_rest))
+    return AT_ERR_ALIGN;
+  if (a.rows > 0 && (!workspace || workspace_bytes < at_attention_bwd_workspace_bytes(shape))) return AT_ERR_WORKSPACE;
+  a.q.p = (char*)q; a.k.p = (char*)k; a.v.p = (char*)v; a.out.p = (char*)out; a.dout.p = (char*)output_grad;
+  a.dq.p = (char*)dq; a.dk.p = (char*)dk; a.dv.p = (char*)dv;
+  a.rest = (char*)out_rest;
+  a.lse = const_cast<float*>(lse);
+  a.delta = (float*)workspace;
+  if (shape->dtype == AT_DTYPE_F32) return launch_dim<float>(a, (hipStream_t)stream);
+  if (shape->dtype == AT_DTYPE_F16) return launch_dim<f16_t>(a, (hipStream_t)stream);
+  return launch_dim<bf16_t>(a, (hipStream_t)stream);
+}
+
+}  // extern "C"

@@ -1,0 +1,320 @@
+// Attention over a sliding window with first tokens that stay visible: forward pass.
+//
+//   s_ij = scale q_i . k_j over the visible j,   out_i = sum_j exp(s_ij - m_i) v_j / sum_j exp(s_ij - m_i)
+//
+// in one pass over the keys: the running maximum m_i and the running sum are kept per row, and what
+// was summed before is rescaled when the maximum grows (exponentials in base 2, fp32 throughout;
+// the probabilities are rounded to the inputs' type for the second product only).
+#include "attention.h"
+
+namespace at_hip {
+namespace {
+
+constexpr int kKeys = 64;        // keys of a tile
+constexpr int kWaves = 4;
+constexpr int kRows = 32 * kWaves;
+
+// Four elements of the output, and what their rounding left over where a backward pass will need it.
+template <typename T>
+__device__ __forceinline__ void store_output(const AttentionArgs& a, int64_t to, const float (&v)[4]) {
+  store_f32<T, 4>(reinterpret_cast<T*>(a.out.p + to), v);
+  if constexpr (sizeof(T) == 2) {
+    if (a.rest) {
+      float r[4];
+#pragma unroll
+      for (int j = 0; j < 4; ++j) r[j] = v[j] - to_f32(from_f32<T>(v[j]));
+      store_f32<T, 4>(reinterpret_cast<T*>(a.rest + to), r);
+    }
+  }
+}
+
+template <typename T, int DT>
+__global__ __launch_bounds__(kWaves * 64, sizeof(T) == 2 ? 2 : 1) void attention_fwd_kernel(AttentionArgs a) {
+  typedef Tile<T, DT> L;
+  typedef typename Frag<T>::type F;
+  constexpr int kTileBytes = kKeys * L::kPitch;
+  __shared__ __attribute__((aligned(1024))) char lds[4 * kTileBytes];   // two stages of keys | values
+
+  const int lane = threadIdx.x & 63, half = lane >> 5;
+  const int wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
+  // the last rows of a causal sequence see the most keys: their workgroups start first
+  const int tile_id = a.tiles - 1 - (int)(blockIdx.x % a.tiles);
+  const int bh = blockIdx.x / a.tiles;
+  const int b = bh / a.kv_heads, h = bh - b * a.kv_heads;
+  const Sequence seq = sequence_of(a, b);
+  const int live_rows = seq.live * a.group, all_rows = a.rows * a.group;
+  const int row0 = tile_id * kRows;
+
+  const int row = row0 + wave * 32 + (lane & 31);
+  const int i = row / a.group, g = row - i * a.group;
+  const bool valid = row < live_rows;
+
+  F qf[L::kSteps];
+  {
+    const char* qp = a.q.p + b * a.q.batch + (int64_t)(h * a.group + g) * a.q.head + i * a.q.token;
+#pragma unroll
+    for (int s = 0; s < L::kSteps; ++s) {
+      const int d = s * 16 + half * 8;
+      qf[s] = valid && d < a.dim ? Frag<T>::load(qp + d * sizeof(T)) : Frag<T>::zero();
+    }
+  }
+  f32x16 o[DT];
+#pragma unroll
+  for (int dt = 0; dt < DT; ++dt) o[dt] = zero_acc();
+  float m = -INFINITY, l = 0.f;
+
+  // what this lane's row sees
+  const int p = seq.start + i;
+  const int see_lo = valid ? p - a.left : 1, see_hi = valid ? min(p + a.right, seq.len - 1) : 0;
+  const int see_sinks = valid ? min(a.sinks, a.causal ? p + 1 : seq.len) : 0;
+  // tokens of the wave's rows (last < first: none is live)
+  const int wrow0 = row0 + wave * 32;
+  const int first = seq.start + wrow0 / a.group;
+  const int last = wrow0 < live_rows ? seq.start + (min(wrow0 + 32, live_rows) - 1) / a.group : first - 1;
+  const KeyRange mine = keys_of(a, seq, first, last);
+
+  int tiles_lo = 0, sink_tiles = 0, tiles = 0;
+  KeyRange range = {0, 0, 0};
+  if (row0 < live_rows) {
+    range = keys_of(a, seq, seq.start + row0 / a.group, seq.start + (min(row0 + kRows, live_rows) - 1) / a.group);
+    tiles_lo = range.lo / kKeys;
+    sink_tiles = min((range.sinks + kKeys - 1) / kKeys, tiles_lo);
+    tiles = sink_tiles + (max(range.hi, range.sinks) + kKeys - 1) / kKeys - tiles_lo;
+  }
+  const int split = blockIdx.y;
+  const int t_begin = (int)((int64_t)tiles * split / a.splits), t_end = (int)((int64_t)tiles * (split + 1) / a.splits);
+
+  const char* kb = a.k.p + b * a.k.batch + h * a.k.head;
+  const char* vb = a.v.p + b * a.v.batch + h * a.v.head;
+  const int dim_bytes = a.dim * (int)sizeof(T);
+  auto first_key = [&](int t) { return (t < sink_tiles ? t : t - sink_tiles + tiles_lo) * kKeys; };
+  auto fetch = [&](int t, char* stage) {
+    const int k0 = first_key(t);
+    L::template fetch<kKeys, kWaves>(open_rsrc(kb + k0 * a.k.token), dim_bytes, stage,
+                                     [&](int r) { return range.has(k0 + r) ? r * (int)a.k.token : -1; });
+    L::template fetch<kKeys, kWaves>(open_rsrc(vb + k0 * a.v.token), dim_bytes, stage + kTileBytes,
+                                     [&](int r) { return range.has(k0 + r) ? r * (int)a.v.token : -1; });
+  };
+
+  if (t_begin < t_end) fetch(t_begin, lds);
+  for (int t = t_begin; t < t_end; ++t) {
+    char* stage = lds + ((t - t_begin) & 1) * 2 * kTileBytes;
+    lds_dma_wait_all();
+    __syncthreads();     // tile t is everybody's, and nobody reads the other stage any more
+    if (t + 1 < t_end) fetch(t + 1, lds + ((t - t_begin + 1) & 1) * 2 * kTileBytes);
+    const int k0 = first_key(t);
+    // does any row of the wave see any key of the tile?
+    if (!((k0 < mine.hi && k0 + kKeys > mine.lo) || k0 < mine.sinks) || last < first) continue;
+
+    f32x16 s[2];
+#pragma unroll
+    for (int n = 0; n < 2; ++n) {
+      s[n] = zero_acc();
+#pragma unroll
+      for (int ks = 0; ks < L::kSteps; ++ks) s[n] = Frag<T>::mma(L::rows_frag(stage, n * 32, ks), qf[ks], s[n]);
+    }
+    const bool whole = k0 >= last - a.left && k0 + kKeys - 1 <= min(first + a.right, seq.len - 1);
+    if (whole) {
+#pragma unroll
+      for (int n = 0; n < 2; ++n)
+#pragma unroll
+        for (int e = 0; e < 16; ++e) s[n][e] *= a.scale_log2;
+    } else {
+#pragma unroll
+      for (int n = 0; n < 2; ++n)
+#pragma unroll
+        for (int e = 0; e < 16; ++e) {
+          const int key = k0 + n * 32 + acc_row(e, half);
+          const bool seen = (key >= see_lo && key <= see_hi) || key < see_sinks;
+          s[n][e] = seen ? s[n][e] * a.scale_log2 : -INFINITY;
+        }
+    }
+    float top = s[0][0];
+#pragma unroll
+    for (int n = 0; n < 2; ++n)
+#pragma unroll
+      for (int e = 0; e < 16; ++e) top = fmaxf(top, s[n][e]);
+    top = fmaxf(m, half_max(top));
+    const float base = top == -INFINITY ? 0.f : top - ProbShift<T>::value;   // a row that has seen nothing yet
+    const float shrink = __builtin_amdgcn_exp2f(m - (top == -INFINITY ? 0.f : top));
+    m = top;
+    float sum = 0.f;
+#pragma unroll
+    for (int n = 0; n < 2; ++n)
+#pragma unroll
+      for (int e = 0; e < 16; ++e) {
+        s[n][e] = __builtin_amdgcn_exp2f(s[n][e] - base);
+        sum += s[n][e];
+      }
+    l = l * shrink + sum;
+#pragma unroll
+    for (int dt = 0; dt < DT; ++dt)
+#pragma unroll
+      for (int e = 0; e < 16; ++e) o[dt][e] *= shrink;
+#pragma unroll
+    for (int ks = 0; ks < kKeys / 16; ++ks) {
+      float pr[8];
+#pragma unroll
+      for (int e = 0; e < 8; ++e) pr[e] = s[ks >> 1][(ks & 1) * 8 + e];
+      const F pf = Frag<T>::pack(pr);
+#pragma unroll
+      for (int dt = 0; dt < DT; ++dt)
+        o[dt] = Frag<T>::mma(L::cols_frag(stage + kTileBytes, ks * 16, dt), pf, o[dt]);
+    }
+  }
+
+  l = half_sum(l);
+  const float inv = l > 0.f ? 1.f / l : l == 0.f ? 0.f : l;
+  if (!valid) {          // a padded row, beside which whole tiles were not masked
+    l = 0.f;
+#pragma unroll
+    for (int dt = 0; dt < DT; ++dt) o[dt] = zero_acc();
+  }
+  const float lse = valid ? m + __builtin_amdgcn_logf(l) - ProbShift<T>::value : INFINITY;
+  if (a.splits > 1) {
+    if (row >= all_rows) return;
+    float* part = a.part + (((int64_t)split * a.batch * a.kv_heads + bh) * all_rows + row) * a.dim;
+#pragma unroll
+    for (int dt = 0; dt < DT; ++dt)
+#pragma unroll
+      for (int q = 0; q < 4; ++q) {
+        const int d = dt * 32 + q * 8 + half * 4;
+        if (d < a.dim)
+          *reinterpret_cast<float4*>(part + d) = make_float4(o[dt][q * 4] * inv, o[dt][q * 4 + 1] * inv,
+                                                             o[dt][q * 4 + 2] * inv, o[dt][q * 4 + 3] * inv);
+      }
+    if (half == 0)
+      a.part_lse[((int64_t)split * a.batch * a.kv_heads + bh) * a.row_pitch + row] = l == 0.f ? -INFINITY : lse;
+    return;
+  }
+  if (a.lse && half == 0 && row < a.row_pitch) a.lse[(int64_t)bh * a.row_pitch + row] = lse;
+  if (row >= all_rows) return;
+  const int64_t to = b * a.out.batch + (int64_t)(h * a.group + g) * a.out.head + i * a.out.token;
+#pragma unroll
+  for (int dt = 0; dt < DT; ++dt)
+#pragma unroll
+    for (int q = 0; q < 4; ++q) {
+      const int d = dt * 32 + q * 8 + half * 4;
+      const float v[4] = {o[dt][q * 4] * inv, o[dt][q * 4 + 1] * inv, o[dt][q * 4 + 2] * inv, o[dt][q * 4 + 3] * inv};
+      if (d < a.dim) store_output<T>(a, to + d * (int)sizeof(T), v);
+    }
+}
+
+// Joins the splits of a row: out = sum_s 2^(lse_s - lse) out_s, lse = log2 sum_s 2^lse_s.  32 lanes per
+// row, four elements of dim per lane.
+template <typename T>
+__global__ __launch_bounds__(256) void attention_join_kernel(AttentionArgs a) {
+  const int all_rows = a.rows * a.group;
+  const int64_t at = (int64_t)blockIdx.x * 8 + (threadIdx.x >> 5);
+  const int64_t bhs = (int64_t)a.batch * a.kv_heads;
+  if (at >= bhs * a.row_pitch) return;
+  const int bh = (int)(at / a.row_pitch), row = (int)(at - (int64_t)bh * a.row_pitch);
+  const int b = bh / a.kv_heads, h = bh - b * a.kv_heads;
+  const int i = row / a.group, g = row - i * a.group;
+  const int d = (threadIdx.x & 31) * 4;
+  const bool valid = i < sequence_of(a, b).live;
+  const float* lses = a.part_lse + (int64_t)bh * a.row_pitch + row;
+  float top = -INFINITY, sum = 0.f, v[4] = {0.f, 0.f, 0.f, 0.f};
+  if (valid) {
+    for (int s = 0; s < a.splits; ++s) top = fmaxf(top, lses[s * bhs * a.row_pitch]);
+    if (top == -INFINITY) top = 0.f;
+    for (int s = 0; s < a.splits; ++s) {
+      const float w = __builtin_amdgcn_exp2f(lses[s * bhs * a.row_pitch] - top);
+      sum += w;
+      if (d < a.dim && w != 0.f) {
+        const float4 x = *reinterpret_cast<const float4*>(a.part + ((s * bhs + bh) * all_rows + row) * a.dim + d);
+        v[0] += w * x.x; v[1] += w * x.y; v[2] += w * x.z; v[3] += w * x.w;
+      }
+    }
+    const float inv = sum == 0.f ? 0.f : 1.f / sum;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) v[j] *= inv;
+  }
+  if (row < all_rows && d < a.dim) {
+    store_output<T>(a, b * a.out.batch + (int64_t)(h * a.group + g) * a.out.head + i * a.out.token + d * (int)sizeof(T), v);
+  }
+  if (a.lse && d == 0) a.lse[at] = valid ? top + __builtin_amdgcn_logf(sum) : INFINITY;
+}
+
+// Splits of the keys per tile of rows: none while the tiles alone give every CU two workgroups,
+// otherwise as many as fill two per CU with at least two tiles of keys each.
+int split_count(const AttentionArgs& a) {
+  const int64_t groups = (int64_t)a.tiles * a.batch * a.kv_heads;
+  const int64_t want = 2 * device_cu_count();
+  if (groups >= want || groups == 0) return 1;
+  // keys that one tile of rows can see
+  const int64_t span = (int64_t)a.left + a.right + cdiv64(kRows, a.group) + a.sinks;
+  const int64_t tiles = cdiv64(span < a.keys ? span : a.keys, kKeys);
+  int64_t n = cdiv64(want, groups);
+  if (n > tiles / 2) n = tiles / 2;
+  return (int)(n < 1 ? 1 : n > 128 ? 128 : n);
+}
+
+template <typename T>
+int launch_dim(const AttentionArgs& a, hipStream_t stream) {
+  const int64_t blocks = (int64_t)a.tiles * a.batch * a.kv_heads;
+  if (!grid_fits(blocks) || !grid_fits(cdiv64((int64_t)a.batch * a.kv_heads * a.row_pitch, 8))) return AT_ERR_DIM;
+  const dim3 grid((unsigned)blocks, (unsigned)a.splits), block(kWaves * 64);
+  switch ((a.dim + 31) / 32) {
+    case 1: hipLaunchKernelGGL((attention_fwd_kernel<T, 1>), grid, block, 0, stream, a); break;
+    case 2: hipLaunchKernelGGL((attention_fwd_kernel<T, 2>), grid, block, 0, stream, a); break;
+    case 3: hipLaunchKernelGGL((attention_fwd_kernel<T, 3>), grid, block, 0, stream, a); break;
+    default: hipLaunchKernelGGL((attention_fwd_kernel<T, 4>), grid, block, 0, stream, a); break;
+  }
+  int rc = launch_status();
+  if (rc == AT_OK && a.splits > 1) {
+    const int64_t rows = (int64_t)a.batch * a.kv_heads * a.row_pitch;
+    hipLaunchKernelGGL((attention_join_kernel<T>), dim3((unsigned)cdiv64(rows, 8)), dim3(256), 0, stream, a);
+    rc = launch_status();
+  }
+  return rc;
+}
+
+int64_t part_bytes(const AttentionArgs& a) {
+  if (a.splits <= 1) return 0;
+  return (int64_t)a.splits * a.batch * a.kv_heads * ((int64_t)a.rows * a.group * a.dim + a.row_pitch) * 4;
+}
+
+}  // namespace
+}  // namespace at_hip
+
+using namespace at_hip;
+
+extern "C" {
+
+int64_t at_attention_row_pitch(int64_t rows, int64_t heads, int64_t kv_heads) {
+  if (rows < 0 || heads <= 0 || kv_heads <= 0 || heads % kv_heads != 0) return 0;
+  return cdiv64(rows * (heads / kv_heads), kRowAlign) * kRowAlign;
+}
+
+int64_t at_attention_fwd_workspace_bytes(const at_attention_t* shape) {
+  AttentionArgs a;
+  if (attention_args(shape, a) != AT_OK) return 0;
+  a.tiles = (int)cdiv64((int64_t)a.rows * a.group, kRows);
+  a.splits = split_count(a);
+  return part_bytes(a);
+}
+
+int at_attention_fwd(const at_attention_t* shape, const void* q, const void* k, const void* v, void* out, float* lse,
+                     void* out_rest, void* workspace, int64_t workspace_bytes, at_stream_t stream) {
+  AttentionArgs a;
+  const int rc = attention_args(shape, a);
+  if (rc != AT_OK) return rc;
+  if (a.batch == 0 || a.rows == 0) return AT_OK;
+  if (!q || !out || (a.keys > 0 && (!k || !v))) return AT_ERR_NULL;
+  if (!aligned16(q) || !aligned16(k) || !aligned16(v) || !aligned16(out) || (lse && !aligned16(lse)) || !aligned16(out_rest)) return AT_ERR_ALIGN;
+  a.q.p = (char*)q; a.k.p = (char*)k; a.v.p = (char*)v; a.out.p = (char*)out;
+  a.lse = lse;
+  a.rest = (char*)out_rest;
+  a.tiles = (int)cdiv64((int64_t)a.rows * a.group, kRows);
+  a.splits = split_count(a);
+  const int64_t need = part_bytes(a);
+  if (need > 0 && (!workspace || workspace_bytes < need)) return AT_ERR_WORKSPACE;
+  a.part = (float*)workspace;
+  a.part_lse = a.splits > 1 ? a.part + (int64_t)a.splits * a.batch * a.kv_heads * a.rows * a.group * a.dim : nullptr;
+  if (shape->dtype == AT_DTYPE_F32) return launch_dim<float>(a, (hipStream_t)stream);
+  if (shape->dtype == AT_DTYPE_F16) return launch_dim<f16_t>(a, (hipStream_t)stream);
+  return launch_dim<bf16_t>(a, (hipStream_t)stream);
+}
+
+}  // extern "C"

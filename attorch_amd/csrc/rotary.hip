@@ -1,0 +1,196 @@
+// Rotary positions with one or several axes: pair n of each head's features is turned by the angle
+//   a = positions[axis of n] * inv_freq[n]:   (x, y) -> (x cos a - y sin a, x sin a + y cos a).
+// The gradient is the same map with -a, so one kernel serves both directions.
+//
+// Bound by memory: every feature is read and written once.  A workgroup takes a few tokens, forms the
+// cosines and sines of their angles once in LDS (all heads of a token share them) and then streams
+// the heads of q and k.  The angles are formed in 64 bits and reduced by whole turns there: at
+// position 2^20 an fp32 product would already be off by 0.06 radians.
+#include "at_common.h"
+
+namespace at_hip {
+namespace {
+
+constexpr int kMaxPairs = 512;
+constexpr int kTable = 1024;           // cosine and sine pairs in LDS
+
+struct RotaryArgs {
+  const char* in[2];                   // q, k
+  char* out[2];
+  int64_t in_stride[2][3], out_stride[2][3];   // batch, head, token; bytes
+  const void* positions;
+  const double* inv_freq;
+  const int* pair_axis;
+  int64_t position_strides[3];
+  int64_t tokens;                      // batch * rows
+  int rows, heads, q_heads, dim, pairs, axes, position_type, inverse, group;
+};
+
+__device__ __forceinline__ double position_of(const RotaryArgs& a, int axis, int64_t b, int t) {
+  if (!a.positions) return (double)t;
+  const int64_t at = axis * a.position_strides[0] + b * a.position_strides[1] + t * a.position_strides[2];
+  if (a.position_type == 0) return (double)reinterpret_cast<const int*>(a.positions)[at];
+  if (a.position_type == 1) return (double)reinterpret_cast<const int64_t*>(a.positions)[at];
+  return (double)reinterpret_cast<const float*>(a.positions)[at];
+}
+
+// VEC features per access (1: any size and alignment).
+template <typename T, bool ADJACENT, int VEC>
+__global__ __launch_bounds__(256) void rotary_kernel(RotaryArgs a) {
+  __shared__ float table_cos[kTable], table_sin[kTable];
+  const int64_t first = (int64_t)blockIdx.x * a.group;
+  const int count = (int)(a.tokens - first < a.group ? a.tokens - first : a.group);
+
+  for (int n = threadIdx.x; n < count * a.pairs; n += 256) {
+    const int local = n / a.pairs, pair = n - local * a.pairs;
+    const int64_t b = (first + local) / a.rows;
+    const int t = (int)(first + local - b * a.rows);
+    const int axis = a.pair_axis ? min(max(a.pair_axis[pair], 0), a.axes - 1) : 0;
+    const double turns = position_of(a, axis, b, t) * (a.inv_freq[pair] * 0.15915494309189533577);
+    float s, c;
+    sincospif(2.f * (float)(turns - rint(turns)), &s, &c);
+    table_cos[n] = c;
+    table_sin[n] = a.inverse ? -s : s;
+  }
+  __syncthreads();
+
+  // items of a head: vectors of pairs, then vectors of the features that are only copied
+  constexpr int kWidth = VEC > 1 || !ADJACENT ? VEC : 2;           // features an adjacent item covers
+  const int turned = ADJACENT ? 2 * a.pairs / kWidth : a.pairs / VEC;
+  const int rest = a.dim - 2 * a.pairs;
+  const int items = turned + rest / VEC;
+  for (int local = 0; local < count; ++local) {
+    const int64_t b = (first + local) / a.rows;
+    const int t = (int)(first + local - b * a.rows);
+    const float* cs = table_cos + local * a.pairs;
+    const float* sn = table_sin + local * a.pairs;
+    for (int n = threadIdx.x; n < a.heads * items; n += 256) {
+      int head = n / items;
+      const int item = n - head * items;
+      const int which = head >= a.q_heads;
+      head -= which ? a.q_heads : 0;
+      const T* x = reinterpret_cast<const T*>(a.in[which] + b * a.in_stride[which][0] + head * a.in_stride[which][1] +
+                                              t * a.in_stride[which][2]);
+      T* y = reinterpret_cast<T*>(a.out[which] + b * a.out_stride[which][0] + head * a.out_stride[which][1] +
+                                  t * a.out_stride[which][2]);
+      if (item >= turned) {
+        const int d = 2 * a.pairs + (item - turned) * VEC;
+        float v[VEC];
+        load_f32<T, VEC>(x + d, v);
+        store_f32<T, VEC>(y + d, v);
+      } else if constexpr (ADJACENT) {
+        const int d = item * kWidth;
+        float v[kWidth];
+        if constexpr (VEC > 1) {
+          load_f32<T, kWidth>(x + d, v);
+        } else {
+          v[0] = to_f32(x[d]);
+          v[1] = to_f32(x[d + 1]);
+        }
+#pragma unroll
+        for (int j = 0; j < kWidth; j += 2) {
+          const float c = cs[(d + j) >> 1], s = sn[(d + j) >> 1], u = v[j], w = v[j + 1];
+          v[j] = u * c - w * s;
+          v[j + 1] = u * s + w * c;
+        }
+        if constexpr (VEC > 1) {
+          store_f32<T, kWidth>(y + d, v);
+        } else {
+          y[d] = from_f32<T>(v[0]);
+          y[d + 1] = from_f32<T>(v[1]);
+        }
+      } else {
+        const int d = item * VEC;
+        float u[VEC], w[VEC];
+        load_f32<T, VEC>(x + d, u);
+        load_f32<T, VEC>(x + d + a.pairs, w);
+#pragma unroll
+        for (int j = 0; j < VEC; ++j) {
+          const float c = cs[d + j], s = sn[d + j], p = u[j], q = w[j];
+          u[j] = p * c - q * s;
+          w[j] = p * s + q * c;
+        }
+        store_f32<T, VEC>(y + d, u);
+        store_f32<T, VEC>(y + d + a.pairs, w);
+      }
+    }
+  }
+}
+
+template <typename T>
+int launch(const RotaryArgs& a, bool adjacent, bool vector, hipStream_t stream) {
+  constexpr int VEC = 16 / (int)sizeof(T);
+  const dim3 grid((unsigned)cdiv64(a.tokens, a.group)), block(256);
+  if (adjacent) {
+    if (vector) hipLaunchKernelGGL((rotary_kernel<T, true, VEC>), grid, block, 0, stream, a);
+    else hipLaunchKernelGGL((rotary_kernel<T, true, 1>), grid, block, 0, stream, a);
+  } else {
+    if (vector) hipLaunchKernelGGL((rotary_kernel<T, false, VEC>), grid, block, 0, stream, a);
+    else hipLaunchKernelGGL((rotary_kernel<T, false, 1>), grid, block, 0, stream, a);
+  }
+  return launch_status();
+}
+
+}  // namespace
+}  // namespace at_hip
+
+using namespace at_hip;
+
+extern "C" {
+
+int at_rotary(const at_rotary_t* s, const void* q, const void* k, void* q_out, void* k_out, const void* positions,
+              const double* inv_freq, const int* pair_axis, at_stream_t stream) {
+  if (!s) return AT_ERR_NULL;
+  if (!dtype_valid(s->dtype)) return AT_ERR_DTYPE;
+  const int64_t limit = (int64_t)1 << 30;
+  if (s->batch < 0 || s->rows < 0 || s->q_heads < 0 || s->k_heads < 0 || s->dim <= 0 || s->pairs < 0 || s->axes <= 0 ||
+      s->pairs > kMaxPairs || 2 * s->pairs > s->dim || s->rows > limit || s->batch > limit ||
+      s->position_type < 0 || s->position_type > 2)
+    return AT_ERR_DIM;
+  const int64_t heads = s->q_heads + s->k_heads;
+  if (heads > 65535 || s->dim > 65535 || heads * s->dim > limit) return AT_ERR_DIM;
+  if (s->batch == 0 || s->rows == 0 || heads == 0) return AT_OK;
+  if ((s->q_heads > 0 && (!q || !q_out)) || (s->k_heads > 0 && (!k || !k_out)) || (s->pairs > 0 && !inv_freq) ||
+      (s->axes > 1 && (!positions || (s->pairs > 0 && !pair_axis))))
+    return AT_ERR_NULL;
+  const int size = dtype_size(s->dtype);
+  RotaryArgs a = {};
+  a.in[0] = (const char*)q; a.in[1] = (const char*)k;
+  a.out[0] = (char*)q_out; a.out[1] = (char*)k_out;
+  bool vector = s->dim * size % 16 == 0;
+  for (int n = 0; n < 2; ++n) {
+    if ((n == 0 ? s->q_heads : s->k_heads) == 0) continue;
+    vector = vector && aligned16(a.in[n]) && aligned16(a.out[n]);
+    for (int j = 0; j < 3; ++j) {
+      a.in_stride[n][j] = s->strides[n][j] * size;
+      a.out_stride[n][j] = s->strides[2 + n][j] * size;
+      vector = vector && a.in_stride[n][j] % 16 == 0 && a.out_stride[n][j] % 16 == 0;
+    }
+  }
+  // whole vectors of pairs, and of features in adjacent pairs
+  vector = vector && (s->adjacent ? 2 : 1) * s->pairs * size % 16 == 0;
+  a.positions = positions;
+  a.inv_freq = inv_freq;
+  a.pair_axis = pair_axis;
+  for (int j = 0; j < 3; ++j) a.position_strides[j] = s->position_strides[j];
+  a.tokens = s->batch * s->rows;
+  a.rows = (int)s->rows;
+  a.heads = (int)heads;
+  a.q_heads = (int)s->q_heads;
+  a.dim = (int)s->dim;
+  a.pairs = (int)s->pairs;
+  a.axes = (int)s->axes;
+  a.position_type = s->position_type;
+  a.inverse = s->inverse != 0;
+  // tokens of a workgroup: as many as fill its lanes with angles, as long as every CU keeps several workgroups
+  int group = a.pairs > 0 ? 256 / a.pairs : 4;
+  if (group > 8) group = 8;
+  while (group > 1 && a.tokens / group < 4 * (int64_t)device_cu_count()) group /= 2;
+  a.group = group < 1 ? 1 : group;
+  if (cdiv64(a.tokens, a.group) >= ((int64_t)1 << 24)) return AT_ERR_DIM;
+  if (s->dtype == AT_DTYPE_F32) return launch<float>(a, s->adjacent != 0, vector, (hipStream_t)stream);
+  if (s->dtype == AT_DTYPE_F16) return launch<f16_t>(a, s->adjacent != 0, vector, (hipStream_t)stream);
+  return launch<bf16_t>(a, s->adjacent != 0, vector, (hipStream_t)stream);
+}
+
+}  // extern "C"

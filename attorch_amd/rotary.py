@@ -1,0 +1,248 @@
+"""
+Rotary positions with one or several axes, with PyTorch autodiff support, running on a gfx950
+kernel that turns queries and keys in one launch.
+
+The reference has no counterpart: its example model adds learned absolute positions to the token
+embeddings (examples/wikitext-2/gpt.py:95-110).
+"""
+
+import ctypes
+from typing import Any, Optional, Sequence, Tuple
+
+import torch
+from torch import Tensor
+from torch import nn
+from torch.autograd.function import once_differentiable
+
+from . import _lib
+
+POSITION_TYPES = {torch.int32: 0, torch.int64: 1, torch.float32: 2}
+MAX_PAIRS = 512
+
+
+class _Shape(ctypes.Structure):
+    """
+    at_rotary_t of include/attorch_hip.h.
+    """
+    _fields_ = ([(name, ctypes.c_int64) for name in ('batch', 'rows', 'q_heads', 'k_heads', 'dim', 'pairs', 'axes')] +
+                [('strides', ctypes.c_int64 * 12), ('position_strides', ctypes.c_int64 * 3),
+                 ('position_type', ctypes.c_int), ('adjacent', ctypes.c_int), ('inverse', ctypes.c_int),
+                 ('dtype', ctypes.c_int)])
+
+
+def _features(tensor: Tensor) -> Tensor:
+    """
+    The tensor itself if its features lie side by side, otherwise a copy.
+    """
+    return tensor if tensor.stride(3) == 1 or tensor.shape[3] <= 1 else tensor.contiguous()
+
+
+def _positions_of(positions: Optional[Tensor], axes: int, batch: int, rows: int) -> Optional[Tensor]:
+    """
+    Positions as [axes, batch, rows], without a copy.
+    """
+    if positions is None:
+        if axes > 1:
+            raise RuntimeError(f'Positions with {axes} axes must be given')
+        return None
+    if positions.dtype not in POSITION_TYPES:
+        raise RuntimeError(f'Positions must be int32, int64 or float32, received {positions.dtype}')
+    shape = tuple(positions.shape)
+    if axes == 1 and shape in ((rows,), (batch, rows)):   # (1, rows) means the same as one axis and as one sequence
+        return positions.expand(1, batch, rows)
+    if shape == (axes, rows):
+        return positions.unsqueeze(1).expand(axes, batch, rows)
+    assert shape == (axes, batch, rows), \
+        f'Positions must be of shape {(axes, batch, rows)} or {(axes, rows)}, received {shape}'
+    return positions
+
+
+def _rotate(tensors: Sequence[Optional[Tensor]], positions: Optional[Tensor], inv_freq: Tensor,
+            pair_axis: Optional[Tensor], axes: int, adjacent: bool, inverse: bool) -> Tuple[Optional[Tensor], ...]:
+    """
+    Turns the queries and keys (either may be absent) by their positions' angles, or back.
+    """
+    present = next(t for t in tensors if t is not None)
+    batch, _, rows, dim = present.shape
+    inputs = [None if t is None else _features(t) for t in tensors]
+    outputs = [None if t is None else torch.empty_like(t) for t in inputs]
+    outputs = [t if t is None or t.stride(3) == 1 or dim <= 1 else torch.empty(t.shape, device=t.device, dtype=t.dtype)
+               for t in outputs]
+    strides = []
+    for t in (*inputs, *outputs):
+        strides += (0, 0, 0) if t is None else t.stride()[:3]
+    heads = [0 if t is None else t.shape[1] for t in inputs]
+    shape = _Shape(batch, rows, heads[0], heads[1], dim, inv_freq.shape[0], axes, (ctypes.c_int64 * 12)(*strides),
+                   (ctypes.c_int64 * 3)(*((0, 0, 0) if positions is None else positions.stride())),
+                   0 if positions is None else POSITION_TYPES[positions.dtype], adjacent, inverse,
+                   _lib.dtype_id(present.dtype))
+    with _lib.device_guard(present):
+        _lib.check(_lib.load().at_rotary(
+            ctypes.byref(shape), *(_lib.ptr(t) for t in inputs), *(_lib.ptr(t) for t in outputs), _lib.ptr(positions),
+            _lib.ptr(inv_freq), _lib.ptr(pair_axis), _lib.stream_of(present)), 'at_rotary')
+    return tuple(outputs)
+
+
+class RotaryAutoGrad(torch.autograd.Function):
+    """
+    Autodiff for rotary positions.
+    """
+    @staticmethod
+    def forward(
+        ctx: Any,
+        query: Tensor,
+        key: Optional[Tensor],
+        positions: Optional[Tensor],
+        inv_freq: Tensor,
+        pair_axis: Optional[Tensor] = None,
+        adjacent: bool = False,
+        ) -> Tuple[Tensor, Optional[Tensor]]:
+        """
+        Turns pair n of every head's features by the angle positions[pair_axis[n]] * inv_freq[n]:
+        (x, y) becomes (x cos a - y sin a, x sin a + y cos a).  Features behind the pairs are kept.
+        Angles are formed in 64 bits, so positions may be far.
+
+        Args:
+            query: Queries of shape [batch, heads, rows, head_dim].
+            key: Optional keys of shape [batch, kv_heads, rows, head_dim].
+            positions: Positions of the tokens, int32, int64 or float32: with pair_axis of shape
+                [axes, batch, rows] or [axes, rows], without it [batch, rows], [rows] or
+                [1, batch, rows]. None (without pair_axis): token t of every sequence is at t.
+            inv_freq: Radians per position of each pair, float64, at most head_dim // 2 of them.
+            pair_axis: Optional axis of each pair, int32 of inv_freq's shape (values are clamped to
+                the axes there are). None: one axis.
+            adjacent: Pairs are features (2 n, 2 n + 1) instead of (n, n + pairs).
+
+        Returns:
+            Turned queries and keys (None without keys), of the dtypes of the inputs.
+        """
+        assert query.ndim == 4, f'Queries must be [batch, heads, rows, head_dim], received {tuple(query.shape)}'
+        batch, _, rows, head_dim = query.shape
+        assert key is None or (key.ndim == 4 and key.shape[0] == batch and key.shape[2:] == query.shape[2:]), \
+            f'Incompatible query ({tuple(query.shape)}) and key ({tuple(key.shape)}) shape'
+        if key is not None and key.dtype is not query.dtype:
+            raise RuntimeError(f'Query and key must have the same dtype, received {query.dtype} and {key.dtype}')
+        if inv_freq.dtype is not torch.float64:
+            raise RuntimeError(f'inv_freq must be float64, received {inv_freq.dtype}')
+        assert inv_freq.ndim == 1 and 2 * inv_freq.shape[0] <= head_dim, \
+            f'inv_freq ({tuple(inv_freq.shape)}) must hold at most half the head dimension ({head_dim})'
+        if inv_freq.shape[0] > MAX_PAIRS:
+            raise RuntimeError(f'At most {MAX_PAIRS} pairs are supported, received {inv_freq.shape[0]}')
+        axes = 1
+        if pair_axis is not None:
+            if pair_axis.dtype is not torch.int32:
+                raise RuntimeError(f'pair_axis must be int32, received {pair_axis.dtype}')
+            assert pair_axis.shape == inv_freq.shape, \
+                f'pair_axis ({tuple(pair_axis.shape)}) must have the shape of inv_freq ({tuple(inv_freq.shape)})'
+            assert positions is not None and positions.ndim in (2, 3) and positions.shape[0] > 0, \
+                'Axes of pairs need positions of shape [axes, batch, rows] or [axes, rows]'
+            axes = positions.shape[0]
+        positions = _positions_of(positions, axes, batch, rows)
+        _lib.require_same_device('Rotary', query, key, positions, inv_freq, pair_axis)
+        inv_freq = inv_freq.contiguous()
+        pair_axis = None if pair_axis is None else pair_axis.contiguous()
+
+        outputs = _rotate((query, key), positions, inv_freq, pair_axis, axes, bool(adjacent), False)
+        ctx.options = (axes, bool(adjacent))
+        ctx.save_for_backward(positions, inv_freq, pair_axis)
+        ctx.set_materialize_grads(False)
+        return outputs
+
+    @staticmethod
+    @once_differentiable
+    def backward(
+        ctx: Any,
+        query_grad: Optional[Tensor],
+        key_grad: Optional[Tensor] = None,
+        ) -> Tuple[Optional[Tensor], ...]:
+        """
+        Gradients of the queries and keys: the outputs' gradients, turned back.
+        """
+        positions, inv_freq, pair_axis = ctx.saved_tensors
+        grads = [query_grad if ctx.needs_input_grad[0] else None, key_grad if ctx.needs_input_grad[1] else None]
+        if grads[0] is not None or grads[1] is not None:
+            _lib.require_same_device('Rotary backward', inv_freq, *grads)
+            axes, adjacent = ctx.options
+            grads = _rotate(grads, positions, inv_freq, pair_axis, axes, adjacent, True)
+
+        # One gradient (or None) per forward argument.
+        return grads[0], grads[1], None, None, None, None
+
+
+class Rotary(nn.Module):
+    """
+    Rotary positions with one or several axes (time, height and width of a video's patches, say)
+    for queries and keys; it has no parameters.  The tables of frequencies and axes are kept as
+    buffers that follow the module from device to device; a change of the module's dtype leaves
+    them as they are.
+
+    Args:
+        head_dim: Size of a head.
+        sections: Number of pairs of each axis, in order; None selects one axis with all pairs.
+        rotary_dim: Number of features to turn (an even one); None selects twice the sections'
+            sum, or head_dim.
+        base: Base of the frequencies: pair n of N turns by base ** (-n / N) radians per position.
+        axis_ladders: Every axis has frequencies of its own (n counts within its section, and N is
+            the section's size) instead of sharing one ladder over all pairs.
+        adjacent: Pairs are features (2 n, 2 n + 1) instead of (n, n + rotary_dim / 2).
+        device: Device to use.
+    """
+    def __init__(
+        self,
+        head_dim: int,
+        sections: Optional[Sequence[int]] = None,
+        rotary_dim: Optional[int] = None,
+        base: float = 10000.0,
+        axis_ladders: bool = False,
+        adjacent: bool = False,
+        device: Any = 'cuda',
+        ) -> None:
+        super().__init__()
+        if rotary_dim is None:
+            rotary_dim = 2 * sum(sections) if sections is not None else head_dim
+        if rotary_dim % 2 != 0 or not 0 <= rotary_dim <= head_dim:
+            raise RuntimeError(f'The rotary dimension must be even and at most {head_dim}, received {rotary_dim}')
+        pairs = rotary_dim // 2
+        sections = (pairs,) if sections is None else tuple(sections)
+        if len(sections) == 0 or min(sections) < 0 or sum(sections) != pairs:
+            raise RuntimeError(f'Sections {sections} must sum to half the rotary dimension ({pairs})')
+        if not base > 0.0:
+            raise RuntimeError(f'The base must be positive, received {base}')
+        if pairs > MAX_PAIRS:
+            raise RuntimeError(f'At most {MAX_PAIRS} pairs are supported, received {pairs}')
+
+        self.head_dim = head_dim
+        self.sections = sections
+        self.base = base
+        self.axis_ladders = axis_ladders
+        self.adjacent = adjacent
+        ladders = [[n / size for n in range(size)] for size in sections] if axis_ladders else \
+            [[n / max(pairs, 1) for n in range(pairs)]]
+        inv_freq = torch.tensor([base ** -step for ladder in ladders for step in ladder], dtype=torch.float64)
+        pair_axis = torch.tensor([axis for axis, size in enumerate(sections) for _ in range(size)], dtype=torch.int32)
+        # kept as the bits of the float64 values: module.to(torch.bfloat16) casts floating-point buffers
+        self.register_buffer('inv_freq_bits', inv_freq.view(torch.int64).to(device), persistent=False)
+        self.register_buffer('pair_axis', pair_axis.to(device), persistent=False)
+
+    @property
+    def inv_freq(self) -> Tensor:
+        return self.inv_freq_bits.view(torch.float64)
+
+    def forward(
+        self,
+        query: Tensor,
+        key: Optional[Tensor] = None,
+        positions: Optional[Tensor] = None,
+        ) -> Tuple[Tensor, Optional[Tensor]]:
+        if query.shape[-1] != self.head_dim:
+            raise RuntimeError(f'Expected heads of size {self.head_dim}, received {query.shape[-1]}')
+        axes = len(self.sections)
+        if axes > 1 or positions is not None:
+            assert query.ndim == 4, f'Queries must be [batch, heads, rows, head_dim], received {tuple(query.shape)}'
+            positions = _positions_of(positions, axes, query.shape[0], query.shape[2])
+        return RotaryAutoGrad.apply(query, key, positions, self.inv_freq, self.pair_axis if axes > 1 else None,
+                                    self.adjacent)
+
+    def extra_repr(self) -> str:
+        return (f'{self.head_dim}, sections={self.sections}, base={self.base}, axis_ladders={self.axis_ladders}, '
+                f'adjacent={self.adjacent}')

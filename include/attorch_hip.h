@@ -584,6 +584,73 @@ int at_act_dropout_bwd(const void* output_grad, const void* input, void* input_g
                        int64_t size, int act, float param, float drop_p, uint32_t seed,
                        int dtype, at_stream_t stream);
 
+/* ------------------------------------------------------------------------------------------
+ * Attention over a sliding window with a few first tokens that stay visible (the reference's own
+ * attention layer, attorch/multi_head_attention_layer.py:77, cannot be constructed).
+ * Tensors are [batch, heads, tokens, dim] with any strides (elements; multiples of 16 bytes) and
+ * unit stride along dim; dim is a multiple of 8 and at most 128.  `heads` is a multiple of
+ * `kv_heads`: query head n reads key head n / (heads / kv_heads).
+ *   lengths[b]        tokens of sequence b, clamped to [0, keys]; null: keys
+ *   query_lengths[b]  rows of it that are tokens, clamped to [0, rows]; null: rows
+ * With L and Q these two, row i is token p = max(L - Q, 0) + i; rows with i >= Q or p >= L are
+ * padding: their output and gradients are zeros.  Row i sees key j < L when j <= p (or not causal)
+ * and |p - j| < window (or window = 0, or j < sinks).  Key, value, query and output_grad rows that
+ * nothing sees are not read into any result, whatever they hold.
+ *   fwd: out = softmax(scale q k^T) v; lse (nullable; batch * kv_heads * at_attention_row_pitch
+ *        floats) keeps what the backward pass needs, and so does out_rest (nullable, in out's layout
+ *        and type): what the rounding of out to 16 bits left over
+ *   bwd: gradients of q, k and v from output_grad, the forward pass's inputs, output and lse
+ * The workspaces have the queried sizes (0: none wanted); strides[] is in the order q, k, v, out,
+ * output_grad, dq, dk, dv (forward: the first four, the others 0).
+ * ------------------------------------------------------------------------------------------ */
+typedef struct at_attention {
+  int64_t batch, heads, kv_heads, rows, keys, dim;
+  int64_t window, sinks;
+  int64_t strides[8][3];          /* batch, head, token */
+  const void* lengths;            /* device, nullable */
+  const void* query_lengths;      /* device, nullable */
+  float scale;
+  int causal;
+  int dtype;
+  int lengths_int64;              /* lengths and query_lengths are int64 (otherwise int32) */
+} at_attention_t;
+
+int64_t at_attention_row_pitch(int64_t rows, int64_t heads, int64_t kv_heads);
+int64_t at_attention_fwd_workspace_bytes(const at_attention_t* shape);
+int at_attention_fwd(const at_attention_t* shape, const void* q, const void* k, const void* v,
+                     void* out, float* lse, void* out_rest, void* workspace,
+                     int64_t workspace_bytes, at_stream_t stream);
+int64_t at_attention_bwd_workspace_bytes(const at_attention_t* shape);
+int at_attention_bwd(const at_attention_t* shape, const void* output_grad, const void* q,
+                     const void* k, const void* v, const void* out, const void* out_rest,
+                     const float* lse, void* dq, void* dk, void* dv, void* workspace,
+                     int64_t workspace_bytes, at_stream_t stream);
+
+/* ------------------------------------------------------------------------------------------
+ * Rotary positions with one or several axes (no counterpart in the reference).  Features of each
+ * head are turned in pairs: pair n by the angle positions[pair_axis[n]] * inv_freq[n], features
+ * (n, n + pairs), or (2 n, 2 n + 1) where adjacent; features from 2 * pairs on are copied.
+ *   (x, y) -> (x cos a - y sin a, x sin a + y cos a);   inverse: by -a (the gradient)
+ * q and k (nullable) are [batch, heads, rows, dim] with unit stride along dim; strides[] in
+ * elements (batch, head, token) of q, k, q_out, k_out.  positions (nullable with one axis: token
+ * t of every sequence is at t) is read at axis * position_strides[0] + batch * [1] + token * [2];
+ * its type is 0 int32, 1 int64, 2 float32.  Angles are formed and reduced in 64 bits.  pair_axis
+ * values are clamped to [0, axes).  An output may be the input itself (same address and strides).
+ * ------------------------------------------------------------------------------------------ */
+typedef struct at_rotary {
+  int64_t batch, rows, q_heads, k_heads, dim, pairs, axes;
+  int64_t strides[4][3];
+  int64_t position_strides[3];
+  int position_type;
+  int adjacent;
+  int inverse;
+  int dtype;
+} at_rotary_t;
+
+int at_rotary(const at_rotary_t* shape, const void* q, const void* k, void* q_out, void* k_out,
+              const void* positions, const double* inv_freq, const int* pair_axis,
+              at_stream_t stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -1,0 +1,302 @@
+"""
+GPU parity tests of attention over a sliding window with visible first tokens against the float64
+oracle, whose error bounds (oracle/attention.py) are the tolerances.
+"""
+
+import pytest
+import torch
+
+import attorch_amd
+from oracle.attention import attention
+from .helpers import DTYPES, randn
+
+pytestmark = pytest.mark.gpu
+
+
+def heads_last(shape, seed, dtype, scale=1.0):
+    """[batch, heads, tokens, dim] seen through a [batch, tokens, heads, dim] tensor."""
+    batch, heads, tokens, dim = shape
+    return randn((batch, tokens, heads, dim), seed, dtype, scale).transpose(1, 2)
+
+
+def assert_within(actual, expected, what) -> None:
+    value, bound = expected
+    actual = actual.detach().double().cpu()
+    assert actual.shape == value.shape, f'{what}: shape {tuple(actual.shape)} != {tuple(value.shape)}'
+    excess = (actual - value).abs() - bound
+    assert not torch.isnan(actual).any(), f'{what}: NaN'
+    worst = excess.argmax() if excess.numel() else 0
+    assert not excess.numel() or excess.max() <= 0, \
+        f'{what}: {actual.reshape(-1)[worst]} is off {value.reshape(-1)[worst]} by more than {bound.reshape(-1)[worst]}'
+
+
+def check(q, k, v, dout=None, lengths=None, query_lengths=None, causal=True, window=None, sinks=0, scale=None):
+    """Forward, and backward where dout is given, on the GPU and in the oracle."""
+    expected = attention(q, k, v, dout, lengths, query_lengths, causal, window, sinks, scale)
+    qd, kd, vd = (t.cuda().requires_grad_(dout is not None) for t in (q, k, v))
+    out = attorch_amd.WindowAttentionAutoGrad.apply(
+        qd, kd, vd, None if lengths is None else lengths.cuda(), None if query_lengths is None else query_lengths.cuda(),
+        causal, window, sinks, scale)
+    assert out.dtype is q.dtype
+    assert_within(out, expected['out'], 'output')
+    if dout is not None:
+        grads = torch.autograd.grad(out, (qd, kd, vd), dout.cuda())
+        for grad, name in zip(grads, ('dq', 'dk', 'dv')):
+            assert grad.dtype is q.dtype
+            assert_within(grad, expected[name], name)
+    return out
+
+
+def inputs(batch, heads, kv_heads, rows, keys, dim, dtype, seed=0):
+    return (heads_last((batch, heads, rows, dim), seed + 1, dtype), heads_last((batch, kv_heads, keys, dim), seed + 2, dtype),
+            heads_last((batch, kv_heads, keys, dim), seed + 3, dtype), heads_last((batch, heads, rows, dim), seed + 4, dtype))
+
+
+# lengths around the tiles of 32, 64 and 128 tokens, and from one token on
+@pytest.mark.parametrize('dtype', DTYPES)
+@pytest.mark.parametrize('tokens', [1, 2, 31, 32, 33, 64, 65, 127, 128, 129, 200, 257])
+def test_lengths(tokens, dtype) -> None:
+    check(*inputs(2, 2, 1, tokens, tokens, 64, dtype))
+
+
+@pytest.mark.parametrize('dtype', DTYPES)
+@pytest.mark.parametrize('dim', [1, 7, 8, 16, 24, 32, 40, 64, 72, 80, 96, 104, 120, 128])
+def test_head_dims(dim, dtype) -> None:
+    check(*inputs(1, 4, 2, 150, 150, dim, dtype), window=70, sinks=3)
+
+
+@pytest.mark.parametrize('dtype', DTYPES)
+@pytest.mark.parametrize('heads, kv_heads', [(1, 1), (3, 3), (6, 2), (5, 1), (8, 1), (7, 7)])
+def test_shared_heads(heads, kv_heads, dtype) -> None:
+    check(*inputs(2, heads, kv_heads, 90, 90, 32, dtype), window=50, sinks=2)
+
+
+@pytest.mark.parametrize('dtype', DTYPES)
+@pytest.mark.parametrize('causal', [True, False])
+@pytest.mark.parametrize('window, sinks', [(None, 0), (None, 5), (1, 0), (1, 1), (2, 64), (16, 4), (63, 0), (64, 1),
+                                           (65, 130), (128, 7), (1000, 0), (1 << 60, 1 << 60)])
+def test_windows(window, sinks, causal, dtype) -> None:
+    check(*inputs(1, 2, 1, 300, 300, 64, dtype), causal=causal, window=window, sinks=sinks)
+
+
+@pytest.mark.parametrize('dtype', DTYPES)
+@pytest.mark.parametrize('causal', [True, False])
+@pytest.mark.parametrize('int_type', [torch.int32, torch.int64])
+def test_ragged_batch(int_type, causal, dtype) -> None:
+    lengths = torch.tensor([0, 1, 130, 77, 128, 64, -3, 999], dtype=int_type)
+    check(*inputs(8, 4, 2, 130, 130, 40, dtype), lengths=lengths, causal=causal, window=40, sinks=3)
+
+
+@pytest.mark.parametrize('dtype', DTYPES)
+@pytest.mark.parametrize('causal', [True, False])
+def test_padded_rows_beside_whole_tiles(causal, dtype) -> None:
+    """Rows behind a sequence that share a wave with rows that see every key of a tile."""
+    check(*inputs(3, 3, 1, 400, 400, 32, dtype), lengths=torch.tensor([301, 111, 397]), causal=causal)
+    check(*inputs(3, 2, 2, 400, 400, 32, dtype), lengths=torch.tensor([301, 111, 397]), causal=causal, window=150, sinks=2)
+
+
+@pytest.mark.parametrize('dtype', DTYPES)
+@pytest.mark.parametrize('causal', [True, False])
+def test_query_lengths(causal, dtype) -> None:
+    lengths = torch.tensor([200, 5, 90, 0, 33, 200])
+    query_lengths = torch.tensor([70, 70, 11, 8, 0, 500])
+    check(*inputs(6, 4, 2, 70, 200, 64, dtype), lengths=lengths, query_lengths=query_lengths, causal=causal, window=50,
+          sinks=2)
+    check(*inputs(6, 4, 2, 70, 200, 64, dtype), query_lengths=query_lengths.int(), lengths=lengths, causal=causal)
+    check(*inputs(6, 4, 2, 70, 200, 64, dtype), query_lengths=query_lengths, causal=causal, window=50)
+
+
+@pytest.mark.parametrize('dtype', DTYPES)
+@pytest.mark.parametrize('rows', [1, 2, 5, 17, 64, 100])
+@pytest.mark.parametrize('heads, kv_heads', [(8, 2), (4, 4), (6, 1)])
+def test_new_tokens_over_a_cache(heads, kv_heads, rows, dtype) -> None:
+    """Single tokens and chunks; few rows and many keys are worked on in pieces that are joined."""
+    q, k, v, dout = inputs(2, heads, kv_heads, rows, 1111, 64, dtype)
+    lengths = torch.tensor([1111, 403])
+    check(q, k, v, dout, lengths=lengths)
+    check(q, k, v, dout, lengths=lengths, window=130, sinks=4)
+    check(q, k, v, lengths=lengths)
+    check(q, k, v, window=300, sinks=70)
+    check(q, k, v, causal=False)
+
+
+def test_scale_and_large_scores() -> None:
+    for dtype in DTYPES:
+        q, k, v, dout = inputs(1, 2, 2, 100, 100, 64, dtype)
+        check(q, k, v, dout, scale=1.0)
+        check((q.float() * 8).to(dtype), k, v, dout, scale=0.9)
+        check(q, k, v, dout, scale=1e-3)
+        # scores so negative or positive that exponentials without the maximum would vanish or overflow
+        check(q, k + 10, v, dout, scale=2.0)
+
+
+@pytest.mark.parametrize('dtype', DTYPES)
+@pytest.mark.parametrize('garbage', [float('nan'), float('inf'), -float('inf'), 'lowest'])
+def test_unseen_places_may_hold_anything(garbage, dtype) -> None:
+    """
+    Room behind the sequences, tokens that fell out of the window, padded query rows and their output
+    gradients.
+    """
+    garbage = torch.finfo(dtype).min if garbage == 'lowest' else garbage
+    q, k, v, dout = inputs(3, 4, 2, 90, 300, 64, dtype)
+    lengths, query_lengths = torch.tensor([300, 150, 0]), torch.tensor([90, 20, 1])
+    for t in (k, v):
+        t[1, :, 150:] = garbage
+        t[2] = garbage
+        t[0, :, 4:300 - 90 - 29] = garbage     # between the sinks and the first row's window of 30
+        t[1, :, 4:150 - 20 - 29] = garbage
+    for t in (q, dout):
+        t[1, :, 20:] = garbage
+        t[2] = garbage
+    check(q, k, v, dout, lengths=lengths, query_lengths=query_lengths, window=30, sinks=4)
+    one = q[:, :, :1].clone()
+    for t in (k, v):
+        t[0, :, 4:300 - 30] = garbage
+        t[1, :, 4:150 - 30] = garbage
+    check(one, k, v, None, lengths=lengths, window=30, sinks=4)
+
+
+@pytest.mark.parametrize('dtype', DTYPES)
+def test_layouts(dtype) -> None:
+    """Packed projections, head-major caches, expanded and misaligned tensors give the same results."""
+    q, k, v, dout = inputs(2, 4, 2, 70, 70, 32, dtype)
+    base = check(q, k, v, dout, window=20)
+
+    def run(qd, kd, vd, dd):
+        qd, kd, vd = (t.detach().requires_grad_() for t in (qd, kd, vd))
+        out = attorch_amd.WindowAttention(window=20)(qd, kd, vd)
+        return (out, *torch.autograd.grad(out, (qd, kd, vd), dd))
+
+    expected = run(*(t.cuda() for t in (q, k, v, dout)))
+    assert torch.equal(expected[0], base)
+    packed = torch.cat([t.transpose(1, 2).flatten(2) for t in (q, k, v)], -1).cuda()
+    views = [t.unflatten(2, (-1, 32)).transpose(1, 2) for t in packed.split([128, 64, 64], -1)]
+    head_major = [t.contiguous().cuda() for t in (q, k, v)]
+    odd = [torch.nn.functional.pad(t, (1, 2)).cuda()[..., 1:-2] for t in (q, k, v)]
+    apart = [torch.stack([t, t], -1).cuda()[..., 0] for t in (q, k, v)]
+    for variant in (views, head_major, odd, apart):
+        for got, want in zip(run(*variant, dout.cuda()), expected):
+            assert torch.equal(got, want)
+    # an output gradient that is expanded, as sum() makes it
+    ones = torch.ones((), dtype=dtype, device='cuda').expand(2, 4, 70, 32)
+    for got, want in zip(run(*head_major, ones), run(*head_major, ones.contiguous())):
+        assert torch.equal(got, want)
+    # keys and values shared by the batch: their gradients are the sums over it
+    kd, vd = (t[:1].cuda().requires_grad_() for t in (k, v))
+    out = attorch_amd.WindowAttention(window=20)(q.cuda(), kd.expand(2, -1, -1, -1), vd.expand(2, -1, -1, -1))
+    out.backward(dout.cuda())
+    same = attention(q, k[:1].expand(2, -1, -1, -1), v[:1].expand(2, -1, -1, -1), dout, window=20)
+    for grad, name in ((kd.grad, 'dk'), (vd.grad, 'dv')):
+        value, bound = same[name]
+        step = torch.finfo(dtype).eps / 2
+        assert_within(grad, (value.sum(0, True), bound.sum(0, True) + step * value.sum(0, True).abs()), name)
+
+
+def test_results_do_not_change_from_run_to_run() -> None:
+    q, k, v, dout = (t.cuda() for t in inputs(2, 8, 2, 500, 500, 128, torch.bfloat16))
+    first = None
+    for _ in range(3):
+        leaves = [t.detach().requires_grad_() for t in (q, k, v)]
+        out = attorch_amd.WindowAttention(window=100, num_sinks=4)(*leaves)
+        got = (out, *torch.autograd.grad(out, leaves, dout))
+        first = got if first is None else first
+        for a, b in zip(got, first):
+            assert torch.equal(a, b)
+
+
+def test_empty_calls() -> None:
+    for batch, rows, keys in ((0, 4, 4), (2, 0, 5), (2, 0, 0)):
+        q, k, v, _ = (t.cuda().requires_grad_() for t in inputs(batch, 4, 2, rows, keys, 16, torch.float32))
+        out = attorch_amd.WindowAttention()(q, k, v)
+        assert out.shape == q.shape
+        grads = torch.autograd.grad(out, (q, k, v), torch.ones_like(out))
+        for grad, leaf in zip(grads, (q, k, v)):
+            assert grad.shape == leaf.shape and not grad.any()
+
+
+def test_autocast() -> None:
+    q, k, v, dout = (t.cuda() for t in inputs(2, 4, 2, 60, 60, 64, torch.float32))
+    leaves = [t.requires_grad_() for t in (q, k, v)]
+    with torch.autocast('cuda', dtype=torch.bfloat16):
+        out = attorch_amd.WindowAttention(window=30)(*leaves)
+    assert out.dtype is torch.bfloat16
+    grads = torch.autograd.grad(out, leaves, dout.bfloat16())
+    plain = [t.detach().bfloat16().requires_grad_() for t in leaves]
+    same = attorch_amd.WindowAttention(window=30)(*plain)
+    assert torch.equal(out, same)
+    for grad, other in zip(grads, torch.autograd.grad(same, plain, dout.bfloat16())):
+        assert grad.dtype is torch.float32 and torch.equal(grad, other.float())
+
+
+def test_frozen_inputs_and_no_grad() -> None:
+    q, k, v, dout = (t.cuda() for t in inputs(1, 2, 2, 40, 40, 32, torch.float16))
+    leaves = [t.detach().requires_grad_() for t in (q, k, v)]
+    full = torch.autograd.grad(attorch_amd.WindowAttention()(*leaves), leaves, dout)
+    for n in range(3):
+        some = [t.detach().requires_grad_(m == n) for m, t in enumerate((q, k, v))]
+        (grad,) = torch.autograd.grad(attorch_amd.WindowAttention()(*some), some[n], dout)
+        assert torch.equal(grad, full[n])
+    with torch.no_grad():
+        out = attorch_amd.WindowAttention()(*leaves)
+    assert not out.requires_grad
+    out = attorch_amd.WindowAttention()(*leaves)
+    (grad,) = torch.autograd.grad(out, leaves[0], dout, create_graph=True)
+    with pytest.raises(RuntimeError):
+        grad.sum().backward()          # no second derivatives
+
+
+def test_other_stream_and_graph() -> None:
+    """A step on a side stream, then captured and replayed with eager work in between."""
+    q, k, v, dout = (t.cuda() for t in inputs(2, 4, 2, 120, 120, 64, torch.bfloat16))
+    one, cache_k, cache_v = (t.cuda() for t in inputs(2, 4, 2, 1, 3000, 64, torch.bfloat16, 9)[:3])
+    lengths = torch.tensor([2000, 3000], device='cuda')
+    leaves = [t.requires_grad_() for t in (q, k, v)]
+    layer = attorch_amd.WindowAttention(window=50, num_sinks=4)
+
+    def step():
+        out = layer(*leaves)
+        token = attorch_amd.WindowAttentionAutoGrad.apply(one, cache_k, cache_v, lengths)
+        return [out, *torch.autograd.grad(out, leaves, dout), token]
+
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        for _ in range(2):
+            on_side = step()
+    torch.cuda.current_stream().wait_stream(side)
+    torch.cuda.synchronize()
+    for a, b in zip(on_side, step()):
+        assert torch.equal(a, b)
+    graphs, outs = [], []
+    for _ in range(2):                 # two graphs, replayed in turn
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            outs.append(step())
+        graphs.append(graph)
+    for seed in range(3):
+        with torch.no_grad():
+            for n, t in enumerate((q, k, v, dout, one)):
+                t.copy_(torch.randn(t.shape, generator=torch.Generator().manual_seed(10 * seed + n)))
+            lengths.copy_(torch.tensor([100 + seed, 3000 - seed]))
+        for graph, out in zip(graphs, outs):
+            graph.replay()
+            torch.cuda.synchronize()
+            got = [t.clone() for t in out]
+            for a, b in zip(got, step()):
+                assert torch.equal(a, b)
+            torch.cuda.synchronize()
+
+
+def test_long_cache_offsets() -> None:
+    """Keys beyond 4 GiB of one head's cache; a single row and a chunk see only the last ones and the sinks."""
+    heads, tokens, dim = 2, (1 << 23) + 321, 128
+    k = torch.zeros(1, heads, tokens, dim, dtype=torch.bfloat16, device='cuda')
+    v = torch.zeros_like(k)
+    assert k.stride(1) * 2 * 2 > 1 << 32
+    tail_k, tail_v = randn((1, heads, 200, dim), 1, torch.bfloat16), randn((1, heads, 200, dim), 2, torch.bfloat16)
+    k[:, :, -196:], v[:, :, -196:] = tail_k[:, :, 4:].cuda(), tail_v[:, :, 4:].cuda()
+    k[:, :, :4], v[:, :, :4] = tail_k[:, :, :4].cuda(), tail_v[:, :, :4].cuda()
+    for rows in (1, 40):
+        q = randn((1, 4, rows, dim), 3, torch.bfloat16)
+        out = attorch_amd.WindowAttention(window=100, num_sinks=4)(q.cuda(), k, v)
+        assert_within(out, attention(q, tail_k, tail_v, window=100, sinks=4)['out'], f'{rows} rows')
