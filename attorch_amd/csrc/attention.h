@@ -35,6 +35,7 @@ struct AttentionArgs {
   int lengths64, causal;
   int batch, kv_heads, group, rows, keys, dim;
   int row_pitch, tiles, splits;
+  int sink_tiles, sink_chunks, chunks, chunk_steps;   // dk and dv: see chunk_plan
   int left, right, sinks;
   float scale, scale_log2;
 };

@@ -6,7 +6,8 @@
 //
 // Two kernels, each of which owns what it sums: the first walks over the keys for a tile of rows (dq, and
 // delta for the second), the second over the rows for a tile of keys (dk, dv).  The scores are formed
-// twice, and no sum crosses workgroups: results do not depend on the order in which they run.
+// twice, and sums that cross workgroups are added in a fixed order by a third kernel (chunk_plan):
+// results do not depend on the order in which workgroups run.
 //
 // delta is taken from the output before its rounding (the forward pass keeps what the rounding left
 // over): an error of delta is common to a whole row of ds, and with the rounded output it was the largest
@@ -157,6 +158,15 @@ __global__ __launch_bounds__(kWaves * 64, sizeof(T) == 2 ? 2 : 1) void attention
     }
 }
 
+// Work items of a head whose results are partial sums, and the number of item `nth` of its class among them.
+__host__ __device__ inline int64_t part_items(const AttentionArgs& a) {
+  return (int64_t)(a.sink_chunks > 1 ? a.sink_tiles * a.sink_chunks : 0) +
+         (a.chunks > 1 ? (int64_t)(a.tiles - a.sink_tiles) * a.chunks : 0);
+}
+__host__ __device__ inline int64_t part_item(const AttentionArgs& a, bool of_sinks, int nth) {
+  return of_sinks || a.sink_chunks <= 1 ? nth : (int64_t)a.sink_tiles * a.sink_chunks + nth;
+}
+
 __device__ __forceinline__ int wave_min(int v) {
   for (int o = 32; o > 0; o >>= 1) v = min(v, __shfl_xor(v, o, kWave));
   return __builtin_amdgcn_readfirstlane(v);
@@ -172,8 +182,14 @@ __global__ __launch_bounds__(kWaves * 64, sizeof(T) == 2 ? 2 : 1) void attention
 
   const int lane = threadIdx.x & 63, half = lane >> 5;
   const int wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
-  const int tile_id = (int)(blockIdx.x % a.tiles);     // the first keys of a causal sequence are seen by the most rows
-  const int bh = blockIdx.x / a.tiles;
+  // the first keys of a causal sequence are seen by the most rows: their workgroups start first
+  const int items = a.sink_tiles * a.sink_chunks + (a.tiles - a.sink_tiles) * a.chunks;
+  const int item = (int)(blockIdx.x % items), bh = (int)(blockIdx.x / items);
+  const bool of_sinks = item < a.sink_tiles * a.sink_chunks;
+  const int nth = of_sinks ? item : item - a.sink_tiles * a.sink_chunks;
+  const int tile_chunks = of_sinks ? a.sink_chunks : a.chunks;
+  const int chunk = nth % tile_chunks;
+  const int tile_id = nth / tile_chunks + (of_sinks ? 0 : a.sink_tiles);
   const int b = bh / a.kv_heads, h = bh - b * a.kv_heads;
   const Sequence seq = sequence_of(a, b);
   const int live_rows = seq.live * a.group;
@@ -223,8 +239,10 @@ __global__ __launch_bounds__(kWaves * 64, sizeof(T) == 2 ? 2 : 1) void attention
     begin = min(begin, ranges[w]);
     end = max(end, ranges[kWaves + w]);
   }
-  begin = __builtin_amdgcn_readfirstlane(begin / kStep);
-  end = __builtin_amdgcn_readfirstlane(end < 0 ? begin : end / kStep + 1);
+  begin = begin / kStep + chunk * a.chunk_steps;
+  end = min(end < 0 ? 0 : end / kStep + 1, begin + a.chunk_steps);
+  begin = __builtin_amdgcn_readfirstlane(begin);
+  end = __builtin_amdgcn_readfirstlane(end);
 
   const char* qb = a.q.p + b * a.q.batch + (int64_t)h * a.group * a.q.head;
   const char* db = a.dout.p + b * a.dout.batch + (int64_t)h * a.group * a.dout.head;
@@ -301,8 +319,29 @@ __global__ __launch_bounds__(kWaves * 64, sizeof(T) == 2 ? 2 : 1) void attention
     }
   }
 
+  const float dv_scale = ProbShift<T>::value != 0.f ? 1.f / 32768.f : 1.f;
+  if (tile_chunks > 1) {               // one of several partial sums
+    float* part = a.part + ((int64_t)bh * part_items(a) + part_item(a, of_sinks, nth)) * 2 * kTileRows * a.dim +
+                  (int64_t)(wave * 32 + (lane & 31)) * a.dim;
+#pragma unroll
+    for (int dt = 0; dt < DT; ++dt)
+#pragma unroll
+      for (int q = 0; q < 4; ++q) {
+        const int d = dt * 32 + q * 8 + half * 4;
+        if (d < a.dim) {
+          float x[4], y[4];
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            x[j] = dk[dt][q * 4 + j] * a.scale;
+            y[j] = dv[dt][q * 4 + j] * dv_scale;
+          }
+          store_f32<float, 4>(part + d, x);
+          store_f32<float, 4>(part + (int64_t)kTileRows * a.dim + d, y);
+        }
+      }
+    return;
+  }
   if (key >= a.keys) return;
-  const float unshift = ProbShift<T>::value != 0.f ? 1.f / 32768.f : 1.f;
   char* kp = a.dk.p + b * a.dk.batch + h * a.dk.head + key * a.dk.token;
   char* vp = a.dv.p + b * a.dv.batch + h * a.dv.head + key * a.dv.token;
 #pragma unroll
@@ -314,7 +353,7 @@ __global__ __launch_bounds__(kWaves * 64, sizeof(T) == 2 ? 2 : 1) void attention
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
         x[j] = dk[dt][q * 4 + j] * a.scale;
-        y[j] = dv[dt][q * 4 + j] * unshift;
+        y[j] = dv[dt][q * 4 + j] * dv_scale;
       }
       if (d < a.dim) {
         store_f32<T, 4>(reinterpret_cast<T*>(kp) + d, x);
@@ -323,19 +362,92 @@ __global__ __launch_bounds__(kWaves * 64, sizeof(T) == 2 ? 2 : 1) void attention
     }
 }
 
+// Sums the partial dk and dv of the tiles that were worked on in chunks, in the chunks' order.  32 lanes per
+// key, four elements of dim per lane.
+template <typename T>
+__global__ __launch_bounds__(256) void attention_dkv_join_kernel(AttentionArgs a) {
+  const int first_tile = a.sink_chunks > 1 ? 0 : a.sink_tiles;
+  const int tiles = (a.chunks > 1 ? a.tiles : a.sink_tiles) - first_tile;
+  const int64_t at = (int64_t)blockIdx.x * 8 + (threadIdx.x >> 5);
+  const int bh = (int)(at / ((int64_t)tiles * kTileRows));
+  if (bh >= a.batch * a.kv_heads) return;
+  const int rest = (int)(at - (int64_t)bh * tiles * kTileRows);
+  const int tile = first_tile + rest / kTileRows, local = rest % kTileRows;
+  const int key = tile * kTileRows + local, d = (threadIdx.x & 31) * 4;
+  if (key >= a.keys || d >= a.dim) return;
+  const bool of_sinks = tile < a.sink_tiles;
+  const int chunks = of_sinks ? a.sink_chunks : a.chunks;
+  const int nth = of_sinks ? tile * chunks : (tile - a.sink_tiles) * chunks;
+  const float* part = a.part + (((int64_t)bh * part_items(a) + part_item(a, of_sinks, nth)) * 2 * kTileRows + local) * a.dim + d;
+  const int64_t other = (int64_t)kTileRows * a.dim;
+  float x[4] = {0.f, 0.f, 0.f, 0.f}, y[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll 4
+  for (int c = 0; c < chunks; ++c) {
+    float u[4], w[4];
+    load_f32<float, 4>(part + c * 2 * other, u);
+    load_f32<float, 4>(part + c * 2 * other + other, w);
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      x[j] += u[j];
+      y[j] += w[j];
+    }
+  }
+  const int b = bh / a.kv_heads, h = bh - b * a.kv_heads;
+  store_f32<T, 4>(reinterpret_cast<T*>(a.dk.p + b * a.dk.batch + h * a.dk.head + key * a.dk.token) + d, x);
+  store_f32<T, 4>(reinterpret_cast<T*>(a.dv.p + b * a.dv.batch + h * a.dv.head + key * a.dv.token) + d, y);
+}
+
+// How dk and dv are cut up.  The rows that see a tile of keys are walked over in chunks of chunk_steps
+// steps; tiles with one chunk write their result, the others partial sums that a second kernel adds.
+// With a window a tile is seen by few rows, but a tile with sinks by all: such tiles are cut to the
+// others' length, or one workgroup per head would run on alone (window 1024 over 8192 tokens: 5.1 ms
+// instead of 1.3).  Where the tiles alone do not give every CU two workgroups, all are cut further.
+void chunk_plan(AttentionArgs& a) {
+  a.tiles = (int)cdiv64(a.keys, kTileRows);
+  const int64_t rows = (int64_t)a.rows * a.group;
+  const int64_t near = (int64_t)(a.left + a.right + kTileRows) * a.group;
+  const int64_t span = near < rows ? near : rows;              // of a tile without sinks
+  a.sink_tiles = span < rows ? (int)cdiv64(a.sinks, kTileRows) : 0;
+  int64_t steps = cdiv64(span, kStep) + 1;                     // the first step need not start at the first row
+  const int64_t groups = (int64_t)a.tiles * a.batch * a.kv_heads;
+  const int64_t want = 2 * device_cu_count();
+  if (groups < want && steps > 2) {
+    int64_t n = cdiv64(want, groups);
+    if (n > steps / 2) n = steps / 2;
+    steps = cdiv64(steps, n);
+  }
+  a.chunk_steps = (int)steps;
+  a.chunks = (int)cdiv64(cdiv64(span, kStep) + 1, steps);
+  a.sink_chunks = (int)cdiv64(cdiv64(rows, kStep) + 1, steps);
+}
+
+int64_t delta_bytes(const AttentionArgs& a) { return (int64_t)a.batch * a.kv_heads * a.row_pitch * 4; }
+
+int64_t part_bytes(const AttentionArgs& a) {
+  return (int64_t)a.batch * a.kv_heads * part_items(a) * 2 * kTileRows * a.dim * 4;
+}
+
 template <typename T, int DT>
 int launch(AttentionArgs a, hipStream_t stream) {
   const int64_t heads = (int64_t)a.batch * a.kv_heads;
-  if (!grid_fits(cdiv64((int64_t)a.rows * a.group, kTileRows) * heads) || !grid_fits(cdiv64(a.keys, kTileRows) * heads))
-    return AT_ERR_DIM;
+  chunk_plan(a);
+  const int64_t items = (int64_t)a.sink_tiles * a.sink_chunks + (int64_t)(a.tiles - a.sink_tiles) * a.chunks;
+  const int64_t row_tiles = cdiv64((int64_t)a.rows * a.group, kTileRows);
+  const int64_t joined = ((a.chunks > 1 ? a.tiles : a.sink_tiles) - (a.sink_chunks > 1 ? 0 : a.sink_tiles)) *
+                         (int64_t)kTileRows * heads;
+  if (!grid_fits(row_tiles * heads) || !grid_fits(items * heads) || !grid_fits(cdiv64(joined, 8))) return AT_ERR_DIM;
+  int rc = AT_OK;
   if (a.rows > 0) {
-    a.tiles = (int)cdiv64((int64_t)a.rows * a.group, kTileRows);
-    hipLaunchKernelGGL((attention_dq_kernel<T, DT>), dim3((unsigned)(a.tiles * heads)), dim3(kWaves * 64), 0, stream, a);
-    const int rc = launch_status();
+    AttentionArgs r = a;
+    r.tiles = (int)row_tiles;
+    hipLaunchKernelGGL((attention_dq_kernel<T, DT>), dim3((unsigned)(row_tiles * heads)), dim3(kWaves * 64), 0, stream, r);
+    rc = launch_status();
     if (rc != AT_OK) return rc;
   }
-  a.tiles = (int)cdiv64(a.keys, kTileRows);
-  hipLaunchKernelGGL((attention_dkv_kernel<T, DT>), dim3((unsigned)(a.tiles * heads)), dim3(kWaves * 64), 0, stream, a);
+  hipLaunchKernelGGL((attention_dkv_kernel<T, DT>), dim3((unsigned)(items * heads)), dim3(kWaves * 64), 0, stream, a);
+  rc = launch_status();
+  if (rc != AT_OK || part_items(a) == 0) return rc;
+  hipLaunchKernelGGL((attention_dkv_join_kernel<T>), dim3((unsigned)cdiv64(joined, 8)), dim3(256), 0, stream, a);
   return launch_status();
 }
 
@@ -358,8 +470,9 @@ extern "C" {
 
 int64_t at_attention_bwd_workspace_bytes(const at_attention_t* shape) {
   AttentionArgs a;
-  if (attention_args(shape, a) != AT_OK) return 0;
-  return (int64_t)a.batch * a.kv_heads * a.row_pitch * 4;
+  if (attention_args(shape, a) != AT_OK || a.keys == 0) return 0;
+  chunk_plan(a);
+  return delta_bytes(a) + part_bytes(a);
 }
 
 int at_attention_bwd(const at_attention_t* shape, const void* output_grad, const void* q, const void* k, const void* v,
@@ -373,12 +486,14 @@ int at_attention_bwd(const at_attention_t* shape, const void* output_grad, const
   if (!aligned16(q) || !aligned16(k) || !aligned16(v) || !aligned16(out) || !aligned16(output_grad) || !aligned16(dq) ||
       !aligned16(dk) || !aligned16(dv) || !aligned16(lse) || !aligned16(workspace) || !aligned16(out_rest))
     return AT_ERR_ALIGN;
-  if (a.rows > 0 && (!workspace || workspace_bytes < at_attention_bwd_workspace_bytes(shape))) return AT_ERR_WORKSPACE;
+  const int64_t need = at_attention_bwd_workspace_bytes(shape);
+  if (need > 0 && (!workspace || workspace_bytes < need)) return AT_ERR_WORKSPACE;
   a.q.p = (char*)q; a.k.p = (char*)k; a.v.p = (char*)v; a.out.p = (char*)out; a.dout.p = (char*)output_grad;
   a.dq.p = (char*)dq; a.dk.p = (char*)dk; a.dv.p = (char*)dv;
   a.rest = (char*)out_rest;
   a.lse = const_cast<float*>(lse);
   a.delta = (float*)workspace;
+  a.part = (float*)((char*)workspace + delta_bytes(a));   // row_pitch keeps it on 256 bytes
   if (shape->dtype == AT_DTYPE_F32) return launch_dim<float>(a, (hipStream_t)stream);
   if (shape->dtype == AT_DTYPE_F16) return launch_dim<f16_t>(a, (hipStream_t)stream);
   return launch_dim<bf16_t>(a, (hipStream_t)stream);
