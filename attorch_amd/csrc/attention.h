@@ -35,7 +35,7 @@ struct AttentionArgs {
   int lengths64, causal;
   int batch, kv_heads, group, rows, keys, dim;
   int row_pitch, tiles, splits;
-  int sink_tiles, sink_chunks, chunks, chunk_steps;   // dk and dv: see chunk_plan
+  int tile_keys, sink_tiles, sink_chunks, chunks, chunk_steps;   // dk and dv: see chunk_plan
   int left, right, sinks;
   float scale, scale_log2;
 };
@@ -71,6 +71,26 @@ __device__ __forceinline__ KeyRange keys_of(const AttentionArgs& a, const Sequen
   r.hi = min(last + a.right + 1, s.len);
   r.sinks = min(a.sinks, a.causal ? last + 1 : s.len);
   return r;
+}
+
+// Which piece of which head a workgroup takes: the pieces of a head stay on one XCD (workgroups go to
+// the 8 XCDs in turn), whose L2 then holds the head's keys and values, and come in order of rank, which
+// the callers make the order of falling work.  Heads beyond a multiple of 8 are spread over all XCDs,
+// every other round of 8 in reverse, so that none gets the heavier piece each time.  (Heads in plain
+// order leave pieces of equal rank to the same XCD: causal, 32 pieces, 38 % of the CU time was idle.)
+struct Piece {
+  int rank, bh;
+};
+__device__ __forceinline__ Piece piece_of(int id, int pieces, int heads) {
+  const int whole = heads & ~7;
+  if (id < whole * pieces) {
+    const int n = (id >> 3) / pieces;
+    return {(id >> 3) - n * pieces, n * 8 + (id & 7)};
+  }
+  const int rest = heads - whole;
+  id -= whole * pieces;
+  if ((id & 8) && (id | 7) < rest * pieces) id ^= 7;
+  return {id / rest, whole + id % rest};
 }
 
 // ---- matrix-core fragments --------------------------------------------------------------------

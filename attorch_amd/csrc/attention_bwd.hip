@@ -30,8 +30,9 @@ __global__ __launch_bounds__(kWaves * 64, sizeof(T) == 2 ? 2 : 1) void attention
 
   const int lane = threadIdx.x & 63, half = lane >> 5;
   const int wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
-  const int tile_id = a.tiles - 1 - (int)(blockIdx.x % a.tiles);
-  const int bh = blockIdx.x / a.tiles;
+  const Piece piece = piece_of(blockIdx.x, a.tiles, a.batch * a.kv_heads);
+  const int tile_id = a.tiles - 1 - piece.rank;    // the last rows of a causal sequence see the most keys
+  const int bh = piece.bh;
   const int b = bh / a.kv_heads, h = bh - b * a.kv_heads;
   const Sequence seq = sequence_of(a, b);
   const int live_rows = seq.live * a.group, all_rows = a.rows * a.group;
@@ -172,19 +173,23 @@ __device__ __forceinline__ int wave_min(int v) {
   return __builtin_amdgcn_readfirstlane(v);
 }
 
-template <typename T, int DT>
-__global__ __launch_bounds__(kWaves * 64, sizeof(T) == 2 ? 2 : 1) void attention_dkv_kernel(AttentionArgs a) {
+// A wave owns KT x 32 keys: their keys and values stay in registers as operands, and every fragment of
+// queries and output gradients that it reads from LDS serves KT products.
+template <typename T, int DT, int KT>
+__global__ __launch_bounds__(kWaves * 64, KT == 1 && sizeof(T) == 2 ? 2 : 1) void attention_dkv_kernel(AttentionArgs a) {
   typedef Tile<T, DT> L;
   typedef typename Frag<T>::type F;
   constexpr int kTileBytes = kStep * L::kPitch;
   constexpr int kStage = 2 * kTileBytes + 2048;                       // queries | output gradients | lse | delta
+  constexpr int kTileKeys = 32 * KT * kWaves;
   __shared__ __attribute__((aligned(1024))) char lds[2 * kStage];
 
   const int lane = threadIdx.x & 63, half = lane >> 5;
   const int wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
-  // the first keys of a causal sequence are seen by the most rows: their workgroups start first
-  const int items = a.sink_tiles * a.sink_chunks + (a.tiles - a.sink_tiles) * a.chunks;
-  const int item = (int)(blockIdx.x % items), bh = (int)(blockIdx.x / items);
+  // the first keys of a causal sequence are seen by the most rows
+  const Piece piece = piece_of(blockIdx.x, a.sink_tiles * a.sink_chunks + (a.tiles - a.sink_tiles) * a.chunks,
+                               a.batch * a.kv_heads);
+  const int item = piece.rank, bh = piece.bh;
   const bool of_sinks = item < a.sink_tiles * a.sink_chunks;
   const int nth = of_sinks ? item : item - a.sink_tiles * a.sink_chunks;
   const int tile_chunks = of_sinks ? a.sink_chunks : a.chunks;
@@ -193,40 +198,51 @@ __global__ __launch_bounds__(kWaves * 64, sizeof(T) == 2 ? 2 : 1) void attention
   const int b = bh / a.kv_heads, h = bh - b * a.kv_heads;
   const Sequence seq = sequence_of(a, b);
   const int live_rows = seq.live * a.group;
-  const int key0 = tile_id * kTileRows;
+  const int key0 = tile_id * kTileKeys + wave * 32 * KT + (lane & 31);   // this lane's keys: key0 + 32 kt
 
-  const int key = key0 + wave * 32 + (lane & 31);
-  const bool valid = key < seq.len;
-  F kf[L::kSteps], vf[L::kSteps];
-  {
+  F kf[KT][L::kSteps], vf[KT][L::kSteps];
+  int row_lo[KT], row_hi[KT];          // rows [row_lo, row_hi] see the key
+  int any_lo = 1 << 30, any_hi = -1, all_lo = 0, all_hi = 1 << 30;
+#pragma unroll
+  for (int kt = 0; kt < KT; ++kt) {
+    const int key = key0 + 32 * kt;
+    const bool valid = key < seq.len;
     const char* kp = a.k.p + b * a.k.batch + h * a.k.head + key * a.k.token;
     const char* vp = a.v.p + b * a.v.batch + h * a.v.head + key * a.v.token;
+    row_lo[kt] = 1 << 30;
+    row_hi[kt] = -1;
+    if (valid) {
+      const bool sink = key < a.sinks;
+      const int tok_lo = !a.causal && sink ? seq.start : max(key - a.right, seq.start);
+      const int tok_hi = sink ? seq.len - 1 : min(key + a.left, seq.len - 1);
+      if (tok_lo <= tok_hi) {
+        row_lo[kt] = (tok_lo - seq.start) * a.group;
+        row_hi[kt] = min((tok_hi - seq.start) * a.group + a.group, live_rows) - 1;
+      }
+    }
 #pragma unroll
     for (int s = 0; s < L::kSteps; ++s) {
       const int d = s * 16 + half * 8;
-      const bool in = valid && d < a.dim;
-      kf[s] = in ? Frag<T>::load(kp + d * sizeof(T)) : Frag<T>::zero();
-      vf[s] = in ? Frag<T>::load(vp + d * sizeof(T)) : Frag<T>::zero();
+      const bool in = row_hi[kt] >= 0 && d < a.dim;       // what nothing sees is not read
+      kf[kt][s] = in ? Frag<T>::load(kp + d * sizeof(T)) : Frag<T>::zero();
+      vf[kt][s] = in ? Frag<T>::load(vp + d * sizeof(T)) : Frag<T>::zero();
     }
-  }
-  f32x16 dk[DT], dv[DT];
-#pragma unroll
-  for (int dt = 0; dt < DT; ++dt) dk[dt] = dv[dt] = zero_acc();
-
-  // rows [row_lo, row_hi] that see this lane's key
-  int row_lo = 1 << 30, row_hi = -1;
-  if (valid) {
-    const bool sink = key < a.sinks;
-    const int tok_lo = !a.causal && sink ? seq.start : max(key - a.right, seq.start);
-    const int tok_hi = sink ? seq.len - 1 : min(key + a.left, seq.len - 1);
-    if (tok_lo <= tok_hi) {
-      row_lo = (tok_lo - seq.start) * a.group;
-      row_hi = min((tok_hi - seq.start) * a.group + a.group, live_rows) - 1;
-    }
+    any_lo = min(any_lo, row_lo[kt]);
+    any_hi = max(any_hi, row_hi[kt]);
+    all_lo = max(all_lo, row_lo[kt]);
+    all_hi = min(all_hi, row_hi[kt]);
   }
   // rows that some key of the wave, and that every key of it, is seen by
-  const int any_lo = wave_min(row_lo), any_hi = -wave_min(-row_hi);
-  const int all_lo = -wave_min(-row_lo), all_hi = wave_min(row_hi);
+  any_lo = wave_min(any_lo);
+  any_hi = -wave_min(-any_hi);
+  all_lo = -wave_min(-all_lo);
+  all_hi = wave_min(all_hi);
+  f32x16 dk[KT][DT], dv[KT][DT];
+#pragma unroll
+  for (int kt = 0; kt < KT; ++kt)
+#pragma unroll
+    for (int dt = 0; dt < DT; ++dt) dk[kt][dt] = dv[kt][dt] = zero_acc();
+
   __shared__ int ranges[2 * kWaves];
   if (lane == 0) {
     ranges[wave] = any_lo;
@@ -279,11 +295,20 @@ __global__ __launch_bounds__(kWaves * 64, sizeof(T) == 2 ? 2 : 1) void attention
       const int r0 = t * kStep + n * 32;
       if (r0 > any_hi || r0 + 31 < any_lo) continue;
       const bool whole = r0 >= all_lo && r0 + 31 <= all_hi;
-      f32x16 s = zero_acc(), dp = zero_acc();
+      f32x16 s[KT], dp[KT];
+#pragma unroll
+      for (int kt = 0; kt < KT; ++kt) s[kt] = dp[kt] = zero_acc();
 #pragma unroll
       for (int ks = 0; ks < L::kSteps; ++ks) {
-        s = Frag<T>::mma(L::rows_frag(stage, n * 32, ks), kf[ks], s);
-        dp = Frag<T>::mma(L::rows_frag(stage + kTileBytes, n * 32, ks), vf[ks], dp);
+        const F qf = L::rows_frag(stage, n * 32, ks);
+#pragma unroll
+        for (int kt = 0; kt < KT; ++kt) s[kt] = Frag<T>::mma(qf, kf[kt][ks], s[kt]);
+      }
+#pragma unroll
+      for (int ks = 0; ks < L::kSteps; ++ks) {
+        const F df = L::rows_frag(stage + kTileBytes, n * 32, ks);
+#pragma unroll
+        for (int kt = 0; kt < KT; ++kt) dp[kt] = Frag<T>::mma(df, vf[kt][ks], dp[kt]);
       }
 #pragma unroll
       for (int q = 0; q < 4; ++q) {
@@ -291,95 +316,100 @@ __global__ __launch_bounds__(kWaves * 64, sizeof(T) == 2 ? 2 : 1) void attention
         const float4 d4 = *reinterpret_cast<const float4*>(stats + 256 + n * 32 + q * 8 + half * 4);
         const float ls[4] = {l4.x, l4.y, l4.z, l4.w}, de[4] = {d4.x, d4.y, d4.z, d4.w};
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          const int e = q * 4 + j;
-          const int r = r0 + q * 8 + half * 4 + j;
-          const bool seen = whole || (r >= row_lo && r <= row_hi);
-          const float pr = seen ? __builtin_amdgcn_exp2f(fmaf(s[e], a.scale_log2, ProbShift<T>::value - ls[j])) : 0.f;
-          s[e] = pr;
-          dp[e] = seen ? pr * (dp[e] - de[j]) : 0.f;
-        }
+        for (int kt = 0; kt < KT; ++kt)
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            const int e = q * 4 + j;
+            float pr = __builtin_amdgcn_exp2f(fmaf(s[kt][e], a.scale_log2, ProbShift<T>::value - ls[j]));
+            float ds = pr * (dp[kt][e] - de[j]);
+            if (!whole) {
+              const int r = r0 + q * 8 + half * 4 + j;
+              const bool seen = r >= row_lo[kt] && r <= row_hi[kt];
+              pr = seen ? pr : 0.f;
+              ds = seen ? ds : 0.f;
+            }
+            s[kt][e] = pr;
+            dp[kt][e] = ds;
+          }
       }
 #pragma unroll
       for (int t16 = 0; t16 < 2; ++t16) {
-        float x[8], y[8];
+        F pf[KT], df[KT];
 #pragma unroll
-        for (int e = 0; e < 8; ++e) {
-          x[e] = s[t16 * 8 + e];
-          y[e] = dp[t16 * 8 + e];
-          if (ProbShift<T>::value != 0.f) y[e] *= 1.f / 32768.f;
+        for (int kt = 0; kt < KT; ++kt) {
+          float x[8], y[8];
+#pragma unroll
+          for (int e = 0; e < 8; ++e) {
+            x[e] = s[kt][t16 * 8 + e];
+            y[e] = dp[kt][t16 * 8 + e];
+            if (ProbShift<T>::value != 0.f) y[e] *= 1.f / 32768.f;
+          }
+          pf[kt] = Frag<T>::pack(x);
+          df[kt] = Frag<T>::pack(y);
         }
-        const F pf = Frag<T>::pack(x), ds = Frag<T>::pack(y);
 #pragma unroll
         for (int dt = 0; dt < DT; ++dt) {
-          dv[dt] = Frag<T>::mma(L::cols_frag(stage + kTileBytes, n * 32 + t16 * 16, dt), pf, dv[dt]);
-          dk[dt] = Frag<T>::mma(L::cols_frag(stage, n * 32 + t16 * 16, dt), ds, dk[dt]);
+          const F dc = L::cols_frag(stage + kTileBytes, n * 32 + t16 * 16, dt);
+          const F qc = L::cols_frag(stage, n * 32 + t16 * 16, dt);
+#pragma unroll
+          for (int kt = 0; kt < KT; ++kt) {
+            dv[kt][dt] = Frag<T>::mma(dc, pf[kt], dv[kt][dt]);
+            dk[kt][dt] = Frag<T>::mma(qc, df[kt], dk[kt][dt]);
+          }
         }
       }
     }
   }
 
   const float dv_scale = ProbShift<T>::value != 0.f ? 1.f / 32768.f : 1.f;
-  if (tile_chunks > 1) {               // one of several partial sums
-    float* part = a.part + ((int64_t)bh * part_items(a) + part_item(a, of_sinks, nth)) * 2 * kTileRows * a.dim +
-                  (int64_t)(wave * 32 + (lane & 31)) * a.dim;
+  float* part = a.part + ((int64_t)bh * part_items(a) + part_item(a, of_sinks, nth)) * 2 * kTileKeys * a.dim +
+                (int64_t)(wave * 32 * KT + (lane & 31)) * a.dim;
+#pragma unroll
+  for (int kt = 0; kt < KT; ++kt) {
+    const int key = key0 + 32 * kt;
+    char* kp = a.dk.p + b * a.dk.batch + h * a.dk.head + key * a.dk.token;
+    char* vp = a.dv.p + b * a.dv.batch + h * a.dv.head + key * a.dv.token;
 #pragma unroll
     for (int dt = 0; dt < DT; ++dt)
 #pragma unroll
       for (int q = 0; q < 4; ++q) {
         const int d = dt * 32 + q * 8 + half * 4;
-        if (d < a.dim) {
-          float x[4], y[4];
+        float x[4], y[4];
 #pragma unroll
-          for (int j = 0; j < 4; ++j) {
-            x[j] = dk[dt][q * 4 + j] * a.scale;
-            y[j] = dv[dt][q * 4 + j] * dv_scale;
-          }
-          store_f32<float, 4>(part + d, x);
-          store_f32<float, 4>(part + (int64_t)kTileRows * a.dim + d, y);
+        for (int j = 0; j < 4; ++j) {
+          x[j] = dk[kt][dt][q * 4 + j] * a.scale;
+          y[j] = dv[kt][dt][q * 4 + j] * dv_scale;
+        }
+        if (d >= a.dim) continue;
+        if (tile_chunks > 1) {         // one of several partial sums
+          store_f32<float, 4>(part + kt * 32 * a.dim + d, x);
+          store_f32<float, 4>(part + (kTileKeys + kt * 32) * a.dim + d, y);
+        } else if (key < a.keys) {
+          store_f32<T, 4>(reinterpret_cast<T*>(kp) + d, x);
+          store_f32<T, 4>(reinterpret_cast<T*>(vp) + d, y);
         }
       }
-    return;
   }
-  if (key >= a.keys) return;
-  char* kp = a.dk.p + b * a.dk.batch + h * a.dk.head + key * a.dk.token;
-  char* vp = a.dv.p + b * a.dv.batch + h * a.dv.head + key * a.dv.token;
-#pragma unroll
-  for (int dt = 0; dt < DT; ++dt)
-#pragma unroll
-    for (int q = 0; q < 4; ++q) {
-      const int d = dt * 32 + q * 8 + half * 4;
-      float x[4], y[4];
-#pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        x[j] = dk[dt][q * 4 + j] * a.scale;
-        y[j] = dv[dt][q * 4 + j] * dv_scale;
-      }
-      if (d < a.dim) {
-        store_f32<T, 4>(reinterpret_cast<T*>(kp) + d, x);
-        store_f32<T, 4>(reinterpret_cast<T*>(vp) + d, y);
-      }
-    }
 }
 
 // Sums the partial dk and dv of the tiles that were worked on in chunks, in the chunks' order.  32 lanes per
 // key, four elements of dim per lane.
-template <typename T>
+template <typename T, int kTileKeys>
 __global__ __launch_bounds__(256) void attention_dkv_join_kernel(AttentionArgs a) {
   const int first_tile = a.sink_chunks > 1 ? 0 : a.sink_tiles;
   const int tiles = (a.chunks > 1 ? a.tiles : a.sink_tiles) - first_tile;
   const int64_t at = (int64_t)blockIdx.x * 8 + (threadIdx.x >> 5);
-  const int bh = (int)(at / ((int64_t)tiles * kTileRows));
+  const int bh = (int)(at / ((int64_t)tiles * kTileKeys));
   if (bh >= a.batch * a.kv_heads) return;
-  const int rest = (int)(at - (int64_t)bh * tiles * kTileRows);
-  const int tile = first_tile + rest / kTileRows, local = rest % kTileRows;
-  const int key = tile * kTileRows + local, d = (threadIdx.x & 31) * 4;
+  const int rest = (int)(at - (int64_t)bh * tiles * kTileKeys);
+  const int tile = first_tile + rest / kTileKeys, local = rest % kTileKeys;
+  const int key = tile * kTileKeys + local, d = (threadIdx.x & 31) * 4;
   if (key >= a.keys || d >= a.dim) return;
   const bool of_sinks = tile < a.sink_tiles;
   const int chunks = of_sinks ? a.sink_chunks : a.chunks;
   const int nth = of_sinks ? tile * chunks : (tile - a.sink_tiles) * chunks;
-  const float* part = a.part + (((int64_t)bh * part_items(a) + part_item(a, of_sinks, nth)) * 2 * kTileRows + local) * a.dim + d;
-  const int64_t other = (int64_t)kTileRows * a.dim;
+  const float* part = a.part + (((int64_t)bh * part_items(a) + part_item(a, of_sinks, nth)) * 2 * kTileKeys + local) * a.dim + d;
+  const int64_t other = (int64_t)kTileKeys * a.dim;
   float x[4] = {0.f, 0.f, 0.f, 0.f}, y[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll 4
   for (int c = 0; c < chunks; ++c) {
@@ -397,17 +427,24 @@ __global__ __launch_bounds__(256) void attention_dkv_join_kernel(AttentionArgs a
   store_f32<T, 4>(reinterpret_cast<T*>(a.dv.p + b * a.dv.batch + h * a.dv.head + key * a.dv.token) + d, y);
 }
 
+#ifndef KTSEL
+#define KTSEL 32
+#endif
+constexpr int keys_per_wave(int dtype, int dim_tiles) { return dtype == AT_DTYPE_F32 ? 32 : KTSEL; }
+template <typename T, int DT> constexpr int keys_per_wave() { return keys_per_wave(dtype_of<T>::value, DT); }
+
 // How dk and dv are cut up.  The rows that see a tile of keys are walked over in chunks of chunk_steps
 // steps; tiles with one chunk write their result, the others partial sums that a second kernel adds.
 // With a window a tile is seen by few rows, but a tile with sinks by all: such tiles are cut to the
 // others' length, or one workgroup per head would run on alone (window 1024 over 8192 tokens: 5.1 ms
 // instead of 1.3).  Where the tiles alone do not give every CU two workgroups, all are cut further.
-void chunk_plan(AttentionArgs& a) {
-  a.tiles = (int)cdiv64(a.keys, kTileRows);
+void chunk_plan(AttentionArgs& a, int tile_keys) {
+  a.tile_keys = tile_keys;
+  a.tiles = (int)cdiv64(a.keys, tile_keys);
   const int64_t rows = (int64_t)a.rows * a.group;
-  const int64_t near = (int64_t)(a.left + a.right + kTileRows) * a.group;
+  const int64_t near = (int64_t)(a.left + a.right + tile_keys) * a.group;
   const int64_t span = near < rows ? near : rows;              // of a tile without sinks
-  a.sink_tiles = span < rows ? (int)cdiv64(a.sinks, kTileRows) : 0;
+  a.sink_tiles = span < rows ? (int)cdiv64(a.sinks, tile_keys) : 0;
   int64_t steps = cdiv64(span, kStep) + 1;                     // the first step need not start at the first row
   const int64_t groups = (int64_t)a.tiles * a.batch * a.kv_heads;
   const int64_t want = 2 * device_cu_count();
@@ -424,17 +461,18 @@ void chunk_plan(AttentionArgs& a) {
 int64_t delta_bytes(const AttentionArgs& a) { return (int64_t)a.batch * a.kv_heads * a.row_pitch * 4; }
 
 int64_t part_bytes(const AttentionArgs& a) {
-  return (int64_t)a.batch * a.kv_heads * part_items(a) * 2 * kTileRows * a.dim * 4;
+  return (int64_t)a.batch * a.kv_heads * part_items(a) * 2 * a.tile_keys * a.dim * 4;
 }
 
 template <typename T, int DT>
 int launch(AttentionArgs a, hipStream_t stream) {
   const int64_t heads = (int64_t)a.batch * a.kv_heads;
-  chunk_plan(a);
+  constexpr int KT = keys_per_wave<T, DT>() / 32;
+  chunk_plan(a, kWaves * 32 * KT);
   const int64_t items = (int64_t)a.sink_tiles * a.sink_chunks + (int64_t)(a.tiles - a.sink_tiles) * a.chunks;
   const int64_t row_tiles = cdiv64((int64_t)a.rows * a.group, kTileRows);
   const int64_t joined = ((a.chunks > 1 ? a.tiles : a.sink_tiles) - (a.sink_chunks > 1 ? 0 : a.sink_tiles)) *
-                         (int64_t)kTileRows * heads;
+                         (int64_t)a.tile_keys * heads;
   if (!grid_fits(row_tiles * heads) || !grid_fits(items * heads) || !grid_fits(cdiv64(joined, 8))) return AT_ERR_DIM;
   int rc = AT_OK;
   if (a.rows > 0) {
@@ -444,10 +482,10 @@ int launch(AttentionArgs a, hipStream_t stream) {
     rc = launch_status();
     if (rc != AT_OK) return rc;
   }
-  hipLaunchKernelGGL((attention_dkv_kernel<T, DT>), dim3((unsigned)(items * heads)), dim3(kWaves * 64), 0, stream, a);
+  hipLaunchKernelGGL((attention_dkv_kernel<T, DT, KT>), dim3((unsigned)(items * heads)), dim3(kWaves * 64), 0, stream, a);
   rc = launch_status();
   if (rc != AT_OK || part_items(a) == 0) return rc;
-  hipLaunchKernelGGL((attention_dkv_join_kernel<T>), dim3((unsigned)cdiv64(joined, 8)), dim3(256), 0, stream, a);
+  hipLaunchKernelGGL((attention_dkv_join_kernel<T, kWaves * 32 * KT>), dim3((unsigned)cdiv64(joined, 8)), dim3(256), 0, stream, a);
   return launch_status();
 }
 
@@ -471,7 +509,7 @@ extern "C" {
 int64_t at_attention_bwd_workspace_bytes(const at_attention_t* shape) {
   AttentionArgs a;
   if (attention_args(shape, a) != AT_OK || a.keys == 0) return 0;
-  chunk_plan(a);
+  chunk_plan(a, kWaves * keys_per_wave(shape->dtype, (a.dim + 31) / 32));
   return delta_bytes(a) + part_bytes(a);
 }
 

@@ -37,9 +37,9 @@ __global__ __launch_bounds__(kWaves * 64, sizeof(T) == 2 ? 2 : 1) void attention
 
   const int lane = threadIdx.x & 63, half = lane >> 5;
   const int wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
-  // the last rows of a causal sequence see the most keys: their workgroups start first
-  const int tile_id = a.tiles - 1 - (int)(blockIdx.x % a.tiles);
-  const int bh = blockIdx.x / a.tiles;
+  const Piece piece = piece_of(blockIdx.x, a.tiles, a.batch * a.kv_heads);
+  const int tile_id = a.tiles - 1 - piece.rank;    // the last rows of a causal sequence see the most keys
+  const int bh = piece.bh;
   const int b = bh / a.kv_heads, h = bh - b * a.kv_heads;
   const Sequence seq = sequence_of(a, b);
   const int live_rows = seq.live * a.group, all_rows = a.rows * a.group;
