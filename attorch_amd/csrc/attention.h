@@ -130,11 +130,13 @@ template <> struct Frag<float> {
   }
 };
 
-// Probabilities of fp16 inputs are multiplied by 2^15 before they are rounded to fp16 (they are at
-// most 1, so nothing overflows): without it those of a long flat row would be subnormal numbers.
-// bf16 has fp32's exponents and needs no such factor.
-template <typename T> struct ProbShift { static constexpr float value = 0.f; };
-template <> struct ProbShift<f16_t> { static constexpr float value = 15.f; };
+// Probabilities of fp16 inputs are multiplied by 2^value before they are rounded to fp16: without it
+// those of a long flat row would be subnormal numbers.  In the backward pass they are at most 1, in the
+// forward pass at most 2^kSlack (see there), so nothing overflows.  bf16 has fp32's exponents and needs
+// no such factor.
+constexpr float kSlack = 8.f;
+template <typename T> struct ProbShift { static constexpr float forward = 0.f, backward = 0.f; };
+template <> struct ProbShift<f16_t> { static constexpr float forward = 15.f - kSlack, backward = 15.f; };
 
 __device__ __forceinline__ f32x16 zero_acc() {
   f32x16 z;

@@ -320,7 +320,7 @@ __global__ __launch_bounds__(kWaves * 64, KT == 1 && sizeof(T) == 2 ? 2 : 1) voi
 #pragma unroll
           for (int j = 0; j < 4; ++j) {
             const int e = q * 4 + j;
-            float pr = __builtin_amdgcn_exp2f(fmaf(s[kt][e], a.scale_log2, ProbShift<T>::value - ls[j]));
+            float pr = __builtin_amdgcn_exp2f(fmaf(s[kt][e], a.scale_log2, ProbShift<T>::backward - ls[j]));
             float ds = pr * (dp[kt][e] - de[j]);
             if (!whole) {
               const int r = r0 + q * 8 + half * 4 + j;
@@ -342,7 +342,7 @@ __global__ __launch_bounds__(kWaves * 64, KT == 1 && sizeof(T) == 2 ? 2 : 1) voi
           for (int e = 0; e < 8; ++e) {
             x[e] = s[kt][t16 * 8 + e];
             y[e] = dp[kt][t16 * 8 + e];
-            if (ProbShift<T>::value != 0.f) y[e] *= 1.f / 32768.f;
+            if (ProbShift<T>::backward != 0.f) y[e] *= 1.f / 32768.f;
           }
           pf[kt] = Frag<T>::pack(x);
           df[kt] = Frag<T>::pack(y);
@@ -361,7 +361,7 @@ __global__ __launch_bounds__(kWaves * 64, KT == 1 && sizeof(T) == 2 ? 2 : 1) voi
     }
   }
 
-  const float dv_scale = ProbShift<T>::value != 0.f ? 1.f / 32768.f : 1.f;
+  const float dv_scale = ProbShift<T>::backward != 0.f ? 1.f / 32768.f : 1.f;
   float* part = a.part + ((int64_t)bh * part_items(a) + part_item(a, of_sinks, nth)) * 2 * kTileKeys * a.dim +
                 (int64_t)(wave * 32 * KT + (lane & 31)) * a.dim;
 #pragma unroll

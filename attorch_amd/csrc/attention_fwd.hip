@@ -113,44 +113,45 @@ __global__ __launch_bounds__(kWaves * 64, sizeof(T) == 2 ? 2 : 1) void attention
 #pragma unroll
       for (int ks = 0; ks < L::kSteps; ++ks) s[n] = Frag<T>::mma(L::rows_frag(stage, n * 32, ks), qf[ks], s[n]);
     }
+    // keys of the lane relative to its first one, as constants: 8 apart, 4 in a row
     const bool whole = k0 >= last - a.left && k0 + kKeys - 1 <= min(first + a.right, seq.len - 1);
-    if (whole) {
-#pragma unroll
-      for (int n = 0; n < 2; ++n)
-#pragma unroll
-        for (int e = 0; e < 16; ++e) s[n][e] *= a.scale_log2;
-    } else {
+    if (!whole) {
+      const int key = k0 + half * 4;
+      const int lo = see_lo - key, hi = see_hi - key, sinks = see_sinks - key;
 #pragma unroll
       for (int n = 0; n < 2; ++n)
 #pragma unroll
         for (int e = 0; e < 16; ++e) {
-          const int key = k0 + n * 32 + acc_row(e, half);
-          const bool seen = (key >= see_lo && key <= see_hi) || key < see_sinks;
-          s[n][e] = seen ? s[n][e] * a.scale_log2 : -INFINITY;
+          const int c = n * 32 + acc_row(e, 0);
+          s[n][e] = (c >= lo && c <= hi) || c < sinks ? s[n][e] : -INFINITY;
         }
     }
-    float top = s[0][0];
+    float top = fmaxf(s[0][0], s[1][0]);
 #pragma unroll
-    for (int n = 0; n < 2; ++n)
+    for (int e = 1; e < 16; ++e) top = fmaxf(fmaxf(top, s[0][e]), s[1][e]);
+    top = half_max(top) * a.scale_log2;
+    // The exponentials are taken relative to a maximum that may lag behind by kSlack: any reference gives
+    // the same result, and moving it costs a pass over the output, which now is rare.
+    if (__any(top > m + kSlack)) {
+      const float old = m;
+      m = fmaxf(m, top);
+      const float shrink = m == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(old - m);
+      l *= shrink;
 #pragma unroll
-      for (int e = 0; e < 16; ++e) top = fmaxf(top, s[n][e]);
-    top = fmaxf(m, half_max(top));
-    const float base = top == -INFINITY ? 0.f : top - ProbShift<T>::value;   // a row that has seen nothing yet
-    const float shrink = __builtin_amdgcn_exp2f(m - (top == -INFINITY ? 0.f : top));
-    m = top;
-    float sum = 0.f;
+      for (int dt = 0; dt < DT; ++dt)
+#pragma unroll
+        for (int e = 0; e < 16; ++e) o[dt][e] *= shrink;
+    }
+    const float base = m == -INFINITY ? 0.f : ProbShift<T>::forward - m;   // -inf: the row has seen nothing yet
+    float sum[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
     for (int n = 0; n < 2; ++n)
 #pragma unroll
       for (int e = 0; e < 16; ++e) {
-        s[n][e] = __builtin_amdgcn_exp2f(s[n][e] - base);
-        sum += s[n][e];
+        s[n][e] = __builtin_amdgcn_exp2f(fmaf(s[n][e], a.scale_log2, base));
+        sum[e & 3] += s[n][e];
       }
-    l = l * shrink + sum;
-#pragma unroll
-    for (int dt = 0; dt < DT; ++dt)
-#pragma unroll
-      for (int e = 0; e < 16; ++e) o[dt][e] *= shrink;
+    l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
 #pragma unroll
     for (int ks = 0; ks < kKeys / 16; ++ks) {
       float pr[8];
@@ -170,7 +171,7 @@ __global__ __launch_bounds__(kWaves * 64, sizeof(T) == 2 ? 2 : 1) void attention
 #pragma unroll
     for (int dt = 0; dt < DT; ++dt) o[dt] = zero_acc();
   }
-  const float lse = valid ? m + __builtin_amdgcn_logf(l) - ProbShift<T>::value : INFINITY;
+  const float lse = valid ? m + __builtin_amdgcn_logf(l) - ProbShift<T>::forward : INFINITY;
   if (a.splits > 1) {
     if (row >= all_rows) return;
     float* part = a.part + (((int64_t)split * a.batch * a.kv_heads + bh) * all_rows + row) * a.dim;
