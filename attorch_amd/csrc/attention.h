@@ -74,18 +74,21 @@ __device__ __forceinline__ KeyRange keys_of(const AttentionArgs& a, const Sequen
 }
 
 // Which piece of which head a workgroup takes: the pieces of a head stay on one XCD (workgroups go to
-// the 8 XCDs in turn), whose L2 then holds the head's keys and values, and come in order of rank, which
-// the callers make the order of falling work.  Heads beyond a multiple of 8 are spread over all XCDs,
-// every other round of 8 in reverse, so that none gets the heavier piece each time.  (Heads in plain
-// order leave pieces of equal rank to the same XCD: causal, 32 pieces, 38 % of the CU time was idle.)
+// the 8 XCDs in turn), whose L2 then holds the head's keys and values, and four heads at a time come in
+// order of rank, which the callers make the order of falling work.  Heads beyond a multiple of 8 are
+// spread over all XCDs, every other round of 8 in reverse, so that none gets the heavier piece each
+// time.  (Heads in plain order leave pieces of equal rank to the same XCD: causal, 32 pieces, 38 % of the
+// CU time was idle.)
 struct Piece {
   int rank, bh;
 };
 __device__ __forceinline__ Piece piece_of(int id, int pieces, int heads) {
   const int whole = heads & ~7;
   if (id < whole * pieces) {
-    const int n = (id >> 3) / pieces;
-    return {(id >> 3) - n * pieces, n * 8 + (id & 7)};
+    const int n = id >> 3, block = n / (4 * pieces);
+    const int size = min(whole / 8 - block * 4, 4), at = n - block * 4 * pieces;
+    const int rank = at / size;
+    return {rank, (block * 4 + at - rank * size) * 8 + (id & 7)};
   }
   const int rest = heads - whole;
   id -= whole * pieces;
@@ -158,6 +161,14 @@ __device__ __forceinline__ float half_sum(float v) {
 // Row of a 32 x 32 result that register e of this lane holds.
 __device__ __forceinline__ int acc_row(int e, int half) { return (e >> 2) * 8 + half * 4 + (e & 3); }
 
+// Global -> LDS without passing through registers, as lds_dma_16, with a uniform part of the offset.
+__device__ __forceinline__ void dma_16(const i32x4& rsrc, int lane_bytes, int uniform_bytes, const char* lds_dst) {
+  const unsigned m0 = (unsigned)__builtin_amdgcn_readfirstlane((int)(uintptr_t)lds_dst);
+  asm volatile("s_mov_b32 m0, %0\n\tbuffer_load_dwordx4 %1, %2, %3 offen lds" ::"s"(m0), "v"(lane_bytes), "s"(rsrc),
+               "s"(uniform_bytes)
+               : "m0");
+}
+
 // ---- tiles in LDS -------------------------------------------------------------------------
 // [ROWS][dim] tile, dim padded with zeros to DT * 32 elements, rows of 64 (DT <= 2) or 128 elements.
 // The 16-byte chunks of a row are permuted by an XOR with spread(row) so that both kinds of
@@ -214,22 +225,46 @@ template <typename T, int DT> struct Tile {
     }
   }
 
-  // Asynchronous copy of ROWS rows into `tile`, shared among NW waves.  offset(row) is the row's byte
-  // offset from the resource's base, negative for a row that is to be zeros.
+  // ---- asynchronous copies of ROWS rows into a tile, shared among NW waves ----
+  // A wave moves kLoadRows rows with one load and NW * kLoadRows with all waves' loads (a round).  The
+  // chunk a lane moves is the same in every round but for the part of spread() that the round sets.
+  static constexpr int kLoadRows = 1024 / kPitch;
+  template <int NW> static __device__ __forceinline__ int lane_row() {
+    return ((int)threadIdx.x >> 6) * kLoadRows + ((int)threadIdx.x & 63) / kChunks;
+  }
+  template <int NW> static __device__ __forceinline__ int lane_byte(int round) {
+    const int chunk = ((int)threadIdx.x & 63) % kChunks;
+    return (chunk ^ spread(lane_row<NW>()) ^ spread(round * NW * kLoadRows)) << 4;
+  }
+  // Byte offset of a lane's part of a row that lies `row_bytes` behind the tile's first: kOobOffset where the
+  // row has no such part.
+  template <int NW> static __device__ __forceinline__ int lane_offset(int row_bytes, int dim_bytes, int round) {
+    const int byte = lane_byte<NW>(round);
+    return byte < dim_bytes ? row_bytes + byte : kOobOffset;
+  }
+
+  // Every row exists, and rounds lie `round_bytes` apart: lane offsets do not change from tile to tile.
+  template <int ROWS, int NW>
+  static __device__ __forceinline__ void fetch_all(const i32x4& rsrc, const int (&offset)[2], int round_bytes, char* tile) {
+    constexpr int kRounds = ROWS / (NW * kLoadRows);
+    static_assert(kRounds * NW * kLoadRows == ROWS, "every wave issues the same number of loads");
+    char* dst = tile + __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6) * 1024;
+#pragma unroll
+    for (int n = 0; n < kRounds; ++n)
+      dma_16(rsrc, offset[spread(n * NW * kLoadRows) != 0], n * round_bytes, dst + n * NW * 1024);
+  }
+
+  // offset(row) is the row's byte offset from the tile's first, negative for a row that is to be zeros.
   template <int ROWS, int NW, typename Offset>
   static __device__ __forceinline__ void fetch(const i32x4& rsrc, int dim_bytes, char* tile, Offset&& offset) {
-    constexpr int kLoads = ROWS * kPitch / 1024;
-    static_assert(kLoads % NW == 0, "every wave issues the same number of loads");
-    const int lane = threadIdx.x & 63;
-    const int wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
+    constexpr int kRounds = ROWS / (NW * kLoadRows);
+    char* dst = tile + __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6) * 1024;
+    int row = lane_row<NW>();
+    asm volatile("" : "+v"(row));      // nothing of this rare path is to be kept in registers between tiles
 #pragma unroll
-    for (int n = 0; n < kLoads / NW; ++n) {
-      const int load = n * NW + wave;
-      const int index = load * 64 + lane;
-      const int row = index / kChunks;
-      const int byte = ((index % kChunks) ^ spread(row)) << 4;
-      const int off = offset(row);
-      lds_dma_16(rsrc, off >= 0 && byte < dim_bytes ? off + byte : kOobOffset, tile + load * 1024);
+    for (int n = 0; n < kRounds; ++n) {
+      const int off = offset(row + n * NW * kLoadRows);
+      dma_16(rsrc, off >= 0 ? lane_offset<NW>(off, dim_bytes, n) : kOobOffset, 0, dst + n * NW * 1024);
     }
   }
 };

@@ -100,12 +100,22 @@ __global__ __launch_bounds__(kWaves * 64, sizeof(T) == 2 ? 2 : 1) void attention
   const char* vb = a.v.p + b * a.v.batch + h * a.v.head;
   const int dim_bytes = a.dim * (int)sizeof(T);
   auto first_key = [&](int t) { return (t < sink_tiles ? t : t - sink_tiles + tiles_lo) * kStep; };
+  const int key_off = L::template lane_row<kWaves>() * (int)a.k.token, val_off = L::template lane_row<kWaves>() * (int)a.v.token;
+  const int key_offs[2] = {L::template lane_offset<kWaves>(key_off, dim_bytes, 0),
+                           L::template lane_offset<kWaves>(key_off, dim_bytes, 1)};
+  const int val_offs[2] = {L::template lane_offset<kWaves>(val_off, dim_bytes, 0),
+                           L::template lane_offset<kWaves>(val_off, dim_bytes, 1)};
   auto fetch = [&](int t, char* stage) {
     const int k0 = first_key(t);
-    L::template fetch<kStep, kWaves>(open_rsrc(kb + k0 * a.k.token), dim_bytes, stage,
-                                     [&](int r) { return range.has(k0 + r) ? r * (int)a.k.token : -1; });
-    L::template fetch<kStep, kWaves>(open_rsrc(vb + k0 * a.v.token), dim_bytes, stage + kTileBytes,
-                                     [&](int r) { return range.has(k0 + r) ? r * (int)a.v.token : -1; });
+    const i32x4 kr = open_rsrc(kb + k0 * a.k.token), vr = open_rsrc(vb + k0 * a.v.token);
+    if (k0 >= range.lo && k0 + kStep <= range.hi) {
+      L::template fetch_all<kStep, kWaves>(kr, key_offs, kWaves * L::kLoadRows * (int)a.k.token, stage);
+      L::template fetch_all<kStep, kWaves>(vr, val_offs, kWaves * L::kLoadRows * (int)a.v.token, stage + kTileBytes);
+    } else {
+      L::template fetch<kStep, kWaves>(kr, dim_bytes, stage, [&](int r) { return range.has(k0 + r) ? r * (int)a.k.token : -1; });
+      L::template fetch<kStep, kWaves>(vr, dim_bytes, stage + kTileBytes,
+                                      [&](int r) { return range.has(k0 + r) ? r * (int)a.v.token : -1; });
+    }
   };
 
   if (tiles > 0) fetch(0, lds);
@@ -266,21 +276,36 @@ __global__ __launch_bounds__(kWaves * 64, KT == 1 && sizeof(T) == 2 ? 2 : 1) voi
   const float* delta = a.delta + (int64_t)bh * a.row_pitch;
   const int dim_bytes = a.dim * (int)sizeof(T);
   const float per_group = 1.f / (float)a.group;
+  // rest + r is small, and the quotient's error far below the 0.5 / group that would change it
+  auto offset = [&](int rest, int r, const Strided& x) {
+    const int n = rest + r, token = (int)(((float)n + 0.5f) * per_group);
+    return token * (int)x.token + (n - token * a.group) * (int)x.head;
+  };
+  // a group that divides the rows of a round: tiles and rounds start at a token's first head
+  constexpr int kRound = kWaves * L::kLoadRows;
+  const bool even = kRound % a.group == 0;
+  const int q_off = offset(0, L::template lane_row<kWaves>(), a.q), d_off = offset(0, L::template lane_row<kWaves>(), a.dout);
+  const int q_offs[2] = {L::template lane_offset<kWaves>(q_off, dim_bytes, 0),
+                         L::template lane_offset<kWaves>(q_off, dim_bytes, 1)};
+  const int d_offs[2] = {L::template lane_offset<kWaves>(d_off, dim_bytes, 0),
+                         L::template lane_offset<kWaves>(d_off, dim_bytes, 1)};
+  const int round_tokens = kRound / a.group;
   auto fetch = [&](int t, char* stage) {
     const int r0 = t * kStep;
     const int i0 = r0 / a.group, rest = r0 - i0 * a.group;
-    // rest + r is small, and the quotient's error far below the 0.5 / group that would change it
-    auto offset = [&](int r, const Strided& x) {
-      const int n = rest + r, token = (int)(((float)n + 0.5f) * per_group);
-      return r0 + r < live_rows ? token * (int)x.token + (n - token * a.group) * (int)x.head : -1;
-    };
-    L::template fetch<kStep, kWaves>(open_rsrc(qb + i0 * a.q.token), dim_bytes, stage,
-                                     [&](int r) { return offset(r, a.q); });
-    L::template fetch<kStep, kWaves>(open_rsrc(db + i0 * a.dout.token), dim_bytes, stage + kTileBytes,
-                                     [&](int r) { return offset(r, a.dout); });
+    const i32x4 qr = open_rsrc(qb + i0 * a.q.token), dr = open_rsrc(db + i0 * a.dout.token);
+    if (even && r0 + kStep <= live_rows) {
+      L::template fetch_all<kStep, kWaves>(qr, q_offs, round_tokens * (int)a.q.token, stage);
+      L::template fetch_all<kStep, kWaves>(dr, d_offs, round_tokens * (int)a.dout.token, stage + kTileBytes);
+    } else {
+      L::template fetch<kStep, kWaves>(qr, dim_bytes, stage,
+                                       [&](int r) { return r0 + r < live_rows ? offset(rest, r, a.q) : -1; });
+      L::template fetch<kStep, kWaves>(dr, dim_bytes, stage + kTileBytes,
+                                       [&](int r) { return r0 + r < live_rows ? offset(rest, r, a.dout) : -1; });
+    }
     if (wave < 2)   // 64 values each: lanes 0..15 move 16 bytes, the others write zeros behind them
-      lds_dma_16(open_rsrc((const char*)((wave == 0 ? lse : delta) + r0)), lane < 16 ? lane * 16 : kOobOffset,
-                 stage + 2 * kTileBytes + wave * 1024);
+      dma_16(open_rsrc((const char*)((wave == 0 ? lse : delta) + r0)), lane < 16 ? lane * 16 : kOobOffset, 0,
+             stage + 2 * kTileBytes + wave * 1024);
   };
 
   if (begin < end) fetch(begin, lds);

@@ -88,12 +88,22 @@ __global__ __launch_bounds__(kWaves * 64, sizeof(T) == 2 ? 2 : 1) void attention
   const char* vb = a.v.p + b * a.v.batch + h * a.v.head;
   const int dim_bytes = a.dim * (int)sizeof(T);
   auto first_key = [&](int t) { return (t < sink_tiles ? t : t - sink_tiles + tiles_lo) * kKeys; };
+  const int key_off = L::template lane_row<kWaves>() * (int)a.k.token, val_off = L::template lane_row<kWaves>() * (int)a.v.token;
+  const int key_offs[2] = {L::template lane_offset<kWaves>(key_off, dim_bytes, 0),
+                           L::template lane_offset<kWaves>(key_off, dim_bytes, 1)};
+  const int val_offs[2] = {L::template lane_offset<kWaves>(val_off, dim_bytes, 0),
+                           L::template lane_offset<kWaves>(val_off, dim_bytes, 1)};
   auto fetch = [&](int t, char* stage) {
     const int k0 = first_key(t);
-    L::template fetch<kKeys, kWaves>(open_rsrc(kb + k0 * a.k.token), dim_bytes, stage,
-                                     [&](int r) { return range.has(k0 + r) ? r * (int)a.k.token : -1; });
-    L::template fetch<kKeys, kWaves>(open_rsrc(vb + k0 * a.v.token), dim_bytes, stage + kTileBytes,
-                                     [&](int r) { return range.has(k0 + r) ? r * (int)a.v.token : -1; });
+    const i32x4 kr = open_rsrc(kb + k0 * a.k.token), vr = open_rsrc(vb + k0 * a.v.token);
+    if (k0 >= range.lo && k0 + kKeys <= range.hi) {
+      L::template fetch_all<kKeys, kWaves>(kr, key_offs, kWaves * L::kLoadRows * (int)a.k.token, stage);
+      L::template fetch_all<kKeys, kWaves>(vr, val_offs, kWaves * L::kLoadRows * (int)a.v.token, stage + kTileBytes);
+    } else {
+      L::template fetch<kKeys, kWaves>(kr, dim_bytes, stage, [&](int r) { return range.has(k0 + r) ? r * (int)a.k.token : -1; });
+      L::template fetch<kKeys, kWaves>(vr, dim_bytes, stage + kTileBytes,
+                                      [&](int r) { return range.has(k0 + r) ? r * (int)a.v.token : -1; });
+    }
   };
 
   if (t_begin < t_end) fetch(t_begin, lds);
