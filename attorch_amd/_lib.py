@@ -81,9 +81,9 @@ PROTOTYPES = {
     # the first argument of these is a ctypes structure, passed by reference (attention.py, rotary.py)
     'at_attention_row_pitch': (L, [L, L, L]),
     'at_attention_fwd_workspace_bytes': (L, [P]),
-    'at_attention_fwd': (I, [P, P, P, P, P, P, P, P, L, P]),
+    'at_attention_fwd': (I, [P] * 10 + [L, P]),
     'at_attention_bwd_workspace_bytes': (L, [P]),
-    'at_attention_bwd': (I, [P, P, P, P, P, P, P, P, P, P, P, P, L, P]),
+    'at_attention_bwd': (I, [P] * 14 + [L, P]),
     'at_rotary': (I, [P, P, P, P, P, P, P, P, P]),
 }
 

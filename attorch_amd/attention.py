@@ -9,7 +9,8 @@ sequences' lengths, for training steps, prompts and single tokens alike.
 """
 
 import ctypes
-from typing import Any, Optional, Tuple
+import functools
+from typing import Any, Optional, Sequence, Tuple
 
 import torch
 from torch import Tensor
@@ -21,7 +22,6 @@ from . import _lib
 from .utils import get_output_dtype
 
 MAX_HEAD_DIM = 128
-_NO_STRIDES = (0, 0, 0)
 
 
 class _Shape(ctypes.Structure):
@@ -30,79 +30,68 @@ class _Shape(ctypes.Structure):
     """
     _fields_ = ([(name, ctypes.c_int64) for name in ('batch', 'heads', 'kv_heads', 'rows', 'keys', 'dim', 'window',
                                                      'sinks')] +
-                [('strides', ctypes.c_int64 * 24), ('lengths', ctypes.c_void_p), ('query_lengths', ctypes.c_void_p),
-                 ('scale', ctypes.c_float), ('causal', ctypes.c_int), ('dtype', ctypes.c_int),
-                 ('lengths_int64', ctypes.c_int)])
+                [('strides', ctypes.c_int64 * 24), ('scale', ctypes.c_float), ('causal', ctypes.c_int),
+                 ('dtype', ctypes.c_int), ('lengths_int64', ctypes.c_int)])
 
 
-def _readable(tensor: Tensor, group: int) -> bool:
+# A tensor's layout: (shape, stride, dtype, whether its first byte lies on a 16-byte boundary)
+Layout = Tuple[torch.Size, Tuple[int, ...], torch.dtype, bool]
+
+
+def _layout(tensor: Tensor) -> Layout:
+    return tensor.shape, tensor.stride(), tensor.dtype, tensor.data_ptr() % 16 == 0
+
+
+def _readable(layout: Layout, group: int) -> bool:
     """
-    Whether the kernels can read the tensor where it lies: whole features, everything on 16-byte
-    boundaries, and a tile's tokens, of `group` heads, within the 31 bits of a buffer offset.
+    Whether the kernels can read a tensor where it lies: whole vectors of features, everything on
+    16-byte boundaries, and a tile's tokens, of `group` heads, within the 31 bits of a buffer offset.
     """
-    stride = tensor.stride()
-    size = tensor.element_size()
-    aligned = 16 // size
-    return (stride[3] == 1 and tensor.data_ptr() % 16 == 0 and
-            all(st % aligned == 0 or extent <= 1 for st, extent in zip(stride, tensor.shape[:3])) and
+    shape, stride, dtype, aligned = layout
+    size = dtype.itemsize
+    return (aligned and stride[3] == 1 and shape[3] % 8 == 0 and
+            all(st * size % 16 == 0 or extent <= 1 for st, extent in zip(stride, shape[:3])) and
             (160 * stride[2] + (group - 1) * stride[1]) * size < (1 << 31) - 1024)
 
 
-def _for_kernel(tensor: Tensor, dim: int, group: int) -> Tensor:
+def _for_kernel(tensor: Tensor, dtype: torch.dtype, group: int) -> Tensor:
     """
     The tensor itself where the kernels can read it, otherwise a copy in [batch, tokens, heads, dim]
-    order, its features padded with zeros to `dim`.
+    order, its features padded with zeros to whole vectors.
     """
-    if tensor.shape[3] == dim and _readable(tensor, group):
+    tensor = tensor.to(dtype)
+    if _readable(_layout(tensor), group):
         return tensor
-    tensor = tensor.transpose(1, 2)
-    if tensor.shape[3] != dim:
-        tensor = F.pad(tensor, (0, dim - tensor.shape[3]))
-    tensor = tensor.contiguous()
-    return (tensor if tensor.data_ptr() % 16 == 0 else tensor.clone()).transpose(1, 2)
+    return F.pad(tensor.transpose(1, 2), (0, -tensor.shape[3] % 8)).clone(
+        memory_format=torch.contiguous_format).transpose(1, 2)
 
 
-def _strides(tensor: Tensor) -> Tuple[int, int, int]:
+def _strides(shape: Sequence[int], stride: Sequence[int]) -> Tuple[int, int, int]:
     """
     Strides of batch, heads and tokens; 0 for an extent of one, whose stride is arbitrary.
     """
-    shape, stride = tensor.shape, tensor.stride()
     return (stride[0] if shape[0] > 1 else 0, stride[1] if shape[1] > 1 else 0, stride[2] if shape[2] > 1 else 0)
 
 
-def _like(tensor: Tensor) -> Tensor:
-    """
-    New tensor for a gradient of `tensor`: in its layout where that is dense.
-    """
-    grad = torch.empty_like(tensor)
-    if _readable(grad, 1):
-        return grad
-    batch, heads, tokens, dim = tensor.shape
-    return torch.empty((batch, tokens, heads, dim), device=tensor.device, dtype=tensor.dtype).transpose(1, 2)
-
-
-def _check(query: Tensor, key: Tensor, value: Tensor, lengths: Optional[Tensor], query_lengths: Optional[Tensor],
+def _check(query: Layout, key: Layout, value: Layout, lengths: Optional[Layout], query_lengths: Optional[Layout],
            window: Optional[int], num_sinks: int, scale: Optional[float]) -> None:
     """
     Refuses what the kernels do not compute, before anything is launched.
     """
-    assert query.ndim == 4 and key.ndim == 4 and value.ndim == 4, \
-        f'Query, key and value must be [batch, heads, tokens, head_dim], received {tuple(query.shape)}, ' \
-        f'{tuple(key.shape)} and {tuple(value.shape)}'
-    assert key.shape == value.shape, \
-        f'Key ({tuple(key.shape)}) and value ({tuple(value.shape)}) must have the same shape'
-    assert query.shape[0] == key.shape[0] and query.shape[3] == key.shape[3], \
-        f'Incompatible query ({tuple(query.shape)}) and key ({tuple(key.shape)}) shape'
-    assert key.shape[1] > 0 and query.shape[1] > 0 and query.shape[1] % key.shape[1] == 0, \
-        f'The number of query heads ({query.shape[1]}) must be a multiple of that of key heads ({key.shape[1]})'
-    if query.shape[2] > key.shape[2]:
-        raise RuntimeError(f'Queries are the last tokens of their sequences: expected at most {key.shape[2]} of them, '
-                           f'as many as keys, received {query.shape[2]}')
-    if not 1 <= query.shape[3] <= MAX_HEAD_DIM:
-        raise RuntimeError(f'Head dimension {query.shape[3]} is not supported; it must be between 1 and {MAX_HEAD_DIM}')
-    if key.dtype is not query.dtype or value.dtype is not query.dtype:
-        raise RuntimeError(f'Query, key and value must have the same dtype, received {query.dtype}, {key.dtype} and '
-                           f'{value.dtype}')
+    (q, _, dtype, _), (k, _, k_dtype, _), (v, _, v_dtype, _) = query, key, value
+    assert len(q) == 4 and len(k) == 4 and len(v) == 4, \
+        f'Query, key and value must be [batch, heads, tokens, head_dim], received {tuple(q)}, {tuple(k)} and {tuple(v)}'
+    assert k == v, f'Key ({tuple(k)}) and value ({tuple(v)}) must have the same shape'
+    assert q[0] == k[0] and q[3] == k[3], f'Incompatible query ({tuple(q)}) and key ({tuple(k)}) shape'
+    assert k[1] > 0 and q[1] > 0 and q[1] % k[1] == 0, \
+        f'The number of query heads ({q[1]}) must be a multiple of that of key heads ({k[1]})'
+    if q[2] > k[2]:
+        raise RuntimeError(f'Queries are the last tokens of their sequences: expected at most {k[2]} of them, '
+                           f'as many as keys, received {q[2]}')
+    if not 1 <= q[3] <= MAX_HEAD_DIM:
+        raise RuntimeError(f'Head dimension {q[3]} is not supported; it must be between 1 and {MAX_HEAD_DIM}')
+    if k_dtype is not dtype or v_dtype is not dtype:
+        raise RuntimeError(f'Query, key and value must have the same dtype, received {dtype}, {k_dtype} and {v_dtype}')
     if window is not None and window < 1:
         raise RuntimeError(f'The window must hold at least one token, received {window}')
     if num_sinks < 0:
@@ -112,23 +101,74 @@ def _check(query: Tensor, key: Tensor, value: Tensor, lengths: Optional[Tensor],
     for name, counts in (('lengths', lengths), ('query_lengths', query_lengths)):
         if counts is None:
             continue
-        if counts.dtype not in (torch.int32, torch.int64):
-            raise RuntimeError(f'{name} must be int32 or int64, received {counts.dtype}')
-        assert counts.shape == query.shape[:1], \
-            f'{name} must have one entry per sequence ({query.shape[0]}), received shape {tuple(counts.shape)}'
+        if counts[2] not in (torch.int32, torch.int64):
+            raise RuntimeError(f'{name} must be int32 or int64, received {counts[2]}')
+        assert tuple(counts[0]) == (q[0],), \
+            f'{name} must have one entry per sequence ({q[0]}), received shape {tuple(counts[0])}'
 
 
-def _shape_of(query: Tensor, key: Tensor, value: Tensor, others: Tuple[Tuple[int, int, int], ...],
-              counts: Tuple[Optional[Tensor], Optional[Tensor]], options: Tuple[bool, int, int, float]) -> _Shape:
-    batch, heads, rows, dim = query.shape
-    causal, window, num_sinks, scale = options
-    strides = [*_strides(query), *_strides(key), *_strides(value)]
-    for other in others:
-        strides += other
-    some = counts[0] if counts[0] is not None else counts[1]
-    return _Shape(batch, heads, key.shape[1], rows, key.shape[2], dim, window, num_sinks,
-                  (ctypes.c_int64 * 24)(*strides), _lib.ptr(counts[0]), _lib.ptr(counts[1]), scale, causal,
-                  _lib.dtype_id(query.dtype), int(some is not None and some.dtype is torch.int64))
+class _Plan:
+    """
+    What a forward call of given layouts and options passes on: nothing in it belongs to a tensor.
+    """
+    __slots__ = ('direct', 'shape', 'ref', 'group', 'output_shape', 'lse_size', 'workspace_bytes', 'scale')
+
+
+@functools.lru_cache(maxsize=4096)
+def _forward_plan(query: Layout, key: Layout, value: Layout, lengths: Optional[Layout], query_lengths: Optional[Layout],
+                  causal: bool, window: Optional[int], num_sinks: int, scale: Optional[float],
+                  dtype: torch.dtype, device: int) -> _Plan:
+    """
+    Checks the arguments and describes the call; `dtype` is the one to compute in, and the workspace
+    depends on the device.  Remembered by layouts and options, since a program repeats few of them and
+    the description takes longer than a small call's kernels.
+    """
+    _check(query, key, value, lengths, query_lengths, window, num_sinks, scale)
+    batch, heads, rows, dim = query[0]
+    kv_heads, keys = key[0][1:3]
+    plan = _Plan()
+    plan.group = heads // kv_heads
+    plan.scale = dim ** -0.5 if scale is None else scale
+    counts = [c for c in (lengths, query_lengths) if c is not None]
+    plan.direct = (query[2] is dtype and _readable(query, plan.group) and _readable(key, 1) and _readable(value, 1) and
+                   all(c[1] == (1,) or batch <= 1 for c in counts) and len({c[2] for c in counts}) <= 1)
+    if not plan.direct:
+        return plan
+    plan.output_shape = (batch, rows, heads, dim)
+    strides = [*_strides(*query[:2]), *_strides(*key[:2]), *_strides(*value[:2]), rows * heads * dim, dim, heads * dim]
+    plan.shape = _Shape(batch, heads, kv_heads, rows, keys, dim, min(window or 0, 1 << 40), min(num_sinks, 1 << 40),
+                        (ctypes.c_int64 * 24)(*strides), plan.scale, bool(causal), _lib.dtype_id(dtype),
+                        int(bool(counts) and counts[0][2] is torch.int64))
+    plan.ref = ctypes.byref(plan.shape)
+    lib = _lib.load()
+    plan.lse_size = batch * kv_heads * lib.at_attention_row_pitch(rows, heads, kv_heads)
+    plan.workspace_bytes = lib.at_attention_fwd_workspace_bytes(plan.ref)
+    return plan
+
+
+@functools.lru_cache(maxsize=4096)
+def _backward_plan(forward: _Plan, output_grad: Layout, query_grad: Layout, key_grad: Layout, value_grad: Layout,
+                   device: int) -> Tuple[_Shape, int]:
+    """
+    Description of the backward call of a forward one, and its workspace in bytes.
+    """
+    shape = _Shape.from_buffer_copy(forward.shape)
+    strides = list(shape.strides[:12])
+    for layout in (output_grad, query_grad, key_grad, value_grad):
+        strides += _strides(*layout[:2])
+    shape.strides = (ctypes.c_int64 * 24)(*strides)
+    return shape, _lib.load().at_attention_bwd_workspace_bytes(ctypes.byref(shape))
+
+
+def _gradient_of(tensor: Tensor) -> Tensor:
+    """
+    New tensor for a gradient: in the layout of `tensor` where that is dense.
+    """
+    grad = torch.empty_like(tensor)
+    if _readable(_layout(grad), 1):
+        return grad
+    batch, heads, tokens, dim = tensor.shape
+    return torch.empty((batch, tokens, heads, dim), device=tensor.device, dtype=tensor.dtype).transpose(1, 2)
 
 
 class WindowAttentionAutoGrad(torch.autograd.Function):
@@ -176,52 +216,45 @@ class WindowAttentionAutoGrad(torch.autograd.Function):
         Returns:
             Output of shape [batch, heads, rows, head_dim], laid out as [batch, rows, heads, head_dim].
         """
-        _check(query, key, value, lengths, query_lengths, window, num_sinks, scale)
-        _lib.require_same_device('WindowAttention', query, key, value, lengths, query_lengths)
-        lib = _lib.load()
-        batch, heads, rows, head_dim = query.shape
-        if scale is None:
-            scale = head_dim ** -0.5
-
         output_dtype = get_output_dtype(query.dtype, autocast='fp16')
-        dim = (head_dim + 7) // 8 * 8
-        query_k = _for_kernel(query.to(output_dtype), dim, heads // key.shape[1])
-        key_k = _for_kernel(key.to(output_dtype), dim, 1)
-        value_k = _for_kernel(value.to(output_dtype), dim, 1)
-        counts = (lengths, query_lengths)
-        if lengths is not None or query_lengths is not None:
-            if lengths is not None and query_lengths is not None and lengths.dtype is not query_lengths.dtype:
-                counts = (lengths.long(), query_lengths.long())
-            counts = tuple(None if c is None else c.contiguous() for c in counts)
+        device = query.get_device()
+        options = (causal, window, num_sinks)
+        counts = (None if lengths is None else _layout(lengths), None if query_lengths is None else _layout(query_lengths))
+        plan = _forward_plan(_layout(query), _layout(key), _layout(value), *counts, *options, scale, output_dtype, device)
+        _lib.require_same_device('WindowAttention', query, key, value, lengths, query_lengths)
+        head_dim = query.shape[3]
+        if not plan.direct:
+            query, key, value = (_for_kernel(t, output_dtype, g) for t, g in ((query, plan.group), (key, 1), (value, 1)))
+            lengths, query_lengths = (None if c is None else c.long().contiguous() for c in (lengths, query_lengths))
+            counts = (None if lengths is None else _layout(lengths),
+                      None if query_lengths is None else _layout(query_lengths))
+            plan = _forward_plan(_layout(query), _layout(key), _layout(value), *counts, *options, plan.scale, output_dtype,
+                                 device)
 
-        output = torch.empty((batch, rows, heads, dim), device=query.device, dtype=output_dtype).transpose(1, 2)
-        options = (bool(causal), min(window or 0, 1 << 40), min(num_sinks, 1 << 40), scale)
-        shape = _shape_of(query_k, key_k, value_k, (_strides(output),) + (_NO_STRIDES,) * 4, counts, options)
-
-        requires_grad = any(ctx.needs_input_grad[:3])
-        lse = rest = None
+        output = torch.empty(plan.output_shape, device=query.device, dtype=output_dtype)
+        lse = rest = workspace = None
+        needs_grad = ctx.needs_input_grad
+        requires_grad = needs_grad[0] or needs_grad[1] or needs_grad[2]
         if requires_grad:
+            lse = torch.empty(plan.lse_size, device=query.device, dtype=torch.float32)
             if output_dtype is not torch.float32:
-                rest = torch.empty((batch, rows, heads, dim), device=query.device, dtype=output_dtype)
-            pitch = lib.at_attention_row_pitch(rows, heads, key.shape[1])
-            lse = torch.empty(batch * key.shape[1] * pitch, device=query.device, dtype=torch.float32)
-        workspace = None
+                rest = torch.empty_like(output)
+        if plan.workspace_bytes:
+            workspace = torch.empty(plan.workspace_bytes, device=query.device, dtype=torch.uint8)
         with _lib.device_guard(query):
-            workspace_bytes = lib.at_attention_fwd_workspace_bytes(ctypes.byref(shape))
-            if workspace_bytes:
-                workspace = torch.empty(workspace_bytes, device=query.device, dtype=torch.uint8)
-            _lib.check(lib.at_attention_fwd(
-                ctypes.byref(shape), _lib.ptr(query_k), _lib.ptr(key_k), _lib.ptr(value_k), _lib.ptr(output), _lib.ptr(lse),
-                _lib.ptr(rest), _lib.ptr(workspace), workspace_bytes, _lib.stream_of(query)), 'at_attention_fwd')
+            _lib.check(_lib.load().at_attention_fwd(
+                plan.ref, query.data_ptr(), key.data_ptr(), value.data_ptr(), _lib.ptr(lengths), _lib.ptr(query_lengths),
+                output.data_ptr(), _lib.ptr(lse), _lib.ptr(rest), _lib.ptr(workspace), plan.workspace_bytes,
+                _lib.stream_of(query)), 'at_attention_fwd')
 
+        output = output.transpose(1, 2)
         if requires_grad:
-            ctx.options = options
+            ctx.plan = plan
             ctx.head_dim = head_dim
-            ctx.save_for_backward(query_k, key_k, value_k, output, rest, lse, *counts)
-        return output if dim == head_dim else output[..., :head_dim]
+            ctx.save_for_backward(query, key, value, output, rest, lse, lengths, query_lengths)
+        return output if output.shape[3] == head_dim else output[..., :head_dim]
 
     @staticmethod
-    @once_differentiable
     def backward(
         ctx: Any,
         output_grad: Tensor,
@@ -229,27 +262,37 @@ class WindowAttentionAutoGrad(torch.autograd.Function):
         """
         Gradients of the queries, keys and values.
         """
-        lib = _lib.load()
-        query, key, value, output, rest, lse, *counts = ctx.saved_tensors
-        _lib.require_same_device('WindowAttention backward', query, output_grad)
-        head_dim = ctx.head_dim
-        output_grad = _for_kernel(output_grad.to(query.dtype), query.shape[3], query.shape[1] // key.shape[1])
-        grads = [_like(tensor) for tensor in (query, key, value)]
-        shape = _shape_of(query, key, value,
-                          (_strides(output), _strides(output_grad), *(_strides(grad) for grad in grads)), counts,
-                          ctx.options)
-        workspace_bytes = lib.at_attention_bwd_workspace_bytes(ctypes.byref(shape))
-        workspace = torch.empty(workspace_bytes, device=query.device, dtype=torch.uint8)
-        with _lib.device_guard(query):
-            _lib.check(lib.at_attention_bwd(
-                ctypes.byref(shape), _lib.ptr(output_grad), _lib.ptr(query), _lib.ptr(key), _lib.ptr(value), _lib.ptr(output),
-                _lib.ptr(rest), _lib.ptr(lse), *(_lib.ptr(grad) for grad in grads), _lib.ptr(workspace), workspace_bytes,
-                _lib.stream_of(query)), 'at_attention_bwd')
-        if head_dim != query.shape[3]:
-            grads = [grad[..., :head_dim] for grad in grads]
+        # under create_graph the gradients are marked as not differentiable again
+        return _backward_once(ctx, output_grad) if torch.is_grad_enabled() else _backward(ctx, output_grad)
 
-        # One gradient (or None) per forward argument.
-        return (*grads, None, None, None, None, None, None)
+
+def _backward(ctx: Any, output_grad: Tensor) -> Tuple[Optional[Tensor], ...]:
+    query, key, value, output, rest, lse, lengths, query_lengths = ctx.saved_tensors
+    _lib.require_same_device('WindowAttention backward', query, output_grad)
+    plan = ctx.plan
+    layout = _layout(output_grad)
+    if layout[2] is not query.dtype or not _readable(layout, plan.group):
+        output_grad = _for_kernel(output_grad, query.dtype, plan.group)
+        layout = _layout(output_grad)
+    query_grad, key_grad, value_grad = _gradient_of(query), _gradient_of(key), _gradient_of(value)
+    shape, workspace_bytes = _backward_plan(plan, layout, _layout(query_grad), _layout(key_grad), _layout(value_grad),
+                                            query.get_device())
+    workspace = torch.empty(workspace_bytes, device=query.device, dtype=torch.uint8)
+    with _lib.device_guard(query):
+        _lib.check(_lib.load().at_attention_bwd(
+            ctypes.byref(shape), output_grad.data_ptr(), query.data_ptr(), key.data_ptr(), value.data_ptr(),
+            _lib.ptr(lengths), _lib.ptr(query_lengths), output.data_ptr(), _lib.ptr(rest), lse.data_ptr(),
+            query_grad.data_ptr(), key_grad.data_ptr(), value_grad.data_ptr(), workspace.data_ptr(), workspace_bytes,
+            _lib.stream_of(query)), 'at_attention_bwd')
+    head_dim = ctx.head_dim
+    if head_dim != query.shape[3]:
+        query_grad, key_grad, value_grad = (grad[..., :head_dim] for grad in (query_grad, key_grad, value_grad))
+
+    # One gradient (or None) per forward argument.
+    return query_grad, key_grad, value_grad, None, None, None, None, None, None
+
+
+_backward_once = once_differentiable(_backward)
 
 
 class WindowAttention(nn.Module):

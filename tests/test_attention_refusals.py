@@ -103,7 +103,7 @@ def attention_shape(**changes):
 def test_attention_codes() -> None:
     lib = _lib.load()
     p = (ctypes.addressof(ctypes.create_string_buffer(4096)) + 63) // 64 * 64
-    fwd = lambda s, *a: lib.at_attention_fwd(ctypes.byref(s), *(a or (p, p, p, p, None, None, None, 0)), None)  # noqa: E731
+    fwd = lambda s, *a: lib.at_attention_fwd(ctypes.byref(s), *(a or (p, p, p, None, None, p, None, None, None, 0)), None)  # noqa: E731
     for changes, code in (({'batch': -1}, -2), ({'heads': 3}, -2), ({'kv_heads': 0}, -2), ({'rows': 9}, -2),
                           ({'keys': (1 << 29) + 1}, -2), ({'dim': 136}, -2), ({'dim': 0}, -2), ({'dim': 12}, -6),
                           ({'window': -1}, -2), ({'sinks': -1}, -2), ({'scale': 0.0}, -2), ({'scale': float('nan')}, -2),
@@ -111,20 +111,20 @@ def test_attention_codes() -> None:
                           ({'strides': [512, -128, 16] * 8}, -2), ({'strides': [1 << 40, 1 << 40, 1 << 40] * 8}, -2),
                           ({'batch': 65536}, -2), ({'rows': 1 << 29, 'keys': 1 << 29}, -2)):
         assert fwd(attention_shape(**changes)) == code, changes
-        assert lib.at_attention_bwd(ctypes.byref(attention_shape(**changes)), *[p] * 11, 1 << 20, None) == code, changes
+        assert lib.at_attention_bwd(ctypes.byref(attention_shape(**changes)), *[p] * 13, 1 << 20, None) == code, changes
         assert lib.at_attention_fwd_workspace_bytes(ctypes.byref(attention_shape(**changes))) == 0
         assert lib.at_attention_bwd_workspace_bytes(ctypes.byref(attention_shape(**changes))) == 0
-    assert lib.at_attention_fwd(None, p, p, p, p, None, None, None, 0, None) == -1
-    assert fwd(attention_shape(), None, p, p, p, None, None, None, 0) == -1
-    assert fwd(attention_shape(), p, p, p, p + 4, None, None, None, 0) == -6
-    assert fwd(attention_shape(batch=0), None, None, None, None, None, None, None, 0) == 0
+    assert lib.at_attention_fwd(None, p, p, p, None, None, p, None, None, None, 0, None) == -1
+    assert fwd(attention_shape(), None, p, p, None, None, p, None, None, None, 0) == -1
+    assert fwd(attention_shape(), p, p, p, None, None, p + 4, None, None, None, 0) == -6
+    assert fwd(attention_shape(batch=0), *[None] * 9, 0) == 0
     # few rows and many keys: pieces in a workspace
     cache = attention_shape(rows=1, keys=100000)
     assert lib.at_attention_fwd_workspace_bytes(ctypes.byref(cache)) > 0
     assert fwd(cache) == -5
     bwd = lambda *a: lib.at_attention_bwd(ctypes.byref(attention_shape()), *a, None)  # noqa: E731
-    assert bwd(*[p] * 10, None, 0) == -5 and bwd(*[p] * 11, 64) == -5
-    assert bwd(None, *[p] * 10, 1 << 20) == -1 and bwd(p, p, p, p + 8, *[p] * 7, 1 << 20) == -6
+    assert bwd(*[p] * 12, None, 0) == -5 and bwd(*[p] * 13, 64) == -5
+    assert bwd(None, *[p] * 12, 1 << 20) == -1 and bwd(p, p, p, p + 8, *[p] * 9, 1 << 20) == -6
     assert lib.at_attention_row_pitch(5, 4, 2) == 64 and lib.at_attention_row_pitch(33, 4, 2) == 128
     assert lib.at_attention_row_pitch(33, 4, 3) == 0
 
