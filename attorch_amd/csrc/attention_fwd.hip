@@ -13,6 +13,7 @@ namespace {
 constexpr int kKeys = 64;        // keys of a tile
 constexpr int kWaves = 4;
 constexpr int kRows = 32 * kWaves;
+constexpr int kMaxSplits = 128;
 
 // Four elements of the output, and what their rounding left over where a backward pass will need it.
 template <typename T>
@@ -211,44 +212,75 @@ __global__ __launch_bounds__(kWaves * 64, sizeof(T) == 2 ? 2 : 1) void attention
     }
 }
 
-// Joins the splits of a row: out = sum_s 2^(lse_s - lse) out_s, lse = log2 sum_s 2^lse_s.  32 lanes per
-// row, four elements of dim per lane.
-template <typename T>
+// Joins the splits of a row: out = sum_s 2^(lse_s - lse) out_s, lse = log2 sum_s 2^lse_s.  32 lanes cover
+// dim with four elements each.  A workgroup of 8 such groups takes GROUPS of them for a row: one where the
+// splits are few (then bound by reading them: 33 MB in 10 us), all 8 where they are many, each on every
+// eighth split (one group over 64 splits: 51 us for one token of 131072, eight: 4).
+constexpr int kFewSplits = 8;
+template <typename T, int GROUPS>
 __global__ __launch_bounds__(256) void attention_join_kernel(AttentionArgs a) {
+  __shared__ float4 sums[8][32];
   const int all_rows = a.rows * a.group;
-  const int64_t at = (int64_t)blockIdx.x * 8 + (threadIdx.x >> 5);
   const int64_t bhs = (int64_t)a.batch * a.kv_heads;
-  if (at >= bhs * a.row_pitch) return;
-  const int bh = (int)(at / a.row_pitch), row = (int)(at - (int64_t)bh * a.row_pitch);
+  const int64_t at = (int64_t)blockIdx.x * (8 / GROUPS) + (GROUPS == 1 ? threadIdx.x >> 5 : 0);
+  if (at >= bhs * all_rows) return;
+  const int bh = (int)(at / all_rows), row = (int)(at - (int64_t)bh * all_rows);
   const int b = bh / a.kv_heads, h = bh - b * a.kv_heads;
   const int i = row / a.group, g = row - i * a.group;
-  const int d = (threadIdx.x & 31) * 4;
+  const int first = GROUPS == 1 ? 0 : threadIdx.x >> 5, d = (threadIdx.x & 31) * 4;
   const bool valid = i < sequence_of(a, b).live;
+
   const float* lses = a.part_lse + (int64_t)bh * a.row_pitch + row;
-  float top = -INFINITY, sum = 0.f, v[4] = {0.f, 0.f, 0.f, 0.f};
-  if (valid) {
-    for (int s = 0; s < a.splits; ++s) top = fmaxf(top, lses[s * bhs * a.row_pitch]);
-    if (top == -INFINITY) top = 0.f;
-    for (int s = 0; s < a.splits; ++s) {
-      const float w = __builtin_amdgcn_exp2f(lses[s * bhs * a.row_pitch] - top);
-      sum += w;
-      if (d < a.dim && w != 0.f) {
-        const float4 x = *reinterpret_cast<const float4*>(a.part + ((s * bhs + bh) * all_rows + row) * a.dim + d);
-        v[0] += w * x.x; v[1] += w * x.y; v[2] += w * x.z; v[3] += w * x.w;
-      }
+  const int64_t next = bhs * a.row_pitch;
+  float top = -INFINITY, total = 0.f, v[4] = {0.f, 0.f, 0.f, 0.f};
+  __shared__ float shared_lse[GROUPS == 1 ? 1 : kMaxSplits];
+  if constexpr (GROUPS == 1) {
+#pragma unroll 8
+    for (int s = 0; s < a.splits; ++s) top = fmaxf(top, lses[s * next]);
+  } else {                             // one round of loads for all splits
+    for (int s = threadIdx.x; s < a.splits; s += 256) shared_lse[s] = lses[s * next];
+    __syncthreads();
+    for (int s = threadIdx.x & 63; s < a.splits; s += 64) top = fmaxf(top, shared_lse[s]);
+    top = wave_reduce(top, kWave, MaxOp());
+  }
+  if (top == -INFINITY) top = 0.f;
+#pragma unroll 4
+  for (int s = first; s < a.splits; s += GROUPS) {
+    const float w = __builtin_amdgcn_exp2f((GROUPS == 1 ? lses[s * next] : shared_lse[s]) - top);
+    total += w;
+    if (d < a.dim) {
+      const float4 x = *reinterpret_cast<const float4*>(a.part + ((s * bhs + bh) * all_rows + row) * a.dim + d);
+      v[0] += w * x.x; v[1] += w * x.y; v[2] += w * x.z; v[3] += w * x.w;
     }
-    const float inv = sum == 0.f ? 0.f : 1.f / sum;
+  }
+  if constexpr (GROUPS > 1) {
+    __shared__ float totals[8];
+    sums[first][threadIdx.x & 31] = make_float4(v[0], v[1], v[2], v[3]);
+    if ((threadIdx.x & 31) == 0) totals[first] = total;
+    __syncthreads();
+    if (first != 0) return;
 #pragma unroll
-    for (int j = 0; j < 4; ++j) v[j] *= inv;
+    for (int n = 1; n < GROUPS; ++n) {
+      const float4 x = sums[n][threadIdx.x];
+      v[0] += x.x; v[1] += x.y; v[2] += x.z; v[3] += x.w;
+      total += totals[n];
+    }
   }
-  if (row < all_rows && d < a.dim) {
+  const float inv = total == 0.f ? 0.f : 1.f / total;
+#pragma unroll
+  for (int j = 0; j < 4; ++j) v[j] = valid ? v[j] * inv : 0.f;
+  if (d < a.dim)
     store_output<T>(a, b * a.out.batch + (int64_t)(h * a.group + g) * a.out.head + i * a.out.token + d * (int)sizeof(T), v);
-  }
-  if (a.lse && d == 0) a.lse[at] = valid ? top + __builtin_amdgcn_logf(sum) : INFINITY;
+  if (!a.lse) return;
+  float* lse = a.lse + (int64_t)bh * a.row_pitch;
+  if (d == 0) lse[row] = valid ? top + __builtin_amdgcn_logf(total) : INFINITY;
+  if (row == all_rows - 1)             // and the padding behind the last row
+    for (int r = all_rows + (threadIdx.x & 31); r < a.row_pitch; r += 32) lse[r] = INFINITY;
 }
 
-// Splits of the keys per tile of rows: none while the tiles alone give every CU two workgroups,
-// otherwise as many as fill two per CU with at least two tiles of keys each.
+// Splits of the keys per tile of rows: none while the tiles alone give every CU two workgroups, otherwise
+// as many as fill two per CU with at least four tiles of keys each (the join is a launch of 4 us; a tile
+// takes a workgroup about 1).
 int split_count(const AttentionArgs& a) {
   const int64_t groups = (int64_t)a.tiles * a.batch * a.kv_heads;
   const int64_t want = 2 * device_cu_count();
@@ -257,14 +289,14 @@ int split_count(const AttentionArgs& a) {
   const int64_t span = (int64_t)a.left + a.right + cdiv64(kRows, a.group) + a.sinks;
   const int64_t tiles = cdiv64(span < a.keys ? span : a.keys, kKeys);
   int64_t n = cdiv64(want, groups);
-  if (n > tiles / 2) n = tiles / 2;
-  return (int)(n < 1 ? 1 : n > 128 ? 128 : n);
+  if (n > tiles / 4) n = tiles / 4;
+  return (int)(n < 1 ? 1 : n > kMaxSplits ? kMaxSplits : n);
 }
 
 template <typename T>
 int launch_dim(const AttentionArgs& a, hipStream_t stream) {
   const int64_t blocks = (int64_t)a.tiles * a.batch * a.kv_heads;
-  if (!grid_fits(blocks) || !grid_fits(cdiv64((int64_t)a.batch * a.kv_heads * a.row_pitch, 8))) return AT_ERR_DIM;
+  if (!grid_fits(blocks) || (a.splits > 1 && !grid_fits((int64_t)a.batch * a.kv_heads * a.rows * a.group))) return AT_ERR_DIM;
   const dim3 grid((unsigned)blocks, (unsigned)a.splits), block(kWaves * 64);
   switch ((a.dim + 31) / 32) {
     case 1: hipLaunchKernelGGL((attention_fwd_kernel<T, 1>), grid, block, 0, stream, a); break;
@@ -274,8 +306,11 @@ int launch_dim(const AttentionArgs& a, hipStream_t stream) {
   }
   int rc = launch_status();
   if (rc == AT_OK && a.splits > 1) {
-    const int64_t rows = (int64_t)a.batch * a.kv_heads * a.row_pitch;
-    hipLaunchKernelGGL((attention_join_kernel<T>), dim3((unsigned)cdiv64(rows, 8)), dim3(256), 0, stream, a);
+    const int64_t rows = (int64_t)a.batch * a.kv_heads * a.rows * a.group;
+    if (a.splits <= kFewSplits)
+      hipLaunchKernelGGL((attention_join_kernel<T, 1>), dim3((unsigned)cdiv64(rows, 8)), dim3(256), 0, stream, a);
+    else
+      hipLaunchKernelGGL((attention_join_kernel<T, 8>), dim3((unsigned)rows), dim3(256), 0, stream, a);
     rc = launch_status();
   }
   return rc;
