@@ -170,6 +170,10 @@ __device__ __forceinline__ void dma_16(const i32x4& rsrc, int lane_bytes, int un
 }
 
 // ---- tiles in LDS -------------------------------------------------------------------------
+typedef __attribute__((address_space(3))) char lds_char;
+typedef __attribute__((address_space(3))) float lds_float;
+typedef __attribute__((address_space(3))) i32x4 lds_i32x4;
+
 // [ROWS][dim] tile, dim padded with zeros to DT * 32 elements, rows of 64 (DT <= 2) or 128 elements.
 // The 16-byte chunks of a row are permuted by an XOR with spread(row) so that both kinds of
 // fragment reads touch all banks: 8 consecutive rows at one chunk (row order) as well as 4
@@ -182,17 +186,34 @@ template <typename T, int DT> struct Tile {
   static __device__ __forceinline__ int spread(int row) {
     return ((row & 3) << 1) | ((row >> 2) & 1) | (kChunks >= 16 ? (row & 8) : 0);
   }
-  static __device__ __forceinline__ int at(int row, int chunk) { return row * kPitch + ((chunk ^ spread(row)) << 4); }
-
-  // Rows `row_base` + lane % 32, elements 16 step .. 16 step + 15, row order.
-  static __device__ __forceinline__ typename Frag<T>::type rows_frag(const char* tile, int row_base, int step) {
-    const int lane = threadIdx.x & 63, row = lane & 31, half = lane >> 5;
-    const char* base = tile + row_base * kPitch;
+  // Where a lane reads: byte addresses in LDS of its first fragments of a tile.  Tiles start at multiples of
+  // kPitch, so a step along dim is an XOR with a constant, and rows further down are immediate offsets:
+  // two registers serve all reads of a stage.
+  struct Reader {
+    int rows, cols;
+  };
+  static __device__ __forceinline__ Reader reader(const char* stage) {
+    const int lane = threadIdx.x & 63, half = lane >> 5, low = lane & 31;
+    const int base = (int)(uintptr_t)(lds_char*)stage;
+    Reader r;
+    r.rows = base + low * kPitch + (((sizeof(T) == 2 ? half : half * 2) ^ spread(low)) << 4);
     if constexpr (sizeof(T) == 2) {
-      return *reinterpret_cast<const uint4*>(base + at(row, step * 2 + half));
+      const int i = lane & 15, row = half * 4 + (i >> 2);
+      r.cols = base + row * kPitch + (((((lane >> 4) & 1) * 2 + ((i & 3) >> 1)) ^ spread(row)) << 4) + (i & 1) * 8;
     } else {
-      const float4 a = *reinterpret_cast<const float4*>(base + at(row, step * 4 + half * 2));
-      const float4 b = *reinterpret_cast<const float4*>(base + at(row, step * 4 + half * 2 + 1));
+      r.cols = base + half * 4 * kPitch + (((low >> 2) ^ spread(half * 4)) << 4) + (low & 3) * 4;
+    }
+    return r;
+  }
+
+  // Rows `row_base` + lane % 32 of the tile `tile` bytes into the stage, elements 16 step .. 16 step + 15, row order.
+  static __device__ __forceinline__ typename Frag<T>::type rows_frag(const Reader& r, int tile, int row_base, int step) {
+    const int off = tile + row_base * kPitch;
+    if constexpr (sizeof(T) == 2) {
+      return __builtin_bit_cast(uint4, *(const lds_i32x4*)((lds_char*)(r.rows ^ (step << 5)) + off));
+    } else {
+      const float4 a = __builtin_bit_cast(float4, *(const lds_i32x4*)((lds_char*)(r.rows ^ (step << 6)) + off));
+      const float4 b = __builtin_bit_cast(float4, *(const lds_i32x4*)((lds_char*)(r.rows ^ (step << 6) ^ 16) + off));
       return Frag32{{a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w}};
     }
   }
@@ -200,26 +221,21 @@ template <typename T, int DT> struct Tile {
   // Elements (columns) 32 dt + lane % 32 as rows, tile rows `row_base` .. + 15 as contraction in
   // accumulator order.  16-bit elements are transposed by the reads themselves
   // (ds_read_b64_tr_b16: within 16 lanes, result[l][e] = source[4 e + l / 4][l % 4]).
-  static __device__ __forceinline__ typename Frag<T>::type cols_frag(const char* tile, int row_base, int dt) {
-    const int lane = threadIdx.x & 63, half = lane >> 5;
-    const char* base = tile + row_base * kPitch;
+  static __device__ __forceinline__ typename Frag<T>::type cols_frag(const Reader& r, int tile, int row_base, int dt) {
+    const int off = tile + row_base * kPitch;
     if constexpr (sizeof(T) == 2) {
-      const int i = lane & 15;
-      const int chunk = dt * 4 + ((lane >> 4) & 1) * 2 + ((i & 3) >> 1);
-      const int row = half * 4 + (i >> 2);
-      const char* p0 = base + at(row, chunk) + (i & 1) * 8;
-      const char* p1 = base + at(row + 8, chunk) + (i & 1) * 8;
+      const int at = r.cols ^ (dt << 6);
       typedef __attribute__((address_space(3))) s16x4 lds_s16x4;
-      const uint2 a = __builtin_bit_cast(uint2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)p0));
-      const uint2 b = __builtin_bit_cast(uint2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)p1));
+      const uint2 a = __builtin_bit_cast(uint2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)((lds_char*)at + off)));
+      const uint2 b = __builtin_bit_cast(uint2, __builtin_amdgcn_ds_read_tr16_b64_v4i16(
+          (lds_s16x4*)((lds_char*)(at ^ (spread(8) << 4)) + off + 8 * kPitch)));
       return make_uint4(a.x, a.y, b.x, b.y);
     } else {
-      const int col = dt * 32 + (lane & 31);
       Frag32 f;
 #pragma unroll
       for (int j = 0; j < 8; ++j) {
-        const int row = (j < 4 ? 0 : 8) + half * 4 + (j & 3);
-        f.e[j] = *reinterpret_cast<const float*>(base + at(row, col >> 2) + (col & 3) * 4);
+        const int row = (j < 4 ? 0 : 8) + (j & 3);
+        f.e[j] = *(const lds_float*)((lds_char*)(r.cols ^ (dt << 7) ^ (spread(row) << 4)) + off + row * kPitch);
       }
       return f;
     }

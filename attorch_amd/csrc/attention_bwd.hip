@@ -128,13 +128,14 @@ __global__ __launch_bounds__(kWaves * 64, sizeof(T) == 2 ? 2 : 1) void attention
     if (!((k0 < mine.hi && k0 + kStep > mine.lo) || k0 < mine.sinks) || last < first) continue;
     const bool whole = k0 >= last - a.left && k0 + kStep - 1 <= min(first + a.right, seq.len - 1);
 
+    const typename L::Reader lr = L::reader(stage);
 #pragma unroll
     for (int n = 0; n < kStep / 32; ++n) {
       f32x16 s = zero_acc(), dp = zero_acc();
 #pragma unroll
       for (int ks = 0; ks < L::kSteps; ++ks) {
-        s = Frag<T>::mma(L::rows_frag(stage, n * 32, ks), qf[ks], s);
-        dp = Frag<T>::mma(L::rows_frag(stage + kTileBytes, n * 32, ks), df[ks], dp);
+        s = Frag<T>::mma(L::rows_frag(lr, 0, n * 32, ks), qf[ks], s);
+        dp = Frag<T>::mma(L::rows_frag(lr, kTileBytes, n * 32, ks), df[ks], dp);
       }
 #pragma unroll
       for (int e = 0; e < 16; ++e) {
@@ -151,7 +152,7 @@ __global__ __launch_bounds__(kWaves * 64, sizeof(T) == 2 ? 2 : 1) void attention
         const F ds = Frag<T>::pack(x);
 #pragma unroll
         for (int dt = 0; dt < DT; ++dt)
-          dq[dt] = Frag<T>::mma(L::cols_frag(stage, n * 32 + t16 * 16, dt), ds, dq[dt]);
+          dq[dt] = Frag<T>::mma(L::cols_frag(lr, 0, n * 32 + t16 * 16, dt), ds, dq[dt]);
       }
     }
   }
@@ -314,6 +315,7 @@ __global__ __launch_bounds__(kWaves * 64, KT == 1 && sizeof(T) == 2 ? 2 : 1) voi
     lds_dma_wait_all();
     __syncthreads();
     if (t + 1 < end) fetch(t + 1, lds + ((t + 1 - begin) & 1) * kStage);
+    const typename L::Reader lr = L::reader(stage);
     const float* stats = reinterpret_cast<const float*>(stage + 2 * kTileBytes);
 #pragma unroll
     for (int n = 0; n < kStep / 32; ++n) {
@@ -325,13 +327,13 @@ __global__ __launch_bounds__(kWaves * 64, KT == 1 && sizeof(T) == 2 ? 2 : 1) voi
       for (int kt = 0; kt < KT; ++kt) s[kt] = dp[kt] = zero_acc();
 #pragma unroll
       for (int ks = 0; ks < L::kSteps; ++ks) {
-        const F qf = L::rows_frag(stage, n * 32, ks);
+        const F qf = L::rows_frag(lr, 0, n * 32, ks);
 #pragma unroll
         for (int kt = 0; kt < KT; ++kt) s[kt] = Frag<T>::mma(qf, kf[kt][ks], s[kt]);
       }
 #pragma unroll
       for (int ks = 0; ks < L::kSteps; ++ks) {
-        const F df = L::rows_frag(stage + kTileBytes, n * 32, ks);
+        const F df = L::rows_frag(lr, kTileBytes, n * 32, ks);
 #pragma unroll
         for (int kt = 0; kt < KT; ++kt) dp[kt] = Frag<T>::mma(df, vf[kt][ks], dp[kt]);
       }
@@ -374,8 +376,8 @@ __global__ __launch_bounds__(kWaves * 64, KT == 1 && sizeof(T) == 2 ? 2 : 1) voi
         }
 #pragma unroll
         for (int dt = 0; dt < DT; ++dt) {
-          const F dc = L::cols_frag(stage + kTileBytes, n * 32 + t16 * 16, dt);
-          const F qc = L::cols_frag(stage, n * 32 + t16 * 16, dt);
+          const F dc = L::cols_frag(lr, kTileBytes, n * 32 + t16 * 16, dt);
+          const F qc = L::cols_frag(lr, 0, n * 32 + t16 * 16, dt);
 #pragma unroll
           for (int kt = 0; kt < KT; ++kt) {
             dv[kt][dt] = Frag<T>::mma(dc, pf[kt], dv[kt][dt]);

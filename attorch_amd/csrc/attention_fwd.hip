@@ -117,12 +117,13 @@ __global__ __launch_bounds__(kWaves * 64, sizeof(T) == 2 ? 2 : 1) void attention
     // does any row of the wave see any key of the tile?
     if (!((k0 < mine.hi && k0 + kKeys > mine.lo) || k0 < mine.sinks) || last < first) continue;
 
+    const typename L::Reader lr = L::reader(stage);
     f32x16 s[2];
 #pragma unroll
     for (int n = 0; n < 2; ++n) {
       s[n] = zero_acc();
 #pragma unroll
-      for (int ks = 0; ks < L::kSteps; ++ks) s[n] = Frag<T>::mma(L::rows_frag(stage, n * 32, ks), qf[ks], s[n]);
+      for (int ks = 0; ks < L::kSteps; ++ks) s[n] = Frag<T>::mma(L::rows_frag(lr, 0, n * 32, ks), qf[ks], s[n]);
     }
     // keys of the lane relative to its first one, as constants: 8 apart, 4 in a row
     const bool whole = k0 >= last - a.left && k0 + kKeys - 1 <= min(first + a.right, seq.len - 1);
@@ -171,7 +172,7 @@ __global__ __launch_bounds__(kWaves * 64, sizeof(T) == 2 ? 2 : 1) void attention
       const F pf = Frag<T>::pack(pr);
 #pragma unroll
       for (int dt = 0; dt < DT; ++dt)
-        o[dt] = Frag<T>::mma(L::cols_frag(stage + kTileBytes, ks * 16, dt), pf, o[dt]);
+        o[dt] = Frag<T>::mma(L::cols_frag(lr, kTileBytes, ks * 16, dt), pf, o[dt]);
     }
   }
 
