@@ -138,11 +138,17 @@ __global__ __launch_bounds__(kWaves * 64, sizeof(T) == 2 ? 2 : 1) void attention
         dp = Frag<T>::mma(L::rows_frag(lr, kTileBytes, n * 32, ks), df[ks], dp);
       }
 #pragma unroll
-      for (int e = 0; e < 16; ++e) {
-        const int key = k0 + n * 32 + acc_row(e, half);
-        const bool seen = whole || (key >= see_lo && key <= see_hi) || key < see_sinks;
-        const float pr = __builtin_amdgcn_exp2f(fmaf(s[e], a.scale_log2, -lse));
-        s[e] = seen ? pr * (dp[e] - delta) : 0.f;
+      for (int e = 0; e < 16; ++e)
+        s[e] = __builtin_amdgcn_exp2f(fmaf(s[e], a.scale_log2, -lse)) * (dp[e] - delta);
+      if (!whole) {
+        int key = k0 + n * 32 + half * 4;
+        asm volatile("" : "+v"(key));    // a branch: as selects the masks would be formed for every tile
+        const int lo = see_lo - key, hi = see_hi - key, sinks = see_sinks - key;
+#pragma unroll
+        for (int e = 0; e < 16; ++e) {
+          const int c = acc_row(e, 0);
+          s[e] = (c >= lo && c <= hi) || c < sinks ? s[e] : 0.f;
+        }
       }
 #pragma unroll
       for (int t16 = 0; t16 < 2; ++t16) {
@@ -347,17 +353,23 @@ __global__ __launch_bounds__(kWaves * 64, KT == 1 && sizeof(T) == 2 ? 2 : 1) voi
 #pragma unroll
           for (int j = 0; j < 4; ++j) {
             const int e = q * 4 + j;
-            float pr = __builtin_amdgcn_exp2f(fmaf(s[kt][e], a.scale_log2, ProbShift<T>::backward - ls[j]));
-            float ds = pr * (dp[kt][e] - de[j]);
-            if (!whole) {
-              const int r = r0 + q * 8 + half * 4 + j;
-              const bool seen = r >= row_lo[kt] && r <= row_hi[kt];
-              pr = seen ? pr : 0.f;
-              ds = seen ? ds : 0.f;
-            }
-            s[kt][e] = pr;
-            dp[kt][e] = ds;
+            s[kt][e] = __builtin_amdgcn_exp2f(fmaf(s[kt][e], a.scale_log2, ProbShift<T>::backward - ls[j]));
+            dp[kt][e] = s[kt][e] * (dp[kt][e] - de[j]);
           }
+      }
+      if (!whole) {
+        int row = r0 + half * 4;
+        asm volatile("" : "+v"(row));    // a branch: as selects the masks would be formed for every tile
+#pragma unroll
+        for (int kt = 0; kt < KT; ++kt) {
+          const int lo = row_lo[kt] - row, hi = row_hi[kt] - row;
+#pragma unroll
+          for (int e = 0; e < 16; ++e) {
+            const bool seen = acc_row(e, 0) >= lo && acc_row(e, 0) <= hi;
+            s[kt][e] = seen ? s[kt][e] : 0.f;
+            dp[kt][e] = seen ? dp[kt][e] : 0.f;
+          }
+        }
       }
 #pragma unroll
       for (int t16 = 0; t16 < 2; ++t16) {

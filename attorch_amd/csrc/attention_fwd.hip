@@ -128,7 +128,8 @@ __global__ __launch_bounds__(kWaves * 64, sizeof(T) == 2 ? 2 : 1) void attention
     // keys of the lane relative to its first one, as constants: 8 apart, 4 in a row
     const bool whole = k0 >= last - a.left && k0 + kKeys - 1 <= min(first + a.right, seq.len - 1);
     if (!whole) {
-      const int key = k0 + half * 4;
+      int key = k0 + half * 4;
+      asm volatile("" : "+v"(key));    // a branch: as selects the masks would be formed for every tile
       const int lo = see_lo - key, hi = see_hi - key, sinks = see_sinks - key;
 #pragma unroll
       for (int n = 0; n < 2; ++n)
