@@ -111,7 +111,8 @@ class _Plan:
     """
     What a forward call of given layouts and options passes on: nothing in it belongs to a tensor.
     """
-    __slots__ = ('direct', 'shape', 'ref', 'group', 'output_shape', 'lse_size', 'workspace_bytes', 'scale')
+    __slots__ = ('direct', 'shape', 'ref', 'group', 'scale', 'output_shape', 'rest_bytes', 'kept_bytes',
+                 'workspace_bytes', 'like_inputs', 'grad_strides')
 
 
 @functools.lru_cache(maxsize=4096)
@@ -141,32 +142,40 @@ def _forward_plan(query: Layout, key: Layout, value: Layout, lengths: Optional[L
                         int(bool(counts) and counts[0][2] is torch.int64))
     plan.ref = ctypes.byref(plan.shape)
     lib = _lib.load()
-    plan.lse_size = batch * kv_heads * lib.at_attention_row_pitch(rows, heads, kv_heads)
     plan.workspace_bytes = lib.at_attention_fwd_workspace_bytes(plan.ref)
+    # what the backward pass needs, in one tensor: what the output's rounding leaves over, and the rows' sums
+    plan.rest_bytes = 0 if dtype is torch.float32 else (batch * rows * heads * dim * dtype.itemsize + 255) // 256 * 256
+    plan.kept_bytes = plan.rest_bytes + 4 * batch * kv_heads * lib.at_attention_row_pitch(rows, heads, kv_heads)
+    # gradients take the inputs' layouts where these are dense and [batch, tokens, heads, dim] otherwise
+    plan.like_inputs, plan.grad_strides = [], []
+    for shape, stride, _, _ in (query, key, value):
+        grad = torch.empty_like(torch.empty_strided(shape, stride, dtype=dtype, device='meta'))
+        like = _readable((shape, grad.stride(), dtype, True), 1)
+        plan.like_inputs.append(like)
+        plan.grad_strides += _strides(shape, grad.stride() if like else
+                                      (shape[2] * shape[1] * dim, dim, shape[1] * dim, 1))
     return plan
 
 
 @functools.lru_cache(maxsize=4096)
-def _backward_plan(forward: _Plan, output_grad: Layout, query_grad: Layout, key_grad: Layout, value_grad: Layout,
-                   device: int) -> Tuple[_Shape, int]:
+def _backward_plan(forward: _Plan, output_grad: Layout, dtype: torch.dtype, device: int) -> Optional[Tuple[_Shape, int]]:
     """
-    Description of the backward call of a forward one, and its workspace in bytes.
+    Description of the backward call of a forward one, and its workspace in bytes; None where the
+    kernels cannot read the output's gradient.
     """
+    if output_grad[2] is not dtype or not _readable(output_grad, forward.group):
+        return None
     shape = _Shape.from_buffer_copy(forward.shape)
-    strides = list(shape.strides[:12])
-    for layout in (output_grad, query_grad, key_grad, value_grad):
-        strides += _strides(*layout[:2])
-    shape.strides = (ctypes.c_int64 * 24)(*strides)
+    shape.strides = (ctypes.c_int64 * 24)(*shape.strides[:12], *_strides(*output_grad[:2]), *forward.grad_strides)
     return shape, _lib.load().at_attention_bwd_workspace_bytes(ctypes.byref(shape))
 
 
-def _gradient_of(tensor: Tensor) -> Tensor:
+def _gradient_of(tensor: Tensor, like: bool) -> Tensor:
     """
-    New tensor for a gradient: in the layout of `tensor` where that is dense.
+    New tensor for a gradient: in the layout of `tensor`, or as [batch, tokens, heads, dim].
     """
-    grad = torch.empty_like(tensor)
-    if _readable(_layout(grad), 1):
-        return grad
+    if like:
+        return torch.empty_like(tensor)
     batch, heads, tokens, dim = tensor.shape
     return torch.empty((batch, tokens, heads, dim), device=tensor.device, dtype=tensor.dtype).transpose(1, 2)
 
@@ -232,26 +241,27 @@ class WindowAttentionAutoGrad(torch.autograd.Function):
                                  device)
 
         output = torch.empty(plan.output_shape, device=query.device, dtype=output_dtype)
-        lse = rest = workspace = None
+        kept = rest = lse = workspace = None
         needs_grad = ctx.needs_input_grad
-        requires_grad = needs_grad[0] or needs_grad[1] or needs_grad[2]
-        if requires_grad:
-            lse = torch.empty(plan.lse_size, device=query.device, dtype=torch.float32)
-            if output_dtype is not torch.float32:
-                rest = torch.empty_like(output)
+        if needs_grad[0] or needs_grad[1] or needs_grad[2]:
+            kept = torch.empty(plan.kept_bytes, device=query.device, dtype=torch.uint8)
+            rest = kept.data_ptr()
+            lse = rest + plan.rest_bytes
         if plan.workspace_bytes:
             workspace = torch.empty(plan.workspace_bytes, device=query.device, dtype=torch.uint8)
         with _lib.device_guard(query):
             _lib.check(_lib.load().at_attention_fwd(
-                plan.ref, query.data_ptr(), key.data_ptr(), value.data_ptr(), _lib.ptr(lengths), _lib.ptr(query_lengths),
-                output.data_ptr(), _lib.ptr(lse), _lib.ptr(rest), _lib.ptr(workspace), plan.workspace_bytes,
-                _lib.stream_of(query)), 'at_attention_fwd')
+                plan.ref, query.data_ptr(), key.data_ptr(), value.data_ptr(),
+                None if lengths is None else lengths.data_ptr(),
+                None if query_lengths is None else query_lengths.data_ptr(), output.data_ptr(), lse, rest,
+                None if workspace is None else workspace.data_ptr(), plan.workspace_bytes, _lib.stream_of(query)),
+                'at_attention_fwd')
 
         output = output.transpose(1, 2)
-        if requires_grad:
+        if kept is not None:
             ctx.plan = plan
             ctx.head_dim = head_dim
-            ctx.save_for_backward(query, key, value, output, rest, lse, lengths, query_lengths)
+            ctx.save_for_backward(query, key, value, output, kept, lengths, query_lengths)
         return output if output.shape[3] == head_dim else output[..., :head_dim]
 
     @staticmethod
@@ -267,23 +277,28 @@ class WindowAttentionAutoGrad(torch.autograd.Function):
 
 
 def _backward(ctx: Any, output_grad: Tensor) -> Tuple[Optional[Tensor], ...]:
-    query, key, value, output, rest, lse, lengths, query_lengths = ctx.saved_tensors
-    _lib.require_same_device('WindowAttention backward', query, output_grad)
-    plan = ctx.plan
-    layout = _layout(output_grad)
-    if layout[2] is not query.dtype or not _readable(layout, plan.group):
-        output_grad = _for_kernel(output_grad, query.dtype, plan.group)
-        layout = _layout(output_grad)
-    query_grad, key_grad, value_grad = _gradient_of(query), _gradient_of(key), _gradient_of(value)
-    shape, workspace_bytes = _backward_plan(plan, layout, _layout(query_grad), _layout(key_grad), _layout(value_grad),
-                                            query.get_device())
+    query, key, value, output, kept, lengths, query_lengths = ctx.saved_tensors
+    forward = ctx.plan
+    device = query.get_device()
+    if output_grad.get_device() != device:
+        _lib.require_same_device('WindowAttention backward', query, output_grad)
+    plan = _backward_plan(forward, _layout(output_grad), query.dtype, device)
+    if plan is None:
+        output_grad = _for_kernel(output_grad, query.dtype, forward.group)
+        plan = _backward_plan(forward, _layout(output_grad), query.dtype, device)
+    shape, workspace_bytes = plan
+    like = forward.like_inputs
+    query_grad, key_grad, value_grad = \
+        _gradient_of(query, like[0]), _gradient_of(key, like[1]), _gradient_of(value, like[2])
     workspace = torch.empty(workspace_bytes, device=query.device, dtype=torch.uint8)
+    rest = kept.data_ptr()
     with _lib.device_guard(query):
         _lib.check(_lib.load().at_attention_bwd(
             ctypes.byref(shape), output_grad.data_ptr(), query.data_ptr(), key.data_ptr(), value.data_ptr(),
-            _lib.ptr(lengths), _lib.ptr(query_lengths), output.data_ptr(), _lib.ptr(rest), lse.data_ptr(),
-            query_grad.data_ptr(), key_grad.data_ptr(), value_grad.data_ptr(), workspace.data_ptr(), workspace_bytes,
-            _lib.stream_of(query)), 'at_attention_bwd')
+            None if lengths is None else lengths.data_ptr(),
+            None if query_lengths is None else query_lengths.data_ptr(), output.data_ptr(), rest,
+            rest + forward.rest_bytes, query_grad.data_ptr(), key_grad.data_ptr(), value_grad.data_ptr(),
+            workspace.data_ptr(), workspace_bytes, _lib.stream_of(query)), 'at_attention_bwd')
     head_dim = ctx.head_dim
     if head_dim != query.shape[3]:
         query_grad, key_grad, value_grad = (grad[..., :head_dim] for grad in (query_grad, key_grad, value_grad))

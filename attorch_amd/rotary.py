@@ -142,8 +142,10 @@ def _rotate(query: Optional[Tensor], key: Optional[Tensor], positions: Optional[
                       inverse)
     with _lib.device_guard(inv_freq):
         _lib.check(_lib.load().at_rotary(
-            ctypes.byref(shape), _lib.ptr(query), _lib.ptr(key), _lib.ptr(query_out), _lib.ptr(key_out),
-            _lib.ptr(positions), inv_freq.data_ptr(), _lib.ptr(pair_axis), _lib.stream_of(inv_freq)), 'at_rotary')
+            ctypes.byref(shape), None if query is None else query.data_ptr(), None if key is None else key.data_ptr(),
+            None if query is None else query_out.data_ptr(), None if key is None else key_out.data_ptr(),
+            None if positions is None else positions.data_ptr(), inv_freq.data_ptr(),
+            None if pair_axis is None else pair_axis.data_ptr(), _lib.stream_of(inv_freq)), 'at_rotary')
     return query_out, key_out
 
 
