@@ -333,15 +333,12 @@ __global__ __launch_bounds__(kWaves * 64, KT == 1 && sizeof(T) == 2 ? 2 : 1) voi
       for (int kt = 0; kt < KT; ++kt) s[kt] = dp[kt] = zero_acc();
 #pragma unroll
       for (int ks = 0; ks < L::kSteps; ++ks) {
-        const F qf = L::rows_frag(lr, 0, n * 32, ks);
+        const F qf = L::rows_frag(lr, 0, n * 32, ks), df = L::rows_frag(lr, kTileBytes, n * 32, ks);
 #pragma unroll
-        for (int kt = 0; kt < KT; ++kt) s[kt] = Frag<T>::mma(qf, kf[kt][ks], s[kt]);
-      }
-#pragma unroll
-      for (int ks = 0; ks < L::kSteps; ++ks) {
-        const F df = L::rows_frag(lr, kTileBytes, n * 32, ks);
-#pragma unroll
-        for (int kt = 0; kt < KT; ++kt) dp[kt] = Frag<T>::mma(df, vf[kt][ks], dp[kt]);
+        for (int kt = 0; kt < KT; ++kt) {
+          s[kt] = Frag<T>::mma(qf, kf[kt][ks], s[kt]);
+          dp[kt] = Frag<T>::mma(df, vf[kt][ks], dp[kt]);
+        }
       }
 #pragma unroll
       for (int q = 0; q < 4; ++q) {

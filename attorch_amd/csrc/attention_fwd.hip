@@ -119,11 +119,11 @@ __global__ __launch_bounds__(kWaves * 64, sizeof(T) == 2 ? 2 : 1) void attention
 
     const typename L::Reader lr = L::reader(stage);
     f32x16 s[2];
+    s[0] = s[1] = zero_acc();
 #pragma unroll
-    for (int n = 0; n < 2; ++n) {
-      s[n] = zero_acc();
-#pragma unroll
-      for (int ks = 0; ks < L::kSteps; ++ks) s[n] = Frag<T>::mma(L::rows_frag(lr, 0, n * 32, ks), qf[ks], s[n]);
+    for (int ks = 0; ks < L::kSteps; ++ks) {
+      s[0] = Frag<T>::mma(L::rows_frag(lr, 0, 0, ks), qf[ks], s[0]);
+      s[1] = Frag<T>::mma(L::rows_frag(lr, 0, 32, ks), qf[ks], s[1]);
     }
     // keys of the lane relative to its first one, as constants: 8 apart, 4 in a row
     const bool whole = k0 >= last - a.left && k0 + kKeys - 1 <= min(first + a.right, seq.len - 1);

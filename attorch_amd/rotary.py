@@ -39,22 +39,6 @@ def _layout(tensor: Tensor) -> Layout:
     return tensor.shape, tensor.stride(), tensor.dtype
 
 
-def _features(tensor: Tensor) -> Tensor:
-    """
-    The tensor itself if its features lie side by side, otherwise a copy.
-    """
-    return tensor if tensor.stride(3) == 1 or tensor.shape[3] <= 1 else tensor.contiguous()
-
-
-def _turned(tensor: Tensor) -> Tensor:
-    """
-    New tensor for the turned one: in its layout where that is dense and keeps the features side by side.
-    """
-    output = torch.empty_like(tensor)
-    return output if output.stride(3) == 1 or output.shape[3] <= 1 else \
-        torch.empty(output.shape, device=output.device, dtype=output.dtype)
-
-
 def _positions_of(positions: Optional[Tensor], axes: int, batch: int, rows: int) -> Optional[Tensor]:
     """
     Positions as [axes, batch, rows], without a copy.
@@ -75,12 +59,10 @@ def _positions_of(positions: Optional[Tensor], axes: int, batch: int, rows: int)
     return positions.unsqueeze(1).expand(axes, batch, rows)
 
 
-@functools.lru_cache(maxsize=4096)
-def _check(query: Layout, key: Optional[Layout], positions: Optional[torch.Size], inv_freq: Layout,
+def _check(query: Layout, key: Optional[Layout], positions: Optional[Layout], inv_freq: Layout,
            pair_axis: Optional[Layout]) -> int:
     """
     Refuses what the kernel does not compute, before anything is launched; returns the number of axes.
-    Remembered by layouts: a program repeats few of them.
     """
     shape = tuple(query[0])
     assert len(shape) == 4, f'Queries must be [batch, heads, rows, head_dim], received {shape}'
@@ -101,45 +83,61 @@ def _check(query: Layout, key: Optional[Layout], positions: Optional[torch.Size]
         raise RuntimeError(f'pair_axis must be int32, received {pair_axis[2]}')
     assert pair_axis[0] == inv_freq[0], \
         f'pair_axis ({tuple(pair_axis[0])}) must have the shape of inv_freq ({tuple(inv_freq[0])})'
-    assert positions is not None and len(positions) in (2, 3) and positions[0] > 0, \
+    assert positions is not None and len(positions[0]) in (2, 3) and positions[0][0] > 0, \
         'Axes of pairs need positions of shape [axes, batch, rows] or [axes, rows]'
-    return positions[0]
+    return positions[0][0]
+
+
+def _side_by_side(layout: Layout) -> bool:
+    return layout[1][3] == 1 or layout[0][3] <= 1 or 0 in layout[0]
 
 
 @functools.lru_cache(maxsize=4096)
-def _shape_of(query: Optional[Layout], key: Optional[Layout], query_out: Optional[Layout], key_out: Optional[Layout],
-              positions: Optional[Layout], pairs: int, axes: int, adjacent: bool, inverse: bool) -> _Shape:
+def _plan(query: Optional[Layout], key: Optional[Layout], positions: Optional[Layout], inv_freq: Layout,
+          pair_axis: Optional[Layout], adjacent: bool, inverse: bool) -> Optional[_Shape]:
     """
-    Description of a call for the kernel, remembered by layouts and options.
+    Checks the arguments and describes the call for the kernel; None where the features of the queries or
+    keys do not lie side by side.  Remembered by layouts and options: a program repeats few of them, and
+    the description takes longer than a small call's kernel.
     """
     present = query if query is not None else key
+    axes = _check(present, key if query is not None else None, positions, inv_freq, pair_axis)
     batch, _, rows, dim = present[0]
-    strides = []
-    for layout in (query, key, query_out, key_out):
-        strides += (0, 0, 0) if layout is None else layout[1][:3]
-    return _Shape(batch, rows, 0 if query is None else query[0][1], 0 if key is None else key[0][1], dim, pairs, axes,
-                  (ctypes.c_int64 * 12)(*strides), (ctypes.c_int64 * 3)(*((0, 0, 0) if positions is None else positions[1])),
-                  0 if positions is None else POSITION_TYPES[positions[2]], adjacent, inverse, _lib.dtype_id(present[2]))
+    position_type, position_strides = 0, (0, 0, 0)
+    if positions is not None:
+        expanded = _positions_of(torch.empty_strided(*positions[:2], dtype=positions[2], device='meta'), axes, batch, rows)
+        position_type, position_strides = POSITION_TYPES[positions[2]], expanded.stride()
+    strides = [0] * 12
+    for n, layout in enumerate((query, key)):
+        if layout is None:
+            continue
+        if not _side_by_side(layout):
+            return None
+        # the output takes the input's layout where that is dense; torch.empty_like keeps the order of the strides
+        output = torch.empty_like(torch.empty_strided(*layout[:2], dtype=layout[2], device='meta'))
+        strides[3 * n:3 * n + 3] = layout[1][:3]
+        strides[6 + 3 * n:9 + 3 * n] = output.stride()[:3]
+        if not _side_by_side((output.shape, output.stride(), output.dtype)):
+            return None
+    return _Shape(batch, rows, 0 if query is None else query[0][1], 0 if key is None else key[0][1], dim, inv_freq[0][0],
+                  axes, (ctypes.c_int64 * 12)(*strides), (ctypes.c_int64 * 3)(*position_strides), position_type, adjacent,
+                  inverse, _lib.dtype_id(present[2]))
 
 
 def _rotate(query: Optional[Tensor], key: Optional[Tensor], positions: Optional[Tensor], inv_freq: Tensor,
-            pair_axis: Optional[Tensor], axes: int, adjacent: bool,
-            inverse: bool) -> Tuple[Optional[Tensor], Optional[Tensor]]:
+            pair_axis: Optional[Tensor], adjacent: bool, inverse: bool) -> Tuple[Optional[Tensor], Optional[Tensor]]:
     """
     Turns the queries and keys (either may be absent) by their positions' angles, or back.
     """
-    query_out = key_out = None
-    layouts = [None] * 4
-    if query is not None:
-        query = _features(query)
-        query_out = _turned(query)
-        layouts[0], layouts[2] = _layout(query), _layout(query_out)
-    if key is not None:
-        key = _features(key)
-        key_out = _turned(key)
-        layouts[1], layouts[3] = _layout(key), _layout(key_out)
-    shape = _shape_of(*layouts, None if positions is None else _layout(positions), inv_freq.shape[0], axes, adjacent,
-                      inverse)
+    tables = (None if positions is None else _layout(positions), _layout(inv_freq),
+              None if pair_axis is None else _layout(pair_axis), adjacent, inverse)
+    shape = _plan(None if query is None else _layout(query), None if key is None else _layout(key), *tables)
+    if shape is None:
+        query, key = (None if t is None else t.contiguous() for t in (query, key))
+        shape = _plan(None if query is None else _layout(query), None if key is None else _layout(key), *tables)
+    _lib.require_same_device('Rotary', inv_freq, query, key, positions, pair_axis)
+    query_out = None if query is None else torch.empty_like(query)
+    key_out = None if key is None else torch.empty_like(key)
     with _lib.device_guard(inv_freq):
         _lib.check(_lib.load().at_rotary(
             ctypes.byref(shape), None if query is None else query.data_ptr(), None if key is None else key.data_ptr(),
@@ -182,18 +180,14 @@ class RotaryAutoGrad(torch.autograd.Function):
         Returns:
             Turned queries and keys (None without keys), of the dtypes of the inputs.
         """
-        axes = _check(_layout(query), None if key is None else _layout(key), None if positions is None else positions.shape,
-                      _layout(inv_freq), None if pair_axis is None else _layout(pair_axis))
-        positions = _positions_of(positions, axes, query.shape[0], query.shape[2])
-        _lib.require_same_device('Rotary', query, key, positions, inv_freq, pair_axis)
         if not inv_freq.is_contiguous():
             inv_freq = inv_freq.contiguous()
         if pair_axis is not None and not pair_axis.is_contiguous():
             pair_axis = pair_axis.contiguous()
 
         adjacent = bool(adjacent)
-        outputs = _rotate(query, key, positions, inv_freq, pair_axis, axes, adjacent, False)
-        ctx.options = (axes, adjacent)
+        outputs = _rotate(query, key, positions, inv_freq, pair_axis, adjacent, False)
+        ctx.adjacent = adjacent
         ctx.save_for_backward(positions, inv_freq, pair_axis)
         ctx.set_materialize_grads(False)
         return outputs
@@ -219,8 +213,7 @@ def _backward(ctx: Any, query_grad: Optional[Tensor], key_grad: Optional[Tensor]
     if not ctx.needs_input_grad[1]:
         key_grad = None
     if query_grad is not None or key_grad is not None:
-        _lib.require_same_device('Rotary backward', inv_freq, query_grad, key_grad)
-        query_grad, key_grad = _rotate(query_grad, key_grad, positions, inv_freq, pair_axis, *ctx.options, True)
+        query_grad, key_grad = _rotate(query_grad, key_grad, positions, inv_freq, pair_axis, ctx.adjacent, True)
 
     # One gradient (or None) per forward argument.
     return query_grad, key_grad, None, None, None, None
