@@ -34,7 +34,7 @@ struct AttentionArgs {
   const void* query_lengths;           // live rows of each sequence, or null: `rows` of all
   int lengths64, causal;
   int batch, kv_heads, group, rows, keys, dim;
-  int row_pitch, tiles, splits;
+  int row_pitch, tiles, splits, waves_per_row;
   int tile_keys, sink_tiles, sink_chunks, chunks, chunk_steps;   // dk and dv: see chunk_plan
   int left, right, sinks;
   float scale, scale_log2;
@@ -282,6 +282,21 @@ template <typename T, int DT> struct Tile {
       const int off = offset(row + n * NW * kLoadRows);
       dma_16(rsrc, off >= 0 ? lane_offset<NW>(off, dim_bytes, n) : kOobOffset, 0, dst + n * NW * 1024);
     }
+  }
+};
+
+// A wave's accumulators through LDS, one word per lane and step: `room` bytes serve a wave.
+template <int N> struct Exchange {
+  static constexpr int kBytes = N * 256;
+  template <int M> static __device__ __forceinline__ void put(char* room, int first, const f32x16 (&v)[M]) {
+    float* p = reinterpret_cast<float*>(room) + (threadIdx.x & 63) + first * 64;
+#pragma unroll
+    for (int m = 0; m < M; ++m)
+#pragma unroll
+      for (int e = 0; e < 16; ++e) p[(m * 16 + e) * 64] = v[m][e];
+  }
+  static __device__ __forceinline__ float get(const char* room, int at) {
+    return reinterpret_cast<const float*>(room)[at * 64 + (threadIdx.x & 63)];
   }
 };
 

@@ -18,13 +18,14 @@ namespace at_hip {
 namespace {
 
 constexpr int kWaves = 4;
-constexpr int kTileRows = 32 * kWaves;   // rows (dq) or keys (dk, dv) that a workgroup owns
 constexpr int kStep = 64;                // keys or rows of a tile it walks over
 
-template <typename T, int DT>
+// WK waves share 32 rows and halve each tile of keys among them (1 or 2); they join at the end.
+template <typename T, int DT, int WK>
 __global__ __launch_bounds__(kWaves * 64, sizeof(T) == 2 ? 2 : 1) void attention_dq_kernel(AttentionArgs a) {
   typedef Tile<T, DT> L;
   typedef typename Frag<T>::type F;
+  constexpr int kRows = 32 * kWaves / WK, kMine = kStep / WK;
   constexpr int kTileBytes = kStep * L::kPitch;
   __shared__ __attribute__((aligned(1024))) char lds[4 * kTileBytes];   // two stages of keys | values
 
@@ -36,9 +37,10 @@ __global__ __launch_bounds__(kWaves * 64, sizeof(T) == 2 ? 2 : 1) void attention
   const int b = bh / a.kv_heads, h = bh - b * a.kv_heads;
   const Sequence seq = sequence_of(a, b);
   const int live_rows = seq.live * a.group, all_rows = a.rows * a.group;
-  const int row0 = tile_id * kTileRows;
+  const int row0 = tile_id * kRows;
 
-  const int row = row0 + wave * 32 + (lane & 31);
+  const int wave_row = wave / WK * 32, wave_key = wave % WK * kMine;
+  const int row = row0 + wave_row + (lane & 31);
   const int i = row / a.group, g = row - i * a.group;
   const bool valid = row < live_rows;
   const int head = h * a.group + g;
@@ -83,7 +85,7 @@ __global__ __launch_bounds__(kWaves * 64, sizeof(T) == 2 ? 2 : 1) void attention
   const int p = seq.start + i;
   const int see_lo = valid ? p - a.left : 1, see_hi = valid ? min(p + a.right, seq.len - 1) : 0;
   const int see_sinks = valid ? min(a.sinks, a.causal ? p + 1 : seq.len) : 0;
-  const int wrow0 = row0 + wave * 32;
+  const int wrow0 = row0 + wave_row;
   const int first = seq.start + wrow0 / a.group;
   const int last = wrow0 < live_rows ? seq.start + (min(wrow0 + 32, live_rows) - 1) / a.group : first - 1;
   const KeyRange mine = keys_of(a, seq, first, last);
@@ -91,7 +93,7 @@ __global__ __launch_bounds__(kWaves * 64, sizeof(T) == 2 ? 2 : 1) void attention
   int tiles_lo = 0, sink_tiles = 0, tiles = 0;
   KeyRange range = {0, 0, 0};
   if (row0 < live_rows) {
-    range = keys_of(a, seq, seq.start + row0 / a.group, seq.start + (min(row0 + kTileRows, live_rows) - 1) / a.group);
+    range = keys_of(a, seq, seq.start + row0 / a.group, seq.start + (min(row0 + kRows, live_rows) - 1) / a.group);
     tiles_lo = range.lo / kStep;
     sink_tiles = min((range.sinks + kStep - 1) / kStep, tiles_lo);
     tiles = sink_tiles + (max(range.hi, range.sinks) + kStep - 1) / kStep - tiles_lo;
@@ -124,13 +126,13 @@ __global__ __launch_bounds__(kWaves * 64, sizeof(T) == 2 ? 2 : 1) void attention
     lds_dma_wait_all();
     __syncthreads();
     if (t + 1 < tiles) fetch(t + 1, lds + ((t + 1) & 1) * 2 * kTileBytes);
-    const int k0 = first_key(t);
-    if (!((k0 < mine.hi && k0 + kStep > mine.lo) || k0 < mine.sinks) || last < first) continue;
-    const bool whole = k0 >= last - a.left && k0 + kStep - 1 <= min(first + a.right, seq.len - 1);
+    const int k0 = first_key(t) + wave_key;
+    if (!((k0 < mine.hi && k0 + kMine > mine.lo) || k0 < mine.sinks) || last < first) continue;
+    const bool whole = k0 >= last - a.left && k0 + kMine - 1 <= min(first + a.right, seq.len - 1);
 
-    const typename L::Reader lr = L::reader(stage);
+    const typename L::Reader lr = L::reader(stage + wave_key * L::kPitch);
 #pragma unroll
-    for (int n = 0; n < kStep / 32; ++n) {
+    for (int n = 0; n < kMine / 32; ++n) {
       f32x16 s = zero_acc(), dp = zero_acc();
 #pragma unroll
       for (int ks = 0; ks < L::kSteps; ++ks) {
@@ -163,6 +165,19 @@ __global__ __launch_bounds__(kWaves * 64, sizeof(T) == 2 ? 2 : 1) void attention
     }
   }
 
+  if constexpr (WK > 1) {              // join the two halves of the keys
+    typedef Exchange<16 * DT> X;
+    static_assert(kWaves / 2 * X::kBytes <= (int)sizeof(lds), "the stages hold what is exchanged");
+    char* room = lds + wave / 2 * X::kBytes;
+    __syncthreads();                   // nobody reads the stages any more
+    if (wave % 2 == 1) X::put(room, 0, dq);
+    __syncthreads();
+    if (wave % 2 == 1) return;
+#pragma unroll
+    for (int dt = 0; dt < DT; ++dt)
+#pragma unroll
+      for (int e = 0; e < 16; ++e) dq[dt][e] += X::get(room, dt * 16 + e);
+  }
   if (row >= all_rows) return;
   char* gp = a.dq.p + b * a.dq.batch + head * a.dq.head + i * a.dq.token;
 #pragma unroll
@@ -506,7 +521,10 @@ int launch(AttentionArgs a, hipStream_t stream) {
   constexpr int KT = keys_per_wave<T, DT>() / 32;
   chunk_plan(a, kWaves * 32 * KT);
   const int64_t items = (int64_t)a.sink_tiles * a.sink_chunks + (int64_t)(a.tiles - a.sink_tiles) * a.chunks;
-  const int64_t row_tiles = cdiv64((int64_t)a.rows * a.group, kTileRows);
+  // tiles of 128 rows, or of 64 where these give no more than two workgroups per CU: see the forward pass
+  const int64_t rows = (int64_t)a.rows * a.group;
+  const bool share = cdiv64(rows, 32 * kWaves) * heads < 2 * device_cu_count();
+  const int64_t row_tiles = cdiv64(rows, 32 * kWaves / (share ? 2 : 1));
   const int64_t joined = ((a.chunks > 1 ? a.tiles : a.sink_tiles) - (a.sink_chunks > 1 ? 0 : a.sink_tiles)) *
                          (int64_t)a.tile_keys * heads;
   if (!grid_fits(row_tiles * heads) || !grid_fits(items * heads) || !grid_fits(cdiv64(joined, 8))) return AT_ERR_DIM;
@@ -514,7 +532,9 @@ int launch(AttentionArgs a, hipStream_t stream) {
   if (a.rows > 0) {
     AttentionArgs r = a;
     r.tiles = (int)row_tiles;
-    hipLaunchKernelGGL((attention_dq_kernel<T, DT>), dim3((unsigned)(row_tiles * heads)), dim3(kWaves * 64), 0, stream, r);
+    const dim3 grid((unsigned)(row_tiles * heads)), block(kWaves * 64);
+    if (share) hipLaunchKernelGGL((attention_dq_kernel<T, DT, 2>), grid, block, 0, stream, r);
+    else hipLaunchKernelGGL((attention_dq_kernel<T, DT, 1>), grid, block, 0, stream, r);
     rc = launch_status();
     if (rc != AT_OK) return rc;
   }

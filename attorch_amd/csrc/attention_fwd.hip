@@ -12,7 +12,6 @@ namespace {
 
 constexpr int kKeys = 64;        // keys of a tile
 constexpr int kWaves = 4;
-constexpr int kRows = 32 * kWaves;
 constexpr int kMaxSplits = 128;
 
 // Four elements of the output, and what their rounding left over where a backward pass will need it.
@@ -29,11 +28,13 @@ __device__ __forceinline__ void store_output(const AttentionArgs& a, int64_t to,
   }
 }
 
-template <typename T, int DT>
+// WK waves share 32 rows and halve each tile of keys among them (1 or 2); they join at the end.
+template <typename T, int DT, int WK>
 __global__ __launch_bounds__(kWaves * 64, sizeof(T) == 2 ? 2 : 1) void attention_fwd_kernel(AttentionArgs a) {
   typedef Tile<T, DT> L;
   typedef typename Frag<T>::type F;
   constexpr int kTileBytes = kKeys * L::kPitch;
+  constexpr int kRows = 32 * kWaves / WK, kMine = kKeys / WK, NS = kMine / 32;
   __shared__ __attribute__((aligned(1024))) char lds[4 * kTileBytes];   // two stages of keys | values
 
   const int lane = threadIdx.x & 63, half = lane >> 5;
@@ -46,7 +47,8 @@ __global__ __launch_bounds__(kWaves * 64, sizeof(T) == 2 ? 2 : 1) void attention
   const int live_rows = seq.live * a.group, all_rows = a.rows * a.group;
   const int row0 = tile_id * kRows;
 
-  const int row = row0 + wave * 32 + (lane & 31);
+  const int wave_row = wave / WK * 32, wave_key = wave % WK * kMine;
+  const int row = row0 + wave_row + (lane & 31);
   const int i = row / a.group, g = row - i * a.group;
   const bool valid = row < live_rows;
 
@@ -69,7 +71,7 @@ __global__ __launch_bounds__(kWaves * 64, sizeof(T) == 2 ? 2 : 1) void attention
   const int see_lo = valid ? p - a.left : 1, see_hi = valid ? min(p + a.right, seq.len - 1) : 0;
   const int see_sinks = valid ? min(a.sinks, a.causal ? p + 1 : seq.len) : 0;
   // tokens of the wave's rows (last < first: none is live)
-  const int wrow0 = row0 + wave * 32;
+  const int wrow0 = row0 + wave_row;
   const int first = seq.start + wrow0 / a.group;
   const int last = wrow0 < live_rows ? seq.start + (min(wrow0 + 32, live_rows) - 1) / a.group : first - 1;
   const KeyRange mine = keys_of(a, seq, first, last);
@@ -113,35 +115,35 @@ __global__ __launch_bounds__(kWaves * 64, sizeof(T) == 2 ? 2 : 1) void attention
     lds_dma_wait_all();
     __syncthreads();     // tile t is everybody's, and nobody reads the other stage any more
     if (t + 1 < t_end) fetch(t + 1, lds + ((t - t_begin + 1) & 1) * 2 * kTileBytes);
-    const int k0 = first_key(t);
-    // does any row of the wave see any key of the tile?
-    if (!((k0 < mine.hi && k0 + kKeys > mine.lo) || k0 < mine.sinks) || last < first) continue;
+    const int k0 = first_key(t) + wave_key;
+    // does any row of the wave see any key of its part of the tile?
+    if (!((k0 < mine.hi && k0 + kMine > mine.lo) || k0 < mine.sinks) || last < first) continue;
 
-    const typename L::Reader lr = L::reader(stage);
-    f32x16 s[2];
-    s[0] = s[1] = zero_acc();
+    const typename L::Reader lr = L::reader(stage + wave_key * L::kPitch);
+    f32x16 s[NS];
 #pragma unroll
-    for (int ks = 0; ks < L::kSteps; ++ks) {
-      s[0] = Frag<T>::mma(L::rows_frag(lr, 0, 0, ks), qf[ks], s[0]);
-      s[1] = Frag<T>::mma(L::rows_frag(lr, 0, 32, ks), qf[ks], s[1]);
-    }
+    for (int n = 0; n < NS; ++n) s[n] = zero_acc();
+#pragma unroll
+    for (int ks = 0; ks < L::kSteps; ++ks)
+#pragma unroll
+      for (int n = 0; n < NS; ++n) s[n] = Frag<T>::mma(L::rows_frag(lr, 0, n * 32, ks), qf[ks], s[n]);
     // keys of the lane relative to its first one, as constants: 8 apart, 4 in a row
-    const bool whole = k0 >= last - a.left && k0 + kKeys - 1 <= min(first + a.right, seq.len - 1);
+    const bool whole = k0 >= last - a.left && k0 + kMine - 1 <= min(first + a.right, seq.len - 1);
     if (!whole) {
       int key = k0 + half * 4;
       asm volatile("" : "+v"(key));    // a branch: as selects the masks would be formed for every tile
       const int lo = see_lo - key, hi = see_hi - key, sinks = see_sinks - key;
 #pragma unroll
-      for (int n = 0; n < 2; ++n)
+      for (int n = 0; n < NS; ++n)
 #pragma unroll
         for (int e = 0; e < 16; ++e) {
           const int c = n * 32 + acc_row(e, 0);
           s[n][e] = (c >= lo && c <= hi) || c < sinks ? s[n][e] : -INFINITY;
         }
     }
-    float top = fmaxf(s[0][0], s[1][0]);
+    float top = -INFINITY;
 #pragma unroll
-    for (int e = 1; e < 16; ++e) top = fmaxf(fmaxf(top, s[0][e]), s[1][e]);
+    for (int e = 0; e < 16; ++e) top = fmaxf(fmaxf(top, s[0][e]), s[NS - 1][e]);
     top = half_max(top) * a.scale_log2;
     // The exponentials are taken relative to a maximum that may lag behind by kSlack: any reference gives
     // the same result, and moving it costs a pass over the output, which now is rare.
@@ -158,7 +160,7 @@ __global__ __launch_bounds__(kWaves * 64, sizeof(T) == 2 ? 2 : 1) void attention
     const float base = m == -INFINITY ? 0.f : ProbShift<T>::forward - m;   // -inf: the row has seen nothing yet
     float sum[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-    for (int n = 0; n < 2; ++n)
+    for (int n = 0; n < NS; ++n)
 #pragma unroll
       for (int e = 0; e < 16; ++e) {
         s[n][e] = __builtin_amdgcn_exp2f(fmaf(s[n][e], a.scale_log2, base));
@@ -166,7 +168,7 @@ __global__ __launch_bounds__(kWaves * 64, sizeof(T) == 2 ? 2 : 1) void attention
       }
     l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
 #pragma unroll
-    for (int ks = 0; ks < kKeys / 16; ++ks) {
+    for (int ks = 0; ks < kMine / 16; ++ks) {
       float pr[8];
 #pragma unroll
       for (int e = 0; e < 8; ++e) pr[e] = s[ks >> 1][(ks & 1) * 8 + e];
@@ -178,6 +180,28 @@ __global__ __launch_bounds__(kWaves * 64, sizeof(T) == 2 ? 2 : 1) void attention
   }
 
   l = half_sum(l);
+  if constexpr (WK > 1) {              // join the two halves of the keys
+    typedef Exchange<16 * DT + 2> X;
+    static_assert(kWaves / 2 * X::kBytes <= (int)sizeof(lds), "the stages hold what is exchanged");
+    char* room = lds + wave / 2 * X::kBytes;
+    __syncthreads();                   // nobody reads the stages any more
+    if (wave % 2 == 1) {
+      X::put(room, 2, o);
+      reinterpret_cast<float*>(room)[lane] = m;
+      reinterpret_cast<float*>(room)[64 + lane] = l;
+    }
+    __syncthreads();
+    if (wave % 2 == 1) return;
+    const float m1 = X::get(room, 0), l1 = X::get(room, 1), top = fmaxf(m, m1);
+    const float w0 = m == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(m - top);
+    const float w1 = m1 == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(m1 - top);
+    m = top;
+    l = l * w0 + l1 * w1;
+#pragma unroll
+    for (int dt = 0; dt < DT; ++dt)
+#pragma unroll
+      for (int e = 0; e < 16; ++e) o[dt][e] = o[dt][e] * w0 + X::get(room, 2 + dt * 16 + e) * w1;
+  }
   const float inv = l > 0.f ? 1.f / l : l == 0.f ? 0.f : l;
   if (!valid) {          // a padded row, beside which whole tiles were not masked
     l = 0.f;
@@ -280,35 +304,48 @@ __global__ __launch_bounds__(256) void attention_join_kernel(AttentionArgs a) {
     for (int r = all_rows + (threadIdx.x & 31); r < a.row_pitch; r += 32) lse[r] = INFINITY;
 }
 
-// Splits of the keys per tile of rows: none while the tiles alone give every CU two workgroups, otherwise
-// as many as fill two per CU with at least four tiles of keys each (the join is a launch of 4 us; a tile
-// takes a workgroup about 1).
-int split_count(const AttentionArgs& a) {
-  const int64_t groups = (int64_t)a.tiles * a.batch * a.kv_heads;
+// How the work is cut.  Tiles of 128 rows leave a wave 32 rows and all keys of a tile; where they give no
+// more than two workgroups per CU, tiles of 64 rows whose waves share rows in pairs give twice as many
+// waves the same work; and where these still do not give every CU two workgroups, the keys are split among
+// several with at least four tiles of keys each, which another launch of 4 us joins (a tile takes a
+// workgroup about 1).
+void plan(AttentionArgs& a) {
+  const int64_t heads = (int64_t)a.batch * a.kv_heads, rows = (int64_t)a.rows * a.group;
   const int64_t want = 2 * device_cu_count();
-  if (groups >= want || groups == 0) return 1;
+  a.waves_per_row = cdiv64(rows, 32 * kWaves) * heads < want ? 2 : 1;
+  const int64_t tile_rows = 32 * kWaves / a.waves_per_row;
+  a.tiles = (int)cdiv64(rows, tile_rows);
+  a.splits = 1;
+  const int64_t groups = a.tiles * heads;
+  if (groups >= want || groups == 0) return;
   // keys that one tile of rows can see
-  const int64_t span = (int64_t)a.left + a.right + cdiv64(kRows, a.group) + a.sinks;
+  const int64_t span = (int64_t)a.left + a.right + cdiv64(tile_rows, a.group) + a.sinks;
   const int64_t tiles = cdiv64(span < a.keys ? span : a.keys, kKeys);
   int64_t n = cdiv64(want, groups);
   if (n > tiles / 4) n = tiles / 4;
-  return (int)(n < 1 ? 1 : n > kMaxSplits ? kMaxSplits : n);
+  a.splits = (int)(n < 1 ? 1 : n > kMaxSplits ? kMaxSplits : n);
+}
+
+template <typename T, int DT>
+void launch(const AttentionArgs& a, const dim3& grid, hipStream_t stream) {
+  if (a.waves_per_row == 1) hipLaunchKernelGGL((attention_fwd_kernel<T, DT, 1>), grid, dim3(kWaves * 64), 0, stream, a);
+  else hipLaunchKernelGGL((attention_fwd_kernel<T, DT, 2>), grid, dim3(kWaves * 64), 0, stream, a);
 }
 
 template <typename T>
 int launch_dim(const AttentionArgs& a, hipStream_t stream) {
   const int64_t blocks = (int64_t)a.tiles * a.batch * a.kv_heads;
-  if (!grid_fits(blocks) || (a.splits > 1 && !grid_fits((int64_t)a.batch * a.kv_heads * a.rows * a.group))) return AT_ERR_DIM;
-  const dim3 grid((unsigned)blocks, (unsigned)a.splits), block(kWaves * 64);
+  const int64_t rows = (int64_t)a.batch * a.kv_heads * a.rows * a.group;
+  if (!grid_fits(blocks) || (a.splits > 1 && !grid_fits(rows))) return AT_ERR_DIM;
+  const dim3 grid((unsigned)blocks, (unsigned)a.splits);
   switch ((a.dim + 31) / 32) {
-    case 1: hipLaunchKernelGGL((attention_fwd_kernel<T, 1>), grid, block, 0, stream, a); break;
-    case 2: hipLaunchKernelGGL((attention_fwd_kernel<T, 2>), grid, block, 0, stream, a); break;
-    case 3: hipLaunchKernelGGL((attention_fwd_kernel<T, 3>), grid, block, 0, stream, a); break;
-    default: hipLaunchKernelGGL((attention_fwd_kernel<T, 4>), grid, block, 0, stream, a); break;
+    case 1: launch<T, 1>(a, grid, stream); break;
+    case 2: launch<T, 2>(a, grid, stream); break;
+    case 3: launch<T, 3>(a, grid, stream); break;
+    default: launch<T, 4>(a, grid, stream); break;
   }
   int rc = launch_status();
   if (rc == AT_OK && a.splits > 1) {
-    const int64_t rows = (int64_t)a.batch * a.kv_heads * a.rows * a.group;
     if (a.splits <= kFewSplits)
       hipLaunchKernelGGL((attention_join_kernel<T, 1>), dim3((unsigned)cdiv64(rows, 8)), dim3(256), 0, stream, a);
     else
@@ -338,8 +375,7 @@ int64_t at_attention_row_pitch(int64_t rows, int64_t heads, int64_t kv_heads) {
 int64_t at_attention_fwd_workspace_bytes(const at_attention_t* shape) {
   AttentionArgs a;
   if (attention_args(shape, a) != AT_OK) return 0;
-  a.tiles = (int)cdiv64((int64_t)a.rows * a.group, kRows);
-  a.splits = split_count(a);
+  plan(a);
   return part_bytes(a);
 }
 
@@ -357,8 +393,7 @@ int at_attention_fwd(const at_attention_t* shape, const void* q, const void* k, 
   a.query_lengths = query_lengths;
   a.lse = lse;
   a.rest = (char*)out_rest;
-  a.tiles = (int)cdiv64((int64_t)a.rows * a.group, kRows);
-  a.splits = split_count(a);
+  plan(a);
   const int64_t need = part_bytes(a);
   if (need > 0 && (!workspace || workspace_bytes < need)) return AT_ERR_WORKSPACE;
   a.part = (float*)workspace;
