@@ -3,16 +3,18 @@
 // The gradient is the same map with -a, so one kernel serves both directions.
 //
 // Bound by memory: every feature is read and written once.  A workgroup takes a few tokens, forms the
-// cosines and sines of their angles once in LDS (all heads of a token share them) and then streams
-// the heads of q and k.  The angles are formed in 64 bits and reduced by whole turns there: at
-// position 2^20 an fp32 product would already be off by 0.06 radians.
+// cosines and sines of their angles and the tokens' addresses once in LDS (all heads of a token share
+// them) and then streams the heads of q and k.  A lane keeps its place in a head and goes from head to
+// head, two at a time, so that it has four vectors in flight.  The angles are formed in 64 bits and
+// reduced by whole turns there: at position 2^20 an fp32 product would already be off by 0.06 radians.
 #include "at_common.h"
 
 namespace at_hip {
 namespace {
 
 constexpr int kMaxPairs = 512;
-constexpr int kTable = 1024;           // cosine and sine pairs in LDS
+constexpr int kTable = 1024;           // cosines and sines in LDS
+constexpr int kMaxTokens = 8;          // of a workgroup
 
 struct RotaryArgs {
   const char* in[2];                   // q, k
@@ -34,13 +36,72 @@ __device__ __forceinline__ double position_of(const RotaryArgs& a, int axis, int
   return (double)reinterpret_cast<const float*>(a.positions)[at];
 }
 
-// VEC features per access (1: any size and alignment).
+// What a lane turns or copies at a time: VEC features (1: any size and alignment) of either half of the
+// pairs, or of adjacent pairs, or of the rest.
+template <typename T, bool ADJACENT, int VEC> struct Item {
+  static constexpr int kWidth = VEC > 1 || !ADJACENT ? VEC : 2;    // features an adjacent item covers
+  static constexpr bool kTwo = !ADJACENT;                          // two places in a head
+  float u[kWidth], w[kTwo ? VEC : 1];
+
+  static __device__ __forceinline__ void read(const T* p, float (&v)[kWidth]) {
+    if constexpr (VEC > 1 || kWidth == 1) {
+      load_f32<T, kWidth>(p, v);
+    } else {
+      v[0] = to_f32(p[0]);
+      v[1] = to_f32(p[1]);
+    }
+  }
+  static __device__ __forceinline__ void write(T* p, const float (&v)[kWidth]) {
+    if constexpr (VEC > 1 || kWidth == 1) {
+      store_f32<T, kWidth>(p, v);
+    } else {
+      p[0] = from_f32<T>(v[0]);
+      p[1] = from_f32<T>(v[1]);
+    }
+  }
+  __device__ __forceinline__ void load(const T* head, int d, int pairs) {
+    read(head + d, u);
+    if constexpr (kTwo) load_f32<T, VEC>(head + d + pairs, w);
+  }
+  __device__ __forceinline__ void turn(const float* cs, const float* sn, int d) {
+    if constexpr (kTwo) {
+#pragma unroll
+      for (int j = 0; j < VEC; ++j) {
+        const float c = cs[d + j], s = sn[d + j], x = u[j], y = w[j];
+        u[j] = x * c - y * s;
+        w[j] = x * s + y * c;
+      }
+    } else {
+#pragma unroll
+      for (int j = 0; j < kWidth; j += 2) {
+        const float c = cs[(d + j) >> 1], s = sn[(d + j) >> 1], x = u[j], y = u[j + 1];
+        u[j] = x * c - y * s;
+        u[j + 1] = x * s + y * c;
+      }
+    }
+  }
+  __device__ __forceinline__ void store(T* head, int d, int pairs) const {
+    write(head + d, u);
+    if constexpr (kTwo) store_f32<T, VEC>(head + d + pairs, w);
+  }
+};
+
 template <typename T, bool ADJACENT, int VEC>
 __global__ __launch_bounds__(256) void rotary_kernel(RotaryArgs a) {
+  typedef Item<T, ADJACENT, VEC> I;
   __shared__ float table_cos[kTable], table_sin[kTable];
+  __shared__ int64_t base[kMaxTokens][4];      // token's offsets in q, k, q_out, k_out
   const int64_t first = (int64_t)blockIdx.x * a.group;
   const int count = (int)(a.tokens - first < a.group ? a.tokens - first : a.group);
 
+  if ((int)threadIdx.x < count) {
+    const int64_t b = (first + threadIdx.x) / a.rows, t = first + threadIdx.x - b * a.rows;
+#pragma unroll
+    for (int n = 0; n < 2; ++n) {
+      base[threadIdx.x][n] = b * a.in_stride[n][0] + t * a.in_stride[n][2];
+      base[threadIdx.x][2 + n] = b * a.out_stride[n][0] + t * a.out_stride[n][2];
+    }
+  }
   for (int n = threadIdx.x; n < count * a.pairs; n += 256) {
     const int local = n / a.pairs, pair = n - local * a.pairs;
     const int64_t b = (first + local) / a.rows;
@@ -54,64 +115,60 @@ __global__ __launch_bounds__(256) void rotary_kernel(RotaryArgs a) {
   }
   __syncthreads();
 
-  // items of a head: vectors of pairs, then vectors of the features that are only copied
-  constexpr int kWidth = VEC > 1 || !ADJACENT ? VEC : 2;           // features an adjacent item covers
-  const int turned = ADJACENT ? 2 * a.pairs / kWidth : a.pairs / VEC;
-  const int rest = a.dim - 2 * a.pairs;
-  const int items = turned + rest / VEC;
-  for (int local = 0; local < count; ++local) {
-    const int64_t b = (first + local) / a.rows;
-    const int t = (int)(first + local - b * a.rows);
-    const float* cs = table_cos + local * a.pairs;
-    const float* sn = table_sin + local * a.pairs;
-    for (int n = threadIdx.x; n < a.heads * items; n += 256) {
-      int head = n / items;
-      const int item = n - head * items;
-      const int which = head >= a.q_heads;
-      head -= which ? a.q_heads : 0;
-      const T* x = reinterpret_cast<const T*>(a.in[which] + b * a.in_stride[which][0] + head * a.in_stride[which][1] +
-                                              t * a.in_stride[which][2]);
-      T* y = reinterpret_cast<T*>(a.out[which] + b * a.out_stride[which][0] + head * a.out_stride[which][1] +
-                                  t * a.out_stride[which][2]);
-      if (item >= turned) {
-        const int d = 2 * a.pairs + (item - turned) * VEC;
+  // places of a head: items of pairs, then vectors of the features that are only copied
+  const int turned = ADJACENT ? 2 * a.pairs / I::kWidth : a.pairs / VEC;
+  const int places = turned + (a.dim - 2 * a.pairs) / VEC;
+  const int across = places < 256 ? places : 256, step = 256 / across;
+  const int mine = (int)threadIdx.x / across;
+  if (mine >= step) return;
+  const int heads = count * a.heads;           // of all tokens
+  const float per_heads = 1.f / (float)a.heads;
+  auto find = [&](int n, const T*& x, T*& y, int& local) {
+    local = (int)(((float)n + 0.5f) * per_heads);   // n < 2^19: off by far less than the 0.5 / heads that would matter
+    int head = n - local * a.heads;
+    const int which = head >= a.q_heads;
+    head -= which ? a.q_heads : 0;
+    x = reinterpret_cast<const T*>(a.in[which] + base[local][which] + head * a.in_stride[which][1]);
+    y = reinterpret_cast<T*>(a.out[which] + base[local][2 + which] + head * a.out_stride[which][1]);
+  };
+  for (int place = (int)threadIdx.x - mine * across; place < places; place += across) {
+    if (place < turned) {
+      const int d = place * I::kWidth;
+      int n = mine;
+      for (; n + step < heads; n += 2 * step) {
+        const T *x0, *x1;
+        T *y0, *y1;
+        int t0, t1;
+        find(n, x0, y0, t0);
+        find(n + step, x1, y1, t1);
+        I i0, i1;
+        i0.load(x0, d, a.pairs);
+        i1.load(x1, d, a.pairs);
+        i0.turn(table_cos + t0 * a.pairs, table_sin + t0 * a.pairs, d);
+        i0.store(y0, d, a.pairs);
+        i1.turn(table_cos + t1 * a.pairs, table_sin + t1 * a.pairs, d);
+        i1.store(y1, d, a.pairs);
+      }
+      if (n < heads) {
+        const T* x;
+        T* y;
+        int t;
+        find(n, x, y, t);
+        I i;
+        i.load(x, d, a.pairs);
+        i.turn(table_cos + t * a.pairs, table_sin + t * a.pairs, d);
+        i.store(y, d, a.pairs);
+      }
+    } else {
+      const int d = 2 * a.pairs + (place - turned) * VEC;
+      for (int n = mine; n < heads; n += step) {
+        const T* x;
+        T* y;
+        int t;
+        find(n, x, y, t);
         float v[VEC];
         load_f32<T, VEC>(x + d, v);
         store_f32<T, VEC>(y + d, v);
-      } else if constexpr (ADJACENT) {
-        const int d = item * kWidth;
-        float v[kWidth];
-        if constexpr (VEC > 1) {
-          load_f32<T, kWidth>(x + d, v);
-        } else {
-          v[0] = to_f32(x[d]);
-          v[1] = to_f32(x[d + 1]);
-        }
-#pragma unroll
-        for (int j = 0; j < kWidth; j += 2) {
-          const float c = cs[(d + j) >> 1], s = sn[(d + j) >> 1], u = v[j], w = v[j + 1];
-          v[j] = u * c - w * s;
-          v[j + 1] = u * s + w * c;
-        }
-        if constexpr (VEC > 1) {
-          store_f32<T, kWidth>(y + d, v);
-        } else {
-          y[d] = from_f32<T>(v[0]);
-          y[d + 1] = from_f32<T>(v[1]);
-        }
-      } else {
-        const int d = item * VEC;
-        float u[VEC], w[VEC];
-        load_f32<T, VEC>(x + d, u);
-        load_f32<T, VEC>(x + d + a.pairs, w);
-#pragma unroll
-        for (int j = 0; j < VEC; ++j) {
-          const float c = cs[d + j], s = sn[d + j], p = u[j], q = w[j];
-          u[j] = p * c - q * s;
-          w[j] = p * s + q * c;
-        }
-        store_f32<T, VEC>(y + d, u);
-        store_f32<T, VEC>(y + d + a.pairs, w);
       }
     }
   }
@@ -184,7 +241,7 @@ int at_rotary(const at_rotary_t* s, const void* q, const void* k, void* q_out, v
   a.inverse = s->inverse != 0;
   // tokens of a workgroup: as many as fill its lanes with angles, as long as every CU keeps several workgroups
   int group = a.pairs > 0 ? 256 / a.pairs : 4;
-  if (group > 8) group = 8;
+  if (group > kMaxTokens) group = kMaxTokens;
   while (group > 1 && a.tokens / group < 4 * (int64_t)device_cu_count()) group /= 2;
   a.group = group < 1 ? 1 : group;
   if (cdiv64(a.tokens, a.group) >= ((int64_t)1 << 24)) return AT_ERR_DIM;
