@@ -35,7 +35,7 @@ struct AttentionArgs {
   int lengths64, causal;
   int batch, kv_heads, group, rows, keys, dim;
   int row_pitch, tiles, splits, waves_per_row;
-  int tile_keys, sink_tiles, sink_chunks, chunks, chunk_steps;   // dk and dv: see chunk_plan
+  int sink_tiles, far_chunks, far_steps, chunks, chunk_steps;   // dk and dv: see chunk_plan
   int left, right, sinks;
   float scale, scale_log2;
 };
@@ -62,7 +62,6 @@ __device__ __forceinline__ Sequence sequence_of(const AttentionArgs& a, int b) {
 // Keys that some row of the tokens [first, last] sees: [lo, hi) and the first `sinks`.
 struct KeyRange {
   int lo, hi, sinks;
-  __device__ __forceinline__ bool has(int key) const { return (key >= lo && key < hi) || key < sinks; }
 };
 
 __device__ __forceinline__ KeyRange keys_of(const AttentionArgs& a, const Sequence& s, int first, int last) {
@@ -72,6 +71,32 @@ __device__ __forceinline__ KeyRange keys_of(const AttentionArgs& a, const Sequen
   r.sinks = min(a.sinks, a.causal ? last + 1 : s.len);
   return r;
 }
+
+// The keys of a range as one list, which is walked over in tiles: place v of the list is key v for the
+// sinks (v < sinks) and key v + shift for the others (v >= begin).  The two parts follow each other
+// without a gap, so that a few sinks cost no tile of their own and the first tile of a window starts at
+// its first key, unless a tile that holds both would span more than a buffer offset can reach.
+struct KeyWalk {
+  int sinks, begin, end, shift;
+  __device__ __forceinline__ KeyWalk(const KeyRange& r, int64_t token_bytes, int tile) {
+    if (r.sinks >= r.lo) {             // one part
+      sinks = begin = shift = 0;
+      end = max(r.hi, r.sinks);
+    } else {
+      sinks = r.sinks;
+      begin = sinks % tile != 0 && (r.lo + tile) * token_bytes > 0x7fff0000 ? (sinks + tile - 1) / tile * tile : sinks;
+      shift = r.lo - begin;
+      end = r.hi - shift;
+    }
+  }
+  // Bytes from the tile's first key (place v0) to place v0 + r; negative where there is none.
+  __device__ __forceinline__ int offset(int v0, int r, int token_bytes) const {
+    const int v = v0 + r;
+    if (v < sinks) return r * token_bytes;
+    return v >= begin && v < end ? (r + (v0 < begin ? shift : 0)) * token_bytes : -1;
+  }
+  __device__ __forceinline__ int first_key(int v0) const { return v0 < begin ? v0 : v0 + shift; }
+};
 
 // Which piece of which head a workgroup takes: the pieces of a head stay on one XCD (workgroups go to
 // the 8 XCDs in turn), whose L2 then holds the head's keys and values, and four heads at a time come in

@@ -18,6 +18,7 @@ namespace at_hip {
 namespace {
 
 constexpr int kWaves = 4;
+constexpr int kTileKeys = 32 * kWaves;   // keys that a workgroup of the second kernel owns
 constexpr int kStep = 64;                // keys or rows of a tile it walks over
 
 // WK waves share 32 rows and halve each tile of keys among them (1 or 2); they join at the end.
@@ -90,33 +91,30 @@ __global__ __launch_bounds__(kWaves * 64, sizeof(T) == 2 ? 2 : 1) void attention
   const int last = wrow0 < live_rows ? seq.start + (min(wrow0 + 32, live_rows) - 1) / a.group : first - 1;
   const KeyRange mine = keys_of(a, seq, first, last);
 
-  int tiles_lo = 0, sink_tiles = 0, tiles = 0;
+  int tiles = 0;
   KeyRange range = {0, 0, 0};
-  if (row0 < live_rows) {
+  if (row0 < live_rows)
     range = keys_of(a, seq, seq.start + row0 / a.group, seq.start + (min(row0 + kRows, live_rows) - 1) / a.group);
-    tiles_lo = range.lo / kStep;
-    sink_tiles = min((range.sinks + kStep - 1) / kStep, tiles_lo);
-    tiles = sink_tiles + (max(range.hi, range.sinks) + kStep - 1) / kStep - tiles_lo;
-  }
+  const KeyWalk walk(range, max(a.k.token, a.v.token), kStep);
+  if (row0 < live_rows) tiles = (walk.end + kStep - 1) / kStep;
   const char* kb = a.k.p + b * a.k.batch + h * a.k.head;
   const char* vb = a.v.p + b * a.v.batch + h * a.v.head;
   const int dim_bytes = a.dim * (int)sizeof(T);
-  auto first_key = [&](int t) { return (t < sink_tiles ? t : t - sink_tiles + tiles_lo) * kStep; };
   const int key_off = L::template lane_row<kWaves>() * (int)a.k.token, val_off = L::template lane_row<kWaves>() * (int)a.v.token;
   const int key_offs[2] = {L::template lane_offset<kWaves>(key_off, dim_bytes, 0),
                            L::template lane_offset<kWaves>(key_off, dim_bytes, 1)};
   const int val_offs[2] = {L::template lane_offset<kWaves>(val_off, dim_bytes, 0),
                            L::template lane_offset<kWaves>(val_off, dim_bytes, 1)};
   auto fetch = [&](int t, char* stage) {
-    const int k0 = first_key(t);
+    const int v0 = t * kStep, k0 = walk.first_key(v0);
     const i32x4 kr = open_rsrc(kb + k0 * a.k.token), vr = open_rsrc(vb + k0 * a.v.token);
-    if (k0 >= range.lo && k0 + kStep <= range.hi) {
+    if (v0 >= walk.begin && v0 + kStep <= walk.end) {
       L::template fetch_all<kStep, kWaves>(kr, key_offs, kWaves * L::kLoadRows * (int)a.k.token, stage);
       L::template fetch_all<kStep, kWaves>(vr, val_offs, kWaves * L::kLoadRows * (int)a.v.token, stage + kTileBytes);
     } else {
-      L::template fetch<kStep, kWaves>(kr, dim_bytes, stage, [&](int r) { return range.has(k0 + r) ? r * (int)a.k.token : -1; });
+      L::template fetch<kStep, kWaves>(kr, dim_bytes, stage, [&](int r) { return walk.offset(v0, r, (int)a.k.token); });
       L::template fetch<kStep, kWaves>(vr, dim_bytes, stage + kTileBytes,
-                                      [&](int r) { return range.has(k0 + r) ? r * (int)a.v.token : -1; });
+                                      [&](int r) { return walk.offset(v0, r, (int)a.v.token); });
     }
   };
 
@@ -126,9 +124,11 @@ __global__ __launch_bounds__(kWaves * 64, sizeof(T) == 2 ? 2 : 1) void attention
     lds_dma_wait_all();
     __syncthreads();
     if (t + 1 < tiles) fetch(t + 1, lds + ((t + 1) & 1) * 2 * kTileBytes);
-    const int k0 = first_key(t) + wave_key;
-    if (!((k0 < mine.hi && k0 + kMine > mine.lo) || k0 < mine.sinks) || last < first) continue;
-    const bool whole = k0 >= last - a.left && k0 + kMine - 1 <= min(first + a.right, seq.len - 1);
+    // the wave's part of the tile: places v0 ..; behind the sinks these are the keys k0 ..
+    const int v0 = t * kStep + wave_key, k0 = v0 + walk.shift;
+    const bool mixed = t * kStep < walk.begin;
+    if (last < first || !(mixed || (k0 < mine.hi && k0 + kMine > mine.lo) || k0 < mine.sinks)) continue;
+    const bool whole = !mixed && k0 >= last - a.left && k0 + kMine - 1 <= min(first + a.right, seq.len - 1);
 
     const typename L::Reader lr = L::reader(stage + wave_key * L::kPitch);
 #pragma unroll
@@ -143,9 +143,9 @@ __global__ __launch_bounds__(kWaves * 64, sizeof(T) == 2 ? 2 : 1) void attention
       for (int e = 0; e < 16; ++e)
         s[e] = __builtin_amdgcn_exp2f(fmaf(s[e], a.scale_log2, -lse)) * (dp[e] - delta);
       if (!whole) {
-        int key = k0 + n * 32 + half * 4;
-        asm volatile("" : "+v"(key));    // a branch: as selects the masks would be formed for every tile
-        const int lo = see_lo - key, hi = see_hi - key, sinks = see_sinks - key;
+        int v = v0 + n * 32 + half * 4;
+        asm volatile("" : "+v"(v));      // a branch: as selects the masks would be formed for every tile
+        const int lo = max(see_lo - walk.shift, walk.begin) - v, hi = see_hi - walk.shift - v, sinks = see_sinks - v;
 #pragma unroll
         for (int e = 0; e < 16; ++e) {
           const int c = acc_row(e, 0);
@@ -191,89 +191,95 @@ __global__ __launch_bounds__(kWaves * 64, sizeof(T) == 2 ? 2 : 1) void attention
     }
 }
 
-// Work items of a head whose results are partial sums, and the number of item `nth` of its class among them.
-__host__ __device__ inline int64_t part_items(const AttentionArgs& a) {
-  return (int64_t)(a.sink_chunks > 1 ? a.sink_tiles * a.sink_chunks : 0) +
-         (a.chunks > 1 ? (int64_t)(a.tiles - a.sink_tiles) * a.chunks : 0);
+// The pieces of a head's dk and dv: `chunks` of every tile of keys, then `far_chunks` of the tiles with
+// sinks (chunk_plan says why).
+struct KeyPiece {
+  int tile, chunk;
+  bool far;
+};
+__host__ __device__ inline int key_pieces(const AttentionArgs& a) { return a.tiles * a.chunks + a.sink_tiles * a.far_chunks; }
+__device__ __forceinline__ KeyPiece key_piece(const AttentionArgs& a, int rank) {
+  const bool far = rank >= a.tiles * a.chunks;
+  const int n = far ? rank - a.tiles * a.chunks : rank, per_tile = far ? a.far_chunks : a.chunks;
+  return {n / per_tile, n % per_tile, far};
 }
-__host__ __device__ inline int64_t part_item(const AttentionArgs& a, bool of_sinks, int nth) {
-  return of_sinks || a.sink_chunks <= 1 ? nth : (int64_t)a.sink_tiles * a.sink_chunks + nth;
+
+// Partial sums of a head: of every tile where all have several chunks, otherwise of the tiles with sinks.
+// The place of a tile's first one (near chunks, then far ones), and for the last tile + 1 their number.
+__host__ __device__ inline int64_t first_part(const AttentionArgs& a, int tile) {
+  const int64_t sinks = tile < a.sink_tiles ? tile : a.sink_tiles;
+  return sinks * (a.chunks + a.far_chunks) + (a.chunks > 1 ? (tile - sinks) * (int64_t)a.chunks : 0);
 }
+
+// Waves that share the walk over the rows that see nothing but the sinks of a tile: the tile's other keys
+// must all lie within the near chunks, which start at the first row that sees the tile.  Not causal, that
+// is the first row of all, and holds for the first tile only.
+__host__ __device__ inline int sink_sharers(const AttentionArgs& a, int tile) {
+  if (!a.causal && tile > 0) return 1;
+  const int sinks = a.sinks - tile * kTileKeys;
+  return sinks <= 32 ? 4 : sinks <= 64 ? 2 : 1;
+}
+
+// Keys of a tile that far pieces have sums of.
+__host__ __device__ inline int far_keys(const AttentionArgs& a, int tile) { return kTileKeys / sink_sharers(a, tile); }
 
 __device__ __forceinline__ int wave_min(int v) {
   for (int o = 32; o > 0; o >>= 1) v = min(v, __shfl_xor(v, o, kWave));
   return __builtin_amdgcn_readfirstlane(v);
 }
 
-// A wave owns KT x 32 keys: their keys and values stay in registers as operands, and every fragment of
-// queries and output gradients that it reads from LDS serves KT products.
-template <typename T, int DT, int KT>
-__global__ __launch_bounds__(kWaves * 64, KT == 1 && sizeof(T) == 2 ? 2 : 1) void attention_dkv_kernel(AttentionArgs a) {
+// A wave owns 32 keys, whose keys and values stay in registers as operands, and walks over the rows that
+// see them.  Of the rows that see sinks only, the waves of a workgroup share the walk instead: those with
+// the same 32 keys take every second or fourth 32 rows (see chunk_plan for how the results are summed).
+template <typename T, int DT>
+__global__ __launch_bounds__(kWaves * 64, sizeof(T) == 2 ? 2 : 1) void attention_dkv_kernel(AttentionArgs a) {
   typedef Tile<T, DT> L;
   typedef typename Frag<T>::type F;
   constexpr int kTileBytes = kStep * L::kPitch;
   constexpr int kStage = 2 * kTileBytes + 2048;                       // queries | output gradients | lse | delta
-  constexpr int kTileKeys = 32 * KT * kWaves;
   __shared__ __attribute__((aligned(1024))) char lds[2 * kStage];
 
   const int lane = threadIdx.x & 63, half = lane >> 5;
   const int wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
-  // the first keys of a causal sequence are seen by the most rows
-  const Piece piece = piece_of(blockIdx.x, a.sink_tiles * a.sink_chunks + (a.tiles - a.sink_tiles) * a.chunks,
-                               a.batch * a.kv_heads);
-  const int item = piece.rank, bh = piece.bh;
-  const bool of_sinks = item < a.sink_tiles * a.sink_chunks;
-  const int nth = of_sinks ? item : item - a.sink_tiles * a.sink_chunks;
-  const int tile_chunks = of_sinks ? a.sink_chunks : a.chunks;
-  const int chunk = nth % tile_chunks;
-  const int tile_id = nth / tile_chunks + (of_sinks ? 0 : a.sink_tiles);
+  // the first keys of a causal sequence are seen by the most rows; the short far pieces come last
+  const Piece head_piece = piece_of(blockIdx.x, key_pieces(a), a.batch * a.kv_heads);
+  const int bh = head_piece.bh;
+  const KeyPiece piece = key_piece(a, head_piece.rank);
   const int b = bh / a.kv_heads, h = bh - b * a.kv_heads;
   const Sequence seq = sequence_of(a, b);
   const int live_rows = seq.live * a.group;
-  const int key0 = tile_id * kTileKeys + wave * 32 * KT + (lane & 31);   // this lane's keys: key0 + 32 kt
-
-  F kf[KT][L::kSteps], vf[KT][L::kSteps];
-  int row_lo[KT], row_hi[KT];          // rows [row_lo, row_hi] see the key
-  int any_lo = 1 << 30, any_hi = -1, all_lo = 0, all_hi = 1 << 30;
-#pragma unroll
-  for (int kt = 0; kt < KT; ++kt) {
-    const int key = key0 + 32 * kt;
-    const bool valid = key < seq.len;
+  // far from the tile's own tokens only its sinks are seen
+  const int sharers = piece.far ? sink_sharers(a, piece.tile) : 1;
+  const int subtile = wave % (kWaves / sharers), share = wave / (kWaves / sharers);
+  const int key = piece.tile * kTileKeys + subtile * 32 + (lane & 31);
+  int row_lo = 1 << 30, row_hi = -1;   // rows [row_lo, row_hi] see the key
+  if (key < seq.len) {
+    const bool sink = key < a.sinks;
+    const int tok_lo = !a.causal && sink ? seq.start : max(key - a.right, seq.start);
+    const int tok_hi = sink ? seq.len - 1 : min(key + a.left, seq.len - 1);
+    if (tok_lo <= tok_hi) {
+      row_lo = (tok_lo - seq.start) * a.group;
+      row_hi = min((tok_hi - seq.start) * a.group + a.group, live_rows) - 1;
+    }
+  }
+  F kf[L::kSteps], vf[L::kSteps];
+  {
     const char* kp = a.k.p + b * a.k.batch + h * a.k.head + key * a.k.token;
     const char* vp = a.v.p + b * a.v.batch + h * a.v.head + key * a.v.token;
-    row_lo[kt] = 1 << 30;
-    row_hi[kt] = -1;
-    if (valid) {
-      const bool sink = key < a.sinks;
-      const int tok_lo = !a.causal && sink ? seq.start : max(key - a.right, seq.start);
-      const int tok_hi = sink ? seq.len - 1 : min(key + a.left, seq.len - 1);
-      if (tok_lo <= tok_hi) {
-        row_lo[kt] = (tok_lo - seq.start) * a.group;
-        row_hi[kt] = min((tok_hi - seq.start) * a.group + a.group, live_rows) - 1;
-      }
-    }
 #pragma unroll
     for (int s = 0; s < L::kSteps; ++s) {
       const int d = s * 16 + half * 8;
-      const bool in = row_hi[kt] >= 0 && d < a.dim;       // what nothing sees is not read
-      kf[kt][s] = in ? Frag<T>::load(kp + d * sizeof(T)) : Frag<T>::zero();
-      vf[kt][s] = in ? Frag<T>::load(vp + d * sizeof(T)) : Frag<T>::zero();
+      const bool in = row_hi >= 0 && d < a.dim;       // what nothing sees is not read
+      kf[s] = in ? Frag<T>::load(kp + d * sizeof(T)) : Frag<T>::zero();
+      vf[s] = in ? Frag<T>::load(vp + d * sizeof(T)) : Frag<T>::zero();
     }
-    any_lo = min(any_lo, row_lo[kt]);
-    any_hi = max(any_hi, row_hi[kt]);
-    all_lo = max(all_lo, row_lo[kt]);
-    all_hi = min(all_hi, row_hi[kt]);
   }
   // rows that some key of the wave, and that every key of it, is seen by
-  any_lo = wave_min(any_lo);
-  any_hi = -wave_min(-any_hi);
-  all_lo = -wave_min(-all_lo);
-  all_hi = wave_min(all_hi);
-  f32x16 dk[KT][DT], dv[KT][DT];
+  const int any_lo = wave_min(row_lo), any_hi = -wave_min(-row_hi);
+  const int all_lo = -wave_min(-row_lo), all_hi = wave_min(row_hi);
+  f32x16 dk[DT], dv[DT];
 #pragma unroll
-  for (int kt = 0; kt < KT; ++kt)
-#pragma unroll
-    for (int dt = 0; dt < DT; ++dt) dk[kt][dt] = dv[kt][dt] = zero_acc();
+  for (int dt = 0; dt < DT; ++dt) dk[dt] = dv[dt] = zero_acc();
 
   __shared__ int ranges[2 * kWaves];
   if (lane == 0) {
@@ -287,8 +293,9 @@ __global__ __launch_bounds__(kWaves * 64, KT == 1 && sizeof(T) == 2 ? 2 : 1) voi
     begin = min(begin, ranges[w]);
     end = max(end, ranges[kWaves + w]);
   }
-  begin = begin / kStep + chunk * a.chunk_steps;
-  end = min(end < 0 ? 0 : end / kStep + 1, begin + a.chunk_steps);
+  const int steps = piece.far ? a.far_steps : a.chunk_steps;
+  begin = begin / kStep + (piece.far ? a.chunks * a.chunk_steps : 0) + piece.chunk * steps;
+  end = min(end < 0 ? 0 : end / kStep + 1, begin + steps);
   begin = __builtin_amdgcn_readfirstlane(begin);
   end = __builtin_amdgcn_readfirstlane(end);
 
@@ -341,19 +348,13 @@ __global__ __launch_bounds__(kWaves * 64, KT == 1 && sizeof(T) == 2 ? 2 : 1) voi
 #pragma unroll
     for (int n = 0; n < kStep / 32; ++n) {
       const int r0 = t * kStep + n * 32;
-      if (r0 > any_hi || r0 + 31 < any_lo) continue;
+      if (r0 > any_hi || r0 + 31 < any_lo || ((t * (kStep / 32) + n) & (sharers - 1)) != share) continue;
       const bool whole = r0 >= all_lo && r0 + 31 <= all_hi;
-      f32x16 s[KT], dp[KT];
-#pragma unroll
-      for (int kt = 0; kt < KT; ++kt) s[kt] = dp[kt] = zero_acc();
+      f32x16 s = zero_acc(), dp = zero_acc();
 #pragma unroll
       for (int ks = 0; ks < L::kSteps; ++ks) {
-        const F qf = L::rows_frag(lr, 0, n * 32, ks), df = L::rows_frag(lr, kTileBytes, n * 32, ks);
-#pragma unroll
-        for (int kt = 0; kt < KT; ++kt) {
-          s[kt] = Frag<T>::mma(qf, kf[kt][ks], s[kt]);
-          dp[kt] = Frag<T>::mma(df, vf[kt][ks], dp[kt]);
-        }
+        s = Frag<T>::mma(L::rows_frag(lr, 0, n * 32, ks), kf[ks], s);
+        dp = Frag<T>::mma(L::rows_frag(lr, kTileBytes, n * 32, ks), vf[ks], dp);
       }
 #pragma unroll
       for (int q = 0; q < 4; ++q) {
@@ -361,173 +362,194 @@ __global__ __launch_bounds__(kWaves * 64, KT == 1 && sizeof(T) == 2 ? 2 : 1) voi
         const float4 d4 = *reinterpret_cast<const float4*>(stats + 256 + n * 32 + q * 8 + half * 4);
         const float ls[4] = {l4.x, l4.y, l4.z, l4.w}, de[4] = {d4.x, d4.y, d4.z, d4.w};
 #pragma unroll
-        for (int kt = 0; kt < KT; ++kt)
-#pragma unroll
-          for (int j = 0; j < 4; ++j) {
-            const int e = q * 4 + j;
-            s[kt][e] = __builtin_amdgcn_exp2f(fmaf(s[kt][e], a.scale_log2, ProbShift<T>::backward - ls[j]));
-            dp[kt][e] = s[kt][e] * (dp[kt][e] - de[j]);
-          }
+        for (int j = 0; j < 4; ++j) {
+          const int e = q * 4 + j;
+          s[e] = __builtin_amdgcn_exp2f(fmaf(s[e], a.scale_log2, ProbShift<T>::backward - ls[j]));
+          dp[e] = s[e] * (dp[e] - de[j]);
+        }
       }
       if (!whole) {
         int row = r0 + half * 4;
         asm volatile("" : "+v"(row));    // a branch: as selects the masks would be formed for every tile
+        const int lo = row_lo - row, hi = row_hi - row;
 #pragma unroll
-        for (int kt = 0; kt < KT; ++kt) {
-          const int lo = row_lo[kt] - row, hi = row_hi[kt] - row;
-#pragma unroll
-          for (int e = 0; e < 16; ++e) {
-            const bool seen = acc_row(e, 0) >= lo && acc_row(e, 0) <= hi;
-            s[kt][e] = seen ? s[kt][e] : 0.f;
-            dp[kt][e] = seen ? dp[kt][e] : 0.f;
-          }
+        for (int e = 0; e < 16; ++e) {
+          const bool seen = acc_row(e, 0) >= lo && acc_row(e, 0) <= hi;
+          s[e] = seen ? s[e] : 0.f;
+          dp[e] = seen ? dp[e] : 0.f;
         }
       }
 #pragma unroll
       for (int t16 = 0; t16 < 2; ++t16) {
-        F pf[KT], df[KT];
+        float x[8], y[8];
 #pragma unroll
-        for (int kt = 0; kt < KT; ++kt) {
-          float x[8], y[8];
-#pragma unroll
-          for (int e = 0; e < 8; ++e) {
-            x[e] = s[kt][t16 * 8 + e];
-            y[e] = dp[kt][t16 * 8 + e];
-            if (ProbShift<T>::backward != 0.f) y[e] *= 1.f / 32768.f;
-          }
-          pf[kt] = Frag<T>::pack(x);
-          df[kt] = Frag<T>::pack(y);
+        for (int e = 0; e < 8; ++e) {
+          x[e] = s[t16 * 8 + e];
+          y[e] = dp[t16 * 8 + e];
+          if (ProbShift<T>::backward != 0.f) y[e] *= 1.f / 32768.f;
         }
+        const F pf = Frag<T>::pack(x), df = Frag<T>::pack(y);
 #pragma unroll
         for (int dt = 0; dt < DT; ++dt) {
-          const F dc = L::cols_frag(lr, kTileBytes, n * 32 + t16 * 16, dt);
-          const F qc = L::cols_frag(lr, 0, n * 32 + t16 * 16, dt);
-#pragma unroll
-          for (int kt = 0; kt < KT; ++kt) {
-            dv[kt][dt] = Frag<T>::mma(dc, pf[kt], dv[kt][dt]);
-            dk[kt][dt] = Frag<T>::mma(qc, df[kt], dk[kt][dt]);
-          }
+          dv[dt] = Frag<T>::mma(L::cols_frag(lr, kTileBytes, n * 32 + t16 * 16, dt), pf, dv[dt]);
+          dk[dt] = Frag<T>::mma(L::cols_frag(lr, 0, n * 32 + t16 * 16, dt), df, dk[dt]);
         }
       }
     }
+  }
+
+  if (sharers > 1) {                   // the first wave of each 32 keys takes the others' sums over
+    typedef Exchange<32 * DT> X;
+    static_assert(2 * X::kBytes <= (int)sizeof(lds), "the stages hold what is exchanged");
+    for (int n = kWaves / 2; n >= kWaves / sharers; n /= 2) {
+      __syncthreads();                 // nobody reads the stages, or what was exchanged, any more
+      if (wave >= n && wave < 2 * n) {
+        X::put(lds + (wave - n) * X::kBytes, 0, dk);
+        X::put(lds + (wave - n) * X::kBytes, 16 * DT, dv);
+      }
+      __syncthreads();
+      if (wave < n) {
+#pragma unroll
+        for (int dt = 0; dt < DT; ++dt)
+#pragma unroll
+          for (int e = 0; e < 16; ++e) {
+            dk[dt][e] += X::get(lds + wave * X::kBytes, dt * 16 + e);
+            dv[dt][e] += X::get(lds + wave * X::kBytes, (DT + dt) * 16 + e);
+          }
+      }
+    }
+    if (share > 0) return;
   }
 
   const float dv_scale = ProbShift<T>::backward != 0.f ? 1.f / 32768.f : 1.f;
-  float* part = a.part + ((int64_t)bh * part_items(a) + part_item(a, of_sinks, nth)) * 2 * kTileKeys * a.dim +
-                (int64_t)(wave * 32 * KT + (lane & 31)) * a.dim;
+  const bool partial = a.chunks > 1 || (piece.tile < a.sink_tiles && subtile * 32 < far_keys(a, piece.tile));
+  float* part = a.part + (int64_t)(wave * 32 + (lane & 31)) * a.dim +
+                (bh * first_part(a, a.tiles) + first_part(a, piece.tile) + (piece.far ? a.chunks : 0) + piece.chunk) *
+                    (2 * kTileKeys * a.dim);
+  char* kp = a.dk.p + b * a.dk.batch + h * a.dk.head + key * a.dk.token;
+  char* vp = a.dv.p + b * a.dv.batch + h * a.dv.head + key * a.dv.token;
 #pragma unroll
-  for (int kt = 0; kt < KT; ++kt) {
-    const int key = key0 + 32 * kt;
-    char* kp = a.dk.p + b * a.dk.batch + h * a.dk.head + key * a.dk.token;
-    char* vp = a.dv.p + b * a.dv.batch + h * a.dv.head + key * a.dv.token;
+  for (int dt = 0; dt < DT; ++dt)
 #pragma unroll
-    for (int dt = 0; dt < DT; ++dt)
+    for (int q = 0; q < 4; ++q) {
+      const int d = dt * 32 + q * 8 + half * 4;
+      float x[4], y[4];
 #pragma unroll
-      for (int q = 0; q < 4; ++q) {
-        const int d = dt * 32 + q * 8 + half * 4;
-        float x[4], y[4];
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          x[j] = dk[kt][dt][q * 4 + j] * a.scale;
-          y[j] = dv[kt][dt][q * 4 + j] * dv_scale;
-        }
-        if (d >= a.dim) continue;
-        if (tile_chunks > 1) {         // one of several partial sums
-          store_f32<float, 4>(part + kt * 32 * a.dim + d, x);
-          store_f32<float, 4>(part + (kTileKeys + kt * 32) * a.dim + d, y);
-        } else if (key < a.keys) {
-          store_f32<T, 4>(reinterpret_cast<T*>(kp) + d, x);
-          store_f32<T, 4>(reinterpret_cast<T*>(vp) + d, y);
-        }
+      for (int j = 0; j < 4; ++j) {
+        x[j] = dk[dt][q * 4 + j] * a.scale;
+        y[j] = dv[dt][q * 4 + j] * dv_scale;
       }
-  }
+      if (d >= a.dim) continue;
+      if (partial) {                   // one of several partial sums
+        store_f32<float, 4>(part + d, x);
+        store_f32<float, 4>(part + kTileKeys * a.dim + d, y);
+      } else if (key < a.keys) {
+        store_f32<T, 4>(reinterpret_cast<T*>(kp) + d, x);
+        store_f32<T, 4>(reinterpret_cast<T*>(vp) + d, y);
+      }
+    }
 }
 
-// Sums the partial dk and dv of the tiles that were worked on in chunks, in the chunks' order.  32 lanes per
-// key, four elements of dim per lane.
-template <typename T, int kTileKeys>
+// Sums the partial dk and dv of a key, in a fixed order.  32 lanes cover dim with four elements each.  A
+// workgroup of 8 such groups takes GROUPS of them for a key: one where all keys have a few sums, all 8
+// where only the sinks have any, and many.
+template <typename T, int GROUPS>
 __global__ __launch_bounds__(256) void attention_dkv_join_kernel(AttentionArgs a) {
-  const int first_tile = a.sink_chunks > 1 ? 0 : a.sink_tiles;
-  const int tiles = (a.chunks > 1 ? a.tiles : a.sink_tiles) - first_tile;
-  const int64_t at = (int64_t)blockIdx.x * 8 + (threadIdx.x >> 5);
-  const int bh = (int)(at / ((int64_t)tiles * kTileKeys));
-  if (bh >= a.batch * a.kv_heads) return;
-  const int rest = (int)(at - (int64_t)bh * tiles * kTileKeys);
-  const int tile = first_tile + rest / kTileKeys, local = rest % kTileKeys;
-  const int key = tile * kTileKeys + local, d = (threadIdx.x & 31) * 4;
-  if (key >= a.keys || d >= a.dim) return;
-  const bool of_sinks = tile < a.sink_tiles;
-  const int chunks = of_sinks ? a.sink_chunks : a.chunks;
-  const int nth = of_sinks ? tile * chunks : (tile - a.sink_tiles) * chunks;
-  const float* part = a.part + (((int64_t)bh * part_items(a) + part_item(a, of_sinks, nth)) * 2 * kTileKeys + local) * a.dim + d;
-  const int64_t other = (int64_t)kTileKeys * a.dim;
+  __shared__ float4 sums[2][8][32];
+  const unsigned tiles = a.chunks > 1 ? a.tiles : a.sink_tiles;
+  const unsigned at = blockIdx.x * (8 / GROUPS) + (GROUPS == 1 ? threadIdx.x >> 5 : 0);
+  const int bh = (int)(at / (tiles * kTileKeys)), rest = (int)(at - bh * tiles * kTileKeys);
+  const int tile = rest / kTileKeys, local = rest % kTileKeys;
+  const int key = tile * kTileKeys + local, group = GROUPS == 1 ? 0 : threadIdx.x >> 5, d = (threadIdx.x & 31) * 4;
+  const bool far = tile < a.sink_tiles && local < far_keys(a, tile);
+  if (key >= a.keys || (a.chunks == 1 && !far)) return;       // written by the only piece that has it
+  const int64_t next = 2LL * kTileKeys * a.dim;
+  const float* part = a.part + (bh * first_part(a, a.tiles) + first_part(a, tile)) * next + (int64_t)local * a.dim + d;
   float x[4] = {0.f, 0.f, 0.f, 0.f}, y[4] = {0.f, 0.f, 0.f, 0.f};
+  if (d < a.dim) {
 #pragma unroll 4
-  for (int c = 0; c < chunks; ++c) {
-    float u[4], w[4];
-    load_f32<float, 4>(part + c * 2 * other, u);
-    load_f32<float, 4>(part + c * 2 * other + other, w);
+    for (int n = group; n < a.chunks + (far ? a.far_chunks : 0); n += GROUPS) {
+      float u[4], w[4];
+      load_f32<float, 4>(part + n * next, u);
+      load_f32<float, 4>(part + n * next + (int64_t)kTileKeys * a.dim, w);
 #pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      x[j] += u[j];
-      y[j] += w[j];
+      for (int j = 0; j < 4; ++j) {
+        x[j] += u[j];
+        y[j] += w[j];
+      }
     }
   }
   const int b = bh / a.kv_heads, h = bh - b * a.kv_heads;
-  store_f32<T, 4>(reinterpret_cast<T*>(a.dk.p + b * a.dk.batch + h * a.dk.head + key * a.dk.token) + d, x);
-  store_f32<T, 4>(reinterpret_cast<T*>(a.dv.p + b * a.dv.batch + h * a.dv.head + key * a.dv.token) + d, y);
+  T* const to_k = reinterpret_cast<T*>(a.dk.p + b * a.dk.batch + h * a.dk.head + key * a.dk.token) + d;
+  T* const to_v = reinterpret_cast<T*>(a.dv.p + b * a.dv.batch + h * a.dv.head + key * a.dv.token) + d;
+  if constexpr (GROUPS == 1) {
+    if (d < a.dim) {
+      store_f32<T, 4>(to_k, x);
+      store_f32<T, 4>(to_v, y);
+    }
+  } else {
+    sums[0][group][threadIdx.x & 31] = make_float4(x[0], x[1], x[2], x[3]);
+    sums[1][group][threadIdx.x & 31] = make_float4(y[0], y[1], y[2], y[3]);
+    __syncthreads();
+    if (group > 1 || d >= a.dim) return;
+    float v[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int n = 0; n < 8; ++n) {
+      const float4 u = sums[group][n][threadIdx.x & 31];
+      v[0] += u.x; v[1] += u.y; v[2] += u.z; v[3] += u.w;
+    }
+    store_f32<T, 4>(group == 0 ? to_k : to_v, v);
+  }
 }
 
-#ifndef KTSEL
-#define KTSEL 32
-#endif
-constexpr int keys_per_wave(int dtype, int dim_tiles) { return dtype == AT_DTYPE_F32 ? 32 : KTSEL; }
-template <typename T, int DT> constexpr int keys_per_wave() { return keys_per_wave(dtype_of<T>::value, DT); }
-
-// How dk and dv are cut up.  The rows that see a tile of keys are walked over in chunks of chunk_steps
-// steps; tiles with one chunk write their result, the others partial sums that a second kernel adds.
-// With a window a tile is seen by few rows, but a tile with sinks by all: such tiles are cut to the
-// others' length, or one workgroup per head would run on alone (window 1024 over 8192 tokens: 5.1 ms
-// instead of 1.3).  Where the tiles alone do not give every CU two workgroups, all are cut further.
-void chunk_plan(AttentionArgs& a, int tile_keys) {
-  a.tile_keys = tile_keys;
-  a.tiles = (int)cdiv64(a.keys, tile_keys);
-  const int64_t rows = (int64_t)a.rows * a.group;
-  const int64_t near = (int64_t)(a.left + a.right + tile_keys) * a.group;
-  const int64_t span = near < rows ? near : rows;              // of a tile without sinks
-  a.sink_tiles = span < rows ? (int)cdiv64(a.sinks, tile_keys) : 0;
-  int64_t steps = cdiv64(span, kStep) + 1;                     // the first step need not start at the first row
-  const int64_t groups = (int64_t)a.tiles * a.batch * a.kv_heads;
+// How dk and dv are cut up.  The rows that see a tile of keys are walked over in steps of 64.  Where the
+// tiles alone do not give every CU two workgroups, the steps of each are cut into chunks, whose partial sums
+// another kernel adds.  With a window a tile is seen by few rows, but a tile with sinks by all of them: the
+// rows beyond the others' reach are far pieces of their own, short ones that fill up the end of the launch
+// (window 1024 over 8192 tokens, bf16: one workgroup per head for all rows of the sinks 5.1 ms).
+void chunk_plan(AttentionArgs& a) {
+  a.tiles = (int)cdiv64(a.keys, kTileKeys);
+  const int64_t heads = (int64_t)a.batch * a.kv_heads, rows = (int64_t)a.rows * a.group;
+  const int64_t near = (int64_t)(a.left + a.right + kTileKeys) * a.group;
+  const int64_t span = near < rows ? near : rows;              // rows that see a tile without sinks
   const int64_t want = 2 * device_cu_count();
-  if (groups < want && steps > 2) {
-    int64_t n = cdiv64(want, groups);
+  int64_t steps = cdiv64(span, kStep) + 1;                     // the first step need not start at the first row
+  a.chunks = 1;
+  if (a.tiles * heads < want && steps > 2) {
+    int64_t n = cdiv64(want, a.tiles * heads);
     if (n > steps / 2) n = steps / 2;
+    a.chunks = (int)n;
     steps = cdiv64(steps, n);
   }
   a.chunk_steps = (int)steps;
-  a.chunks = (int)cdiv64(cdiv64(span, kStep) + 1, steps);
-  a.sink_chunks = (int)cdiv64(cdiv64(rows, kStep) + 1, steps);
+  const int64_t far = cdiv64(rows, kStep) + 1 - steps * a.chunks;
+  a.sink_tiles = a.sinks > 0 && far > 0 ? (int)cdiv64(a.sinks, kTileKeys) : 0;
+  a.far_chunks = a.far_steps = 0;
+  if (a.sink_tiles > 0) {
+    int64_t n = cdiv64(want, a.sink_tiles * heads);
+    if (n > cdiv64(far, 8)) n = cdiv64(far, 8);
+    a.far_steps = (int)cdiv64(far, n);
+    a.far_chunks = (int)cdiv64(far, a.far_steps);
+  }
 }
 
 int64_t delta_bytes(const AttentionArgs& a) { return (int64_t)a.batch * a.kv_heads * a.row_pitch * 4; }
 
 int64_t part_bytes(const AttentionArgs& a) {
-  return (int64_t)a.batch * a.kv_heads * part_items(a) * 2 * a.tile_keys * a.dim * 4;
+  return (int64_t)a.batch * a.kv_heads * first_part(a, a.tiles) * 2 * kTileKeys * a.dim * 4;
 }
 
 template <typename T, int DT>
 int launch(AttentionArgs a, hipStream_t stream) {
   const int64_t heads = (int64_t)a.batch * a.kv_heads;
-  constexpr int KT = keys_per_wave<T, DT>() / 32;
-  chunk_plan(a, kWaves * 32 * KT);
-  const int64_t items = (int64_t)a.sink_tiles * a.sink_chunks + (int64_t)(a.tiles - a.sink_tiles) * a.chunks;
+  chunk_plan(a);
+  const int64_t pieces = key_pieces(a) * heads;
+  const int64_t joined = (int64_t)(a.chunks > 1 ? a.tiles : a.sink_tiles) * kTileKeys * heads;
   // tiles of 128 rows, or of 64 where these give no more than two workgroups per CU: see the forward pass
   const int64_t rows = (int64_t)a.rows * a.group;
   const bool share = cdiv64(rows, 32 * kWaves) * heads < 2 * device_cu_count();
   const int64_t row_tiles = cdiv64(rows, 32 * kWaves / (share ? 2 : 1));
-  const int64_t joined = ((a.chunks > 1 ? a.tiles : a.sink_tiles) - (a.sink_chunks > 1 ? 0 : a.sink_tiles)) *
-                         (int64_t)a.tile_keys * heads;
-  if (!grid_fits(row_tiles * heads) || !grid_fits(items * heads) || !grid_fits(cdiv64(joined, 8))) return AT_ERR_DIM;
+  if (!grid_fits(row_tiles * heads) || !grid_fits(pieces) || !grid_fits(joined)) return AT_ERR_DIM;
   int rc = AT_OK;
   if (a.rows > 0) {
     AttentionArgs r = a;
@@ -538,10 +560,13 @@ int launch(AttentionArgs a, hipStream_t stream) {
     rc = launch_status();
     if (rc != AT_OK) return rc;
   }
-  hipLaunchKernelGGL((attention_dkv_kernel<T, DT, KT>), dim3((unsigned)(items * heads)), dim3(kWaves * 64), 0, stream, a);
+  hipLaunchKernelGGL((attention_dkv_kernel<T, DT>), dim3((unsigned)pieces), dim3(kWaves * 64), 0, stream, a);
   rc = launch_status();
-  if (rc != AT_OK || part_items(a) == 0) return rc;
-  hipLaunchKernelGGL((attention_dkv_join_kernel<T, kWaves * 32 * KT>), dim3((unsigned)cdiv64(joined, 8)), dim3(256), 0, stream, a);
+  if (rc != AT_OK || joined == 0) return rc;
+  if (a.chunks > 1)                    // whole tiles of keys: a multiple of 8 of them
+    hipLaunchKernelGGL((attention_dkv_join_kernel<T, 1>), dim3((unsigned)(joined / 8)), dim3(256), 0, stream, a);
+  else
+    hipLaunchKernelGGL((attention_dkv_join_kernel<T, 8>), dim3((unsigned)joined), dim3(256), 0, stream, a);
   return launch_status();
 }
 
@@ -565,7 +590,7 @@ extern "C" {
 int64_t at_attention_bwd_workspace_bytes(const at_attention_t* shape) {
   AttentionArgs a;
   if (attention_args(shape, a) != AT_OK || a.keys == 0) return 0;
-  chunk_plan(a, kWaves * keys_per_wave(shape->dtype, (a.dim + 31) / 32));
+  chunk_plan(a);
   return delta_bytes(a) + part_bytes(a);
 }
 

@@ -76,36 +76,33 @@ __global__ __launch_bounds__(kWaves * 64, sizeof(T) == 2 ? 2 : 1) void attention
   const int last = wrow0 < live_rows ? seq.start + (min(wrow0 + 32, live_rows) - 1) / a.group : first - 1;
   const KeyRange mine = keys_of(a, seq, first, last);
 
-  int tiles_lo = 0, sink_tiles = 0, tiles = 0;
+  int tiles = 0;
   KeyRange range = {0, 0, 0};
-  if (row0 < live_rows) {
+  if (row0 < live_rows)
     range = keys_of(a, seq, seq.start + row0 / a.group, seq.start + (min(row0 + kRows, live_rows) - 1) / a.group);
-    tiles_lo = range.lo / kKeys;
-    sink_tiles = min((range.sinks + kKeys - 1) / kKeys, tiles_lo);
-    tiles = sink_tiles + (max(range.hi, range.sinks) + kKeys - 1) / kKeys - tiles_lo;
-  }
+  const KeyWalk walk(range, max(a.k.token, a.v.token), kKeys);
+  if (row0 < live_rows) tiles = (walk.end + kKeys - 1) / kKeys;
   const int split = blockIdx.y;
   const int t_begin = (int)((int64_t)tiles * split / a.splits), t_end = (int)((int64_t)tiles * (split + 1) / a.splits);
 
   const char* kb = a.k.p + b * a.k.batch + h * a.k.head;
   const char* vb = a.v.p + b * a.v.batch + h * a.v.head;
   const int dim_bytes = a.dim * (int)sizeof(T);
-  auto first_key = [&](int t) { return (t < sink_tiles ? t : t - sink_tiles + tiles_lo) * kKeys; };
   const int key_off = L::template lane_row<kWaves>() * (int)a.k.token, val_off = L::template lane_row<kWaves>() * (int)a.v.token;
   const int key_offs[2] = {L::template lane_offset<kWaves>(key_off, dim_bytes, 0),
                            L::template lane_offset<kWaves>(key_off, dim_bytes, 1)};
   const int val_offs[2] = {L::template lane_offset<kWaves>(val_off, dim_bytes, 0),
                            L::template lane_offset<kWaves>(val_off, dim_bytes, 1)};
   auto fetch = [&](int t, char* stage) {
-    const int k0 = first_key(t);
+    const int v0 = t * kKeys, k0 = walk.first_key(v0);
     const i32x4 kr = open_rsrc(kb + k0 * a.k.token), vr = open_rsrc(vb + k0 * a.v.token);
-    if (k0 >= range.lo && k0 + kKeys <= range.hi) {
+    if (v0 >= walk.begin && v0 + kKeys <= walk.end) {
       L::template fetch_all<kKeys, kWaves>(kr, key_offs, kWaves * L::kLoadRows * (int)a.k.token, stage);
       L::template fetch_all<kKeys, kWaves>(vr, val_offs, kWaves * L::kLoadRows * (int)a.v.token, stage + kTileBytes);
     } else {
-      L::template fetch<kKeys, kWaves>(kr, dim_bytes, stage, [&](int r) { return range.has(k0 + r) ? r * (int)a.k.token : -1; });
+      L::template fetch<kKeys, kWaves>(kr, dim_bytes, stage, [&](int r) { return walk.offset(v0, r, (int)a.k.token); });
       L::template fetch<kKeys, kWaves>(vr, dim_bytes, stage + kTileBytes,
-                                      [&](int r) { return range.has(k0 + r) ? r * (int)a.v.token : -1; });
+                                      [&](int r) { return walk.offset(v0, r, (int)a.v.token); });
     }
   };
 
@@ -115,9 +112,10 @@ __global__ __launch_bounds__(kWaves * 64, sizeof(T) == 2 ? 2 : 1) void attention
     lds_dma_wait_all();
     __syncthreads();     // tile t is everybody's, and nobody reads the other stage any more
     if (t + 1 < t_end) fetch(t + 1, lds + ((t - t_begin + 1) & 1) * 2 * kTileBytes);
-    const int k0 = first_key(t) + wave_key;
-    // does any row of the wave see any key of its part of the tile?
-    if (!((k0 < mine.hi && k0 + kMine > mine.lo) || k0 < mine.sinks) || last < first) continue;
+    // the wave's part of the tile: places v0 ..; behind the sinks these are the keys k0 ..
+    const int v0 = t * kKeys + wave_key, k0 = v0 + walk.shift;
+    const bool mixed = t * kKeys < walk.begin;
+    if (last < first || !(mixed || (k0 < mine.hi && k0 + kMine > mine.lo) || k0 < mine.sinks)) continue;
 
     const typename L::Reader lr = L::reader(stage + wave_key * L::kPitch);
     f32x16 s[NS];
@@ -127,12 +125,12 @@ __global__ __launch_bounds__(kWaves * 64, sizeof(T) == 2 ? 2 : 1) void attention
     for (int ks = 0; ks < L::kSteps; ++ks)
 #pragma unroll
       for (int n = 0; n < NS; ++n) s[n] = Frag<T>::mma(L::rows_frag(lr, 0, n * 32, ks), qf[ks], s[n]);
-    // keys of the lane relative to its first one, as constants: 8 apart, 4 in a row
-    const bool whole = k0 >= last - a.left && k0 + kMine - 1 <= min(first + a.right, seq.len - 1);
+    // places of the lane relative to its first one are constants: 8 apart, 4 in a row
+    const bool whole = !mixed && k0 >= last - a.left && k0 + kMine - 1 <= min(first + a.right, seq.len - 1);
     if (!whole) {
-      int key = k0 + half * 4;
-      asm volatile("" : "+v"(key));    // a branch: as selects the masks would be formed for every tile
-      const int lo = see_lo - key, hi = see_hi - key, sinks = see_sinks - key;
+      int v = v0 + half * 4;
+      asm volatile("" : "+v"(v));      // a branch: as selects the masks would be formed for every tile
+      const int lo = max(see_lo - walk.shift, walk.begin) - v, hi = see_hi - walk.shift - v, sinks = see_sinks - v;
 #pragma unroll
       for (int n = 0; n < NS; ++n)
 #pragma unroll

@@ -81,6 +81,19 @@ def test_windows(window, sinks, causal, dtype) -> None:
 
 @pytest.mark.parametrize('dtype', DTYPES)
 @pytest.mark.parametrize('causal', [True, False])
+@pytest.mark.parametrize('window, sinks', [(20, 1), (20, 33), (20, 64), (33, 65), (20, 129), (100, 140), (20, 300), (1, 700)])
+def test_sinks_far_from_their_readers(window, sinks, causal, dtype) -> None:
+    """
+    Rows that see the sinks of a tile of keys and nothing else of it, in whole batches, padded ones and
+    chunks over a cache.
+    """
+    check(*inputs(1, 4, 2, 700, 700, 32, dtype), causal=causal, window=window, sinks=sinks)
+    check(*inputs(2, 3, 1, 650, 650, 16, dtype), lengths=torch.tensor([333, 650]), causal=causal, window=window, sinks=sinks)
+    check(*inputs(1, 2, 2, 200, 900, 32, dtype), causal=causal, window=window, sinks=sinks)
+
+
+@pytest.mark.parametrize('dtype', DTYPES)
+@pytest.mark.parametrize('causal', [True, False])
 @pytest.mark.parametrize('int_type', [torch.int32, torch.int64])
 def test_ragged_batch(int_type, causal, dtype) -> None:
     lengths = torch.tensor([0, 1, 130, 77, 128, 64, -3, 999], dtype=int_type)
