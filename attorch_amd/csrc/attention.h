@@ -15,6 +15,9 @@
 
 namespace at_hip {
 
+// Workgroups of four waves that a CU holds: two, but for the wide tiles of fp32.
+template <typename T, int DT> constexpr int kPerCu = sizeof(T) == 4 && DT > 2 ? 1 : 2;
+
 constexpr float kLog2E = 1.4426950408889634f;
 constexpr int kFar = 1 << 30;          // more than any distance between two tokens
 
@@ -133,7 +136,17 @@ template <typename T> struct Frag {
   static __device__ __forceinline__ type load(const char* p) { return *reinterpret_cast<const uint4*>(p); }
   static __device__ __forceinline__ type pack(const float (&f)[8]) { return pack16<T>(f); }
   static __device__ __forceinline__ void unpack(const type& x, float (&f)[8]) { unpack16<T>(x, f); }
-  static __device__ __forceinline__ f32x16 mma(const type& x, const type& y, f32x16 c) { return Mfma16<T>::run(x, y, c); }
+  // c0 += x0 y0^T and c1 += x1 y1^T
+  static __device__ __forceinline__ void mma2(const type& x0, const type& y0, f32x16& c0, const type& x1, const type& y1,
+                                              f32x16& c1) {
+    c0 = Mfma16<T>::run(x0, y0, c0);
+    c1 = Mfma16<T>::run(x1, y1, c1);
+  }
+  // c[n] += x(n) y^T
+  template <int N, typename X> static __device__ __forceinline__ void mma_all(X&& x, const type& y, f32x16 (&c)[N]) {
+#pragma unroll
+    for (int n = 0; n < N; ++n) c[n] = Mfma16<T>::run(x(n), y, c[n]);
+  }
 };
 struct Frag32 { float e[8]; };
 template <> struct Frag<float> {
@@ -150,11 +163,24 @@ template <> struct Frag<float> {
 #pragma unroll
     for (int j = 0; j < 8; ++j) f[j] = x.e[j];
   }
-  // eight steps of two elements each: element j of either half, in whatever order the fragments are
-  static __device__ __forceinline__ f32x16 mma(const type& x, const type& y, f32x16 c) {
+  // eight steps of two elements each: element j of either half, in whatever order the fragments are;
+  // two sums in turn, since one would wait for each step's result
+  static __device__ __forceinline__ void mma2(const type& x0, const type& y0, f32x16& c0, const type& x1, const type& y1,
+                                              f32x16& c1) {
 #pragma unroll
-    for (int j = 0; j < 8; ++j) c = __builtin_amdgcn_mfma_f32_32x32x2f32(x.e[j], y.e[j], c, 0, 0, 0);
-    return c;
+    for (int j = 0; j < 8; ++j) {
+      c0 = __builtin_amdgcn_mfma_f32_32x32x2f32(x0.e[j], y0.e[j], c0, 0, 0, 0);
+      c1 = __builtin_amdgcn_mfma_f32_32x32x2f32(x1.e[j], y1.e[j], c1, 0, 0, 0);
+    }
+  }
+  template <int N, typename X> static __device__ __forceinline__ void mma_all(X&& x, const type& y, f32x16 (&c)[N]) {
+    type f[N];
+#pragma unroll
+    for (int n = 0; n < N; ++n) f[n] = x(n);
+#pragma unroll
+    for (int j = 0; j < 8; ++j)
+#pragma unroll
+      for (int n = 0; n < N; ++n) c[n] = __builtin_amdgcn_mfma_f32_32x32x2f32(f[n].e[j], y.e[j], c[n], 0, 0, 0);
   }
 };
 

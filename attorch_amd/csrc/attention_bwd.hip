@@ -23,7 +23,7 @@ constexpr int kStep = 64;                // keys or rows of a tile it walks over
 
 // WK waves share 32 rows and halve each tile of keys among them (1 or 2); they join at the end.
 template <typename T, int DT, int WK>
-__global__ __launch_bounds__(kWaves * 64, sizeof(T) == 2 ? 2 : 1) void attention_dq_kernel(AttentionArgs a) {
+__global__ __launch_bounds__(kWaves * 64, (kPerCu<T, DT>)) void attention_dq_kernel(AttentionArgs a) {
   typedef Tile<T, DT> L;
   typedef typename Frag<T>::type F;
   constexpr int kRows = 32 * kWaves / WK, kMine = kStep / WK;
@@ -136,8 +136,7 @@ __global__ __launch_bounds__(kWaves * 64, sizeof(T) == 2 ? 2 : 1) void attention
       f32x16 s = zero_acc(), dp = zero_acc();
 #pragma unroll
       for (int ks = 0; ks < L::kSteps; ++ks) {
-        s = Frag<T>::mma(L::rows_frag(lr, 0, n * 32, ks), qf[ks], s);
-        dp = Frag<T>::mma(L::rows_frag(lr, kTileBytes, n * 32, ks), df[ks], dp);
+        Frag<T>::mma2(L::rows_frag(lr, 0, n * 32, ks), qf[ks], s, L::rows_frag(lr, kTileBytes, n * 32, ks), df[ks], dp);
       }
 #pragma unroll
       for (int e = 0; e < 16; ++e)
@@ -158,9 +157,7 @@ __global__ __launch_bounds__(kWaves * 64, sizeof(T) == 2 ? 2 : 1) void attention
 #pragma unroll
         for (int e = 0; e < 8; ++e) x[e] = s[t16 * 8 + e];
         const F ds = Frag<T>::pack(x);
-#pragma unroll
-        for (int dt = 0; dt < DT; ++dt)
-          dq[dt] = Frag<T>::mma(L::cols_frag(lr, 0, n * 32 + t16 * 16, dt), ds, dq[dt]);
+        Frag<T>::mma_all([&](int dt) { return L::cols_frag(lr, 0, n * 32 + t16 * 16, dt); }, ds, dq);
       }
     }
   }
@@ -232,7 +229,7 @@ __device__ __forceinline__ int wave_min(int v) {
 // see them.  Of the rows that see sinks only, the waves of a workgroup share the walk instead: those with
 // the same 32 keys take every second or fourth 32 rows (see chunk_plan for how the results are summed).
 template <typename T, int DT>
-__global__ __launch_bounds__(kWaves * 64, sizeof(T) == 2 ? 2 : 1) void attention_dkv_kernel(AttentionArgs a) {
+__global__ __launch_bounds__(kWaves * 64, (kPerCu<T, DT>)) void attention_dkv_kernel(AttentionArgs a) {
   typedef Tile<T, DT> L;
   typedef typename Frag<T>::type F;
   constexpr int kTileBytes = kStep * L::kPitch;
@@ -353,8 +350,7 @@ __global__ __launch_bounds__(kWaves * 64, sizeof(T) == 2 ? 2 : 1) void attention
       f32x16 s = zero_acc(), dp = zero_acc();
 #pragma unroll
       for (int ks = 0; ks < L::kSteps; ++ks) {
-        s = Frag<T>::mma(L::rows_frag(lr, 0, n * 32, ks), kf[ks], s);
-        dp = Frag<T>::mma(L::rows_frag(lr, kTileBytes, n * 32, ks), vf[ks], dp);
+        Frag<T>::mma2(L::rows_frag(lr, 0, n * 32, ks), kf[ks], s, L::rows_frag(lr, kTileBytes, n * 32, ks), vf[ks], dp);
       }
 #pragma unroll
       for (int q = 0; q < 4; ++q) {
@@ -391,8 +387,8 @@ __global__ __launch_bounds__(kWaves * 64, sizeof(T) == 2 ? 2 : 1) void attention
         const F pf = Frag<T>::pack(x), df = Frag<T>::pack(y);
 #pragma unroll
         for (int dt = 0; dt < DT; ++dt) {
-          dv[dt] = Frag<T>::mma(L::cols_frag(lr, kTileBytes, n * 32 + t16 * 16, dt), pf, dv[dt]);
-          dk[dt] = Frag<T>::mma(L::cols_frag(lr, 0, n * 32 + t16 * 16, dt), df, dk[dt]);
+          Frag<T>::mma2(L::cols_frag(lr, kTileBytes, n * 32 + t16 * 16, dt), pf, dv[dt],
+                        L::cols_frag(lr, 0, n * 32 + t16 * 16, dt), df, dk[dt]);
         }
       }
     }

@@ -30,7 +30,7 @@ __device__ __forceinline__ void store_output(const AttentionArgs& a, int64_t to,
 
 // WK waves share 32 rows and halve each tile of keys among them (1 or 2); they join at the end.
 template <typename T, int DT, int WK>
-__global__ __launch_bounds__(kWaves * 64, sizeof(T) == 2 ? 2 : 1) void attention_fwd_kernel(AttentionArgs a) {
+__global__ __launch_bounds__(kWaves * 64, (kPerCu<T, DT>)) void attention_fwd_kernel(AttentionArgs a) {
   typedef Tile<T, DT> L;
   typedef typename Frag<T>::type F;
   constexpr int kTileBytes = kKeys * L::kPitch;
@@ -123,8 +123,7 @@ __global__ __launch_bounds__(kWaves * 64, sizeof(T) == 2 ? 2 : 1) void attention
     for (int n = 0; n < NS; ++n) s[n] = zero_acc();
 #pragma unroll
     for (int ks = 0; ks < L::kSteps; ++ks)
-#pragma unroll
-      for (int n = 0; n < NS; ++n) s[n] = Frag<T>::mma(L::rows_frag(lr, 0, n * 32, ks), qf[ks], s[n]);
+      Frag<T>::mma_all([&](int n) { return L::rows_frag(lr, 0, n * 32, ks); }, qf[ks], s);
     // places of the lane relative to its first one are constants: 8 apart, 4 in a row
     const bool whole = !mixed && k0 >= last - a.left && k0 + kMine - 1 <= min(first + a.right, seq.len - 1);
     if (!whole) {
@@ -171,9 +170,7 @@ __global__ __launch_bounds__(kWaves * 64, sizeof(T) == 2 ? 2 : 1) void attention
 #pragma unroll
       for (int e = 0; e < 8; ++e) pr[e] = s[ks >> 1][(ks & 1) * 8 + e];
       const F pf = Frag<T>::pack(pr);
-#pragma unroll
-      for (int dt = 0; dt < DT; ++dt)
-        o[dt] = Frag<T>::mma(L::cols_frag(lr, kTileBytes, ks * 16, dt), pf, o[dt]);
+      Frag<T>::mma_all([&](int dt) { return L::cols_frag(lr, kTileBytes, ks * 16, dt); }, pf, o);
     }
   }
 
