@@ -511,8 +511,8 @@ void chunk_plan(AttentionArgs& a) {
   const int64_t want = 2 * device_cu_count();
   int64_t steps = cdiv64(span, kStep) + 1;                     // the first step need not start at the first row
   a.chunks = 1;
-  if (a.tiles * heads < want && steps > 2) {
-    int64_t n = cdiv64(want, a.tiles * heads);
+  if (a.tiles * heads > 0 && a.tiles * heads < want && steps > 2) {
+    int64_t n = (want + a.tiles * heads / 2) / (a.tiles * heads);
     if (n > steps / 2) n = steps / 2;
     a.chunks = (int)n;
     steps = cdiv64(steps, n);

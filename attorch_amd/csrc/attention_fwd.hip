@@ -316,7 +316,7 @@ void plan(AttentionArgs& a) {
   // keys that one tile of rows can see
   const int64_t span = (int64_t)a.left + a.right + cdiv64(tile_rows, a.group) + a.sinks;
   const int64_t tiles = cdiv64(span < a.keys ? span : a.keys, kKeys);
-  int64_t n = cdiv64(want, groups);
+  int64_t n = want / groups;           // rounded up, a few workgroups would run after all the others
   if (n > tiles / 4) n = tiles / 4;
   a.splits = (int)(n < 1 ? 1 : n > kMaxSplits ? kMaxSplits : n);
 }
