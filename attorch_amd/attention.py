@@ -96,7 +96,7 @@ def _check(query: Layout, key: Layout, value: Layout, lengths: Optional[Layout],
         raise RuntimeError(f'The window must hold at least one token, received {window}')
     if num_sinks < 0:
         raise RuntimeError(f'The number of sinks must not be negative, received {num_sinks}')
-    if scale is not None and not 0.0 < scale < 3e38:
+    if scale is not None and not 0.0 < scale < 1e38:
         raise RuntimeError(f'The scale must be positive and finite, received {scale}')
     for name, counts in (('lengths', lengths), ('query_lengths', query_lengths)):
         if counts is None:

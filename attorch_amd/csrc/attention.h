@@ -373,7 +373,7 @@ inline int attention_args(const at_attention_t* s, AttentionArgs& a) {
       s->heads % s->kv_heads != 0 || s->rows < 0 || s->keys < s->rows || s->keys > limit || s->dim <= 0 || s->dim > 128 ||
       s->window < 0 || s->sinks < 0)
     return AT_ERR_DIM;
-  if (!(s->scale > 0.f) || s->scale > 3e38f) return AT_ERR_DIM;
+  if (!(s->scale > 0.f) || s->scale > 1e38f) return AT_ERR_DIM;
   if (s->dim % 8 != 0) return AT_ERR_ALIGN;
   a = AttentionArgs{};
   a.batch = (int)s->batch;

@@ -13,7 +13,7 @@ pre_act_add of BatchNorm2d) are spelled out as separate torch layers for the lat
 `load_from` copies the parameters of one variant into the other so the two can be compared.
 """
 
-from typing import Optional
+from typing import List, Optional, Tuple
 
 import torch
 from torch import Tensor
@@ -124,27 +124,84 @@ class BasicBlock(nn.Module):
 
 
 class TransformerBlock(nn.Module):
-    """Pre-norm block: x + attention(LN(x)), then + MLP(LN(.)) with a fused Linear+GELU."""
-    def __init__(self, backend, dim: int, num_heads: int) -> None:
+    """
+    Pre-norm block: x + attention(LN(x)), then + MLP(LN(.)) with a fused Linear+GELU.
+
+    The attention core is torch's on both backends unless one of the options is given: rotary turns
+    queries and keys by the tokens' positions, window and num_sinks limit what a token sees to the
+    window's last tokens and the sequence's first ones, and kv_heads < num_heads shares key heads
+    among query heads.  With any of them the fused backend runs on its Rotary and WindowAttention,
+    and torch on the same arithmetic spelled out; only the former can continue sequences from a
+    cache of keys and values.
+    """
+    def __init__(self, backend, dim: int, num_heads: int, kv_heads: Optional[int] = None, window: Optional[int] = None,
+                 num_sinks: int = 0, rotary: bool = False) -> None:
         super().__init__()
         self.num_heads = num_heads
+        self.kv_heads = num_heads if kv_heads is None else kv_heads
+        self.head_dim = dim // num_heads
+        self.window, self.num_sinks, self.rotary = window, num_sinks, rotary
+        self.plain = window is None and not rotary and self.kv_heads == num_heads
+        self.fused = _is_fused(backend) and not self.plain
+        if self.fused:
+            self.turn = backend.Rotary(self.head_dim) if rotary else None
+            self.core = backend.WindowAttention(window=window, num_sinks=num_sinks)
         self.ln1 = backend.LayerNorm(dim)
-        self.qkv = FusedLinear(backend, dim, 3 * dim, None)
+        self.qkv = FusedLinear(backend, dim, dim + 2 * self.kv_heads * self.head_dim, None)
         self.proj = FusedLinear(backend, dim, dim, None)
         self.ln2 = backend.LayerNorm(dim)
         self.fc1 = FusedLinear(backend, dim, 4 * dim, 'gelu')
         self.fc2 = FusedLinear(backend, 4 * dim, dim, None)
 
-    def attention(self, input: Tensor) -> Tensor:
+    def _spelled_out(self, q: Tensor, k: Tensor, v: Tensor) -> Tensor:
+        position = torch.arange(q.shape[2], device=q.device)
+        if self.rotary:
+            half = self.head_dim // 2
+            angle = position[:, None] * 10000.0 ** (torch.arange(half, device=q.device, dtype=torch.float64) / -half)
+            cos, sin = angle.cos().float(), angle.sin().float()
+
+            def turned(x: Tensor) -> Tensor:
+                a, b = x.float().chunk(2, -1)
+                return torch.cat((a * cos - b * sin, a * sin + b * cos), -1).to(x.dtype)
+
+            q, k = turned(q), turned(k)
+        ahead = position - position[:, None]
+        seen = ahead <= 0
+        if self.window is not None:
+            seen = seen & ((ahead > -self.window) | (position < self.num_sinks))
+        group = self.num_heads // self.kv_heads
+        return F.scaled_dot_product_attention(q, k.repeat_interleave(group, 1), v.repeat_interleave(group, 1),
+                                              attn_mask=seen)
+
+    def attention(self, input: Tensor, cache: Optional[Tuple[Tensor, Tensor]] = None,
+                  lengths: Optional[Tensor] = None) -> Tensor:
         batch, seq, dim = input.shape
-        qkv = self.qkv(input).view(batch, seq, 3, self.num_heads, dim // self.num_heads)
-        q, k, v = qkv.permute(2, 0, 3, 1, 4)
-        # the attention core is not on the layer-kernel path: torch's on both backends
-        out = F.scaled_dot_product_attention(q, k, v, is_causal=True)
+        if self.plain and cache is None:
+            qkv = self.qkv(input).view(batch, seq, 3, self.num_heads, dim // self.num_heads)
+            q, k, v = qkv.permute(2, 0, 3, 1, 4)
+            out = F.scaled_dot_product_attention(q, k, v, is_causal=True)
+            return self.proj(out.transpose(1, 2).reshape(batch, seq, dim))
+        heads = self.qkv(input).view(batch, seq, self.num_heads + 2 * self.kv_heads, self.head_dim).transpose(1, 2)
+        q, k, v = heads.split((self.num_heads, self.kv_heads, self.kv_heads), 1)
+        if not self.fused:
+            out = self._spelled_out(q, k, v)
+        else:
+            positions = None
+            if cache is not None:          # the new tokens are the last of each sequence
+                positions = (lengths - seq)[:, None] + torch.arange(seq, device=input.device)
+            if self.turn is not None:
+                q, k = self.turn(q, k, positions)
+            if cache is not None:
+                rows = torch.arange(batch, device=input.device)[:, None]
+                for stored, new in zip(cache, (k, v)):
+                    stored[rows, :, positions] = new.transpose(1, 2)
+                k, v = cache
+            out = self.core(q, k, v, lengths)
         return self.proj(out.transpose(1, 2).reshape(batch, seq, dim))
 
-    def forward(self, input: Tensor) -> Tensor:
-        output = input + self.attention(self.ln1(input))
+    def forward(self, input: Tensor, cache: Optional[Tuple[Tensor, Tensor]] = None,
+                lengths: Optional[Tensor] = None) -> Tensor:
+        output = input + self.attention(self.ln1(input), cache, lengths)
         return output + self.fc2(self.fc1(self.ln2(output)))
 
     def load_from(self, other: 'TransformerBlock') -> None:
@@ -157,20 +214,25 @@ class TransformerBlock(nn.Module):
 
 
 class TinyGPT(nn.Module):
-    """Embeddings, transformer blocks, final LayerNorm, vocabulary head, next-token loss."""
+    """
+    Embeddings, transformer blocks, final LayerNorm, vocabulary head, next-token loss.  Further
+    arguments go to the blocks; with rotary there are no position embeddings.
+    """
     def __init__(self, backend, vocab_size: int, depth: int, dim: int, num_heads: int,
-                 max_seq_len: int = 512) -> None:
+                 max_seq_len: int = 512, rotary: bool = False, **block_options) -> None:
         super().__init__()
         self.tok_embed = nn.Embedding(vocab_size, dim)
-        self.pos_embed = nn.Embedding(max_seq_len, dim)
-        self.blocks = nn.ModuleList(TransformerBlock(backend, dim, num_heads) for _ in range(depth))
+        self.pos_embed = None if rotary else nn.Embedding(max_seq_len, dim)
+        self.blocks = nn.ModuleList(TransformerBlock(backend, dim, num_heads, rotary=rotary, **block_options)
+                                    for _ in range(depth))
         self.norm = backend.LayerNorm(dim)
         self.head = FusedLinear(backend, dim, vocab_size, None)
         self.loss_func = backend.CrossEntropyLoss()
 
     def forward(self, tokens: Tensor, return_loss: bool = False) -> Tensor:
-        positions = torch.arange(tokens.shape[1], device=tokens.device)
-        output = self.tok_embed(tokens) + self.pos_embed(positions)
+        output = self.tok_embed(tokens)
+        if self.pos_embed is not None:
+            output = output + self.pos_embed(torch.arange(tokens.shape[1], device=tokens.device))
         for block in self.blocks:
             output = block(output)
         logits = self.head(self.norm(output))
@@ -178,10 +240,30 @@ class TinyGPT(nn.Module):
             return logits
         return self.loss_func(logits[:, :-1].reshape(-1, logits.shape[-1]), tokens[:, 1:].reshape(-1))
 
+    def new_cache(self, batch: int, max_tokens: int) -> List[Tuple[Tensor, Tensor]]:
+        """
+        Room for the keys and values of max_tokens tokens of each sequence, for every block.
+        """
+        weight = self.tok_embed.weight
+        return [tuple(torch.empty(batch, block.kv_heads, max_tokens, block.head_dim, device=weight.device, dtype=weight.dtype)
+                      for _ in range(2)) for block in self.blocks]
+
+    def extend(self, tokens: Tensor, cache: List[Tuple[Tensor, Tensor]], lengths: Tensor) -> Tensor:
+        """
+        Logits of new tokens (a prompt, a part of one or single tokens), which are the last ones of
+        sequences that have `lengths` tokens with them; their keys and values go into the cache.
+        For the fused backend with rotary.
+        """
+        output = self.tok_embed(tokens)
+        for block, stored in zip(self.blocks, cache):
+            output = block(output, stored, lengths)
+        return self.head(self.norm(output))
+
     def load_from(self, other: 'TinyGPT') -> None:
         with torch.no_grad():
             self.tok_embed.weight.copy_(other.tok_embed.weight)
-            self.pos_embed.weight.copy_(other.pos_embed.weight)
+            if self.pos_embed is not None:
+                self.pos_embed.weight.copy_(other.pos_embed.weight)
             self.norm.weight.copy_(other.norm.weight)
             self.norm.bias.copy_(other.norm.bias)
         for mine, theirs in zip(self.blocks, other.blocks):

@@ -100,6 +100,9 @@ def main() -> int:
     tok = torch.randint(0, 8192, (8, 512), generator=gen).cuda()
     cases.append(('GPT block x2, dim 1024, 16 heads, vocab 8192, tokens [8,512]',
                   make(TinyGPT, 8192, 2, 1024, 16), lambda m: m(tok, return_loss=True)))
+    cases.append(('GPT block x2 with rotary positions, 4 key heads, window 128 and 4 sinks, dim 1024, 16 heads, vocab 8192, '
+                  'tokens [8,512]', make(TinyGPT, 8192, 2, 1024, 16, rotary=True, kv_heads=4, window=128, num_sinks=4),
+                  lambda m: m(tok, return_loss=True)))
 
     for name, models, run in cases:
         for backend, model in models.items():
