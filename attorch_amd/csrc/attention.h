@@ -37,7 +37,7 @@ struct AttentionArgs {
   const void* query_lengths;           // live rows of each sequence, or null: `rows` of all
   int lengths64, causal;
   int batch, kv_heads, group, rows, keys, dim;
-  int row_pitch, tiles, splits, waves_per_row;
+  int row_pitch, tiles, splits, waves_per_row, slots;
   int sink_tiles, far_chunks, far_steps, chunks, chunk_steps;   // dk and dv: see chunk_plan
   int left, right, sinks;
   float scale, scale_log2;
@@ -362,6 +362,15 @@ __device__ __forceinline__ i32x4 open_rsrc(const char* base) {
 // ---- host side ----------------------------------------------------------------------------
 constexpr int kRowAlign = 64;          // rows of lse and delta are padded to whole tiles
 
+inline int workgroups_per_cu(int dtype, int dim) { return dtype == AT_DTYPE_F32 && dim > 64 ? 1 : 2; }
+
+// Waves that share 32 rows and halve each tile of keys (kernels that own rows): two where workgroups of
+// whole rows leave some of the GPU's `slots` for workgroups empty.  Sharing reads keys and values twice as
+// often, empty slots cost more (a chunk of 1024 over 16384 keys, bf16: 256 workgroups on 512 slots 107 us,
+// split and joined 92 us, shared 93 us without the join's workspace; fp32 patches: dq 88 -> 52 us; fp32,
+// causal, 4486 tokens, 282 workgroups: dq 98 -> 57 us; with all slots taken, a block of 512 tokens: 27 -> 30 us).
+inline int waves_per_row(int64_t rows, int64_t heads, int64_t slots) { return cdiv64(rows, 128) * heads < slots ? 2 : 1; }
+
 inline bool grid_fits(int64_t workgroups) { return workgroups < ((int64_t)1 << 24); }   // 256 threads each, 32-bit grid
 
 // Checks the shape and fills the arguments that do not depend on the pointers.
@@ -389,6 +398,7 @@ inline int attention_args(const at_attention_t* s, AttentionArgs& a) {
   a.right = s->causal ? 0 : (int)reach;
   a.sinks = (int)(s->sinks < s->keys ? s->sinks : s->keys);
   a.causal = s->causal != 0;
+  a.slots = workgroups_per_cu(s->dtype, a.dim) * device_cu_count();
   a.scale = s->scale;
   a.scale_log2 = s->scale * kLog2E;
   a.lengths64 = s->lengths_int64;

@@ -217,6 +217,27 @@ __host__ __device__ inline int sink_sharers(const AttentionArgs& a, int tile) {
   return sinks <= 32 ? 4 : sinks <= 64 ? 2 : 1;
 }
 
+// Steps of rows [begin, end) that see some key of a tile.
+struct Steps {
+  int begin, end;
+};
+__device__ __forceinline__ Steps steps_of(const AttentionArgs& a, const Sequence& s, int tile) {
+  const int first = tile * kTileKeys, last = min(first + kTileKeys, s.len) - 1;
+  const bool sinks = first < a.sinks;
+  const int lo = !a.causal && sinks ? s.start : max(first - a.right, s.start);
+  const int hi = sinks ? s.len - 1 : min(last + a.left, s.len - 1);
+  if (first > last || lo > hi) return {0, 0};
+  const int rows = min((hi - s.start + 1) * a.group, s.live * a.group);
+  return {(lo - s.start) * a.group / kStep, (rows + kStep - 1) / kStep};
+}
+
+// The part of a tile's steps that a piece walks over.
+__device__ __forceinline__ Steps steps_of(const AttentionArgs& a, const Steps& tile, int chunk, bool far) {
+  const int length = far ? a.far_steps : a.chunk_steps;
+  const int begin = tile.begin + (far ? a.chunks * a.chunk_steps : 0) + chunk * length;
+  return {begin, min(tile.end, begin + length)};
+}
+
 // Keys of a tile that far pieces have sums of.
 __host__ __device__ inline int far_keys(const AttentionArgs& a, int tile) { return kTileKeys / sink_sharers(a, tile); }
 
@@ -245,6 +266,9 @@ __global__ __launch_bounds__(kWaves * 64, (kPerCu<T, DT>)) void attention_dkv_ke
   const int b = bh / a.kv_heads, h = bh - b * a.kv_heads;
   const Sequence seq = sequence_of(a, b);
   const int live_rows = seq.live * a.group;
+  const Steps steps = steps_of(a, steps_of(a, seq, piece.tile), piece.chunk, piece.far);
+  const int begin = __builtin_amdgcn_readfirstlane(steps.begin), end = __builtin_amdgcn_readfirstlane(steps.end);
+  if (begin >= end && (piece.far || a.chunks > 1)) return;    // no partial sum: the kernel that adds them knows
   // far from the tile's own tokens only its sinks are seen
   const int sharers = piece.far ? sink_sharers(a, piece.tile) : 1;
   const int subtile = wave % (kWaves / sharers), share = wave / (kWaves / sharers);
@@ -277,24 +301,6 @@ __global__ __launch_bounds__(kWaves * 64, (kPerCu<T, DT>)) void attention_dkv_ke
   f32x16 dk[DT], dv[DT];
 #pragma unroll
   for (int dt = 0; dt < DT; ++dt) dk[dt] = dv[dt] = zero_acc();
-
-  __shared__ int ranges[2 * kWaves];
-  if (lane == 0) {
-    ranges[wave] = any_lo;
-    ranges[kWaves + wave] = any_hi;
-  }
-  __syncthreads();
-  int begin = ranges[0], end = ranges[kWaves];
-#pragma unroll
-  for (int w = 1; w < kWaves; ++w) {
-    begin = min(begin, ranges[w]);
-    end = max(end, ranges[kWaves + w]);
-  }
-  const int steps = piece.far ? a.far_steps : a.chunk_steps;
-  begin = begin / kStep + (piece.far ? a.chunks * a.chunk_steps : 0) + piece.chunk * steps;
-  end = min(end < 0 ? 0 : end / kStep + 1, begin + steps);
-  begin = __builtin_amdgcn_readfirstlane(begin);
-  end = __builtin_amdgcn_readfirstlane(end);
 
   const char* qb = a.q.p + b * a.q.batch + (int64_t)h * a.group * a.q.head;
   const char* db = a.dout.p + b * a.dout.batch + (int64_t)h * a.group * a.dout.head;
@@ -457,17 +463,25 @@ __global__ __launch_bounds__(256) void attention_dkv_join_kernel(AttentionArgs a
   const int bh = (int)(at / (tiles * kTileKeys)), rest = (int)(at - bh * tiles * kTileKeys);
   const int tile = rest / kTileKeys, local = rest % kTileKeys;
   const int key = tile * kTileKeys + local, group = GROUPS == 1 ? 0 : threadIdx.x >> 5, d = (threadIdx.x & 31) * 4;
-  const bool far = tile < a.sink_tiles && local < far_keys(a, tile);
-  if (key >= a.keys || (a.chunks == 1 && !far)) return;       // written by the only piece that has it
+  const bool sinks = tile < a.sink_tiles && local < far_keys(a, tile);
+  if (key >= a.keys || (a.chunks == 1 && !sinks)) return;     // written by the only piece that has it
+  const int b = bh / a.kv_heads, h = bh - b * a.kv_heads;
+  // the sums that were written: pieces without rows wrote none
+  const Steps steps = steps_of(a, sequence_of(a, b), tile);
+  const int count = max(steps.end - steps.begin, 0);
+  const int near = a.chunks == 1 ? 1 : min(a.chunks, (count + a.chunk_steps - 1) / a.chunk_steps);
+  const int beyond = count - a.chunks * a.chunk_steps;
+  const int far = sinks && beyond > 0 ? min(a.far_chunks, (beyond + a.far_steps - 1) / a.far_steps) : 0;
   const int64_t next = 2LL * kTileKeys * a.dim;
   const float* part = a.part + (bh * first_part(a, a.tiles) + first_part(a, tile)) * next + (int64_t)local * a.dim + d;
   float x[4] = {0.f, 0.f, 0.f, 0.f}, y[4] = {0.f, 0.f, 0.f, 0.f};
   if (d < a.dim) {
 #pragma unroll 4
-    for (int n = group; n < a.chunks + (far ? a.far_chunks : 0); n += GROUPS) {
+    for (int n = group; n < near + far; n += GROUPS) {
+      const float* p = part + (n < near ? n : a.chunks + n - near) * next;
       float u[4], w[4];
-      load_f32<float, 4>(part + n * next, u);
-      load_f32<float, 4>(part + n * next + (int64_t)kTileKeys * a.dim, w);
+      load_f32<float, 4>(p, u);
+      load_f32<float, 4>(p + (int64_t)kTileKeys * a.dim, w);
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
         x[j] += u[j];
@@ -475,7 +489,6 @@ __global__ __launch_bounds__(256) void attention_dkv_join_kernel(AttentionArgs a
       }
     }
   }
-  const int b = bh / a.kv_heads, h = bh - b * a.kv_heads;
   T* const to_k = reinterpret_cast<T*>(a.dk.p + b * a.dk.batch + h * a.dk.head + key * a.dk.token) + d;
   T* const to_v = reinterpret_cast<T*>(a.dv.p + b * a.dv.batch + h * a.dv.head + key * a.dv.token) + d;
   if constexpr (GROUPS == 1) {
@@ -508,11 +521,13 @@ void chunk_plan(AttentionArgs& a) {
   const int64_t heads = (int64_t)a.batch * a.kv_heads, rows = (int64_t)a.rows * a.group;
   const int64_t near = (int64_t)(a.left + a.right + kTileKeys) * a.group;
   const int64_t span = near < rows ? near : rows;              // rows that see a tile without sinks
-  const int64_t want = 2 * device_cu_count();
+  const int64_t want = a.slots;
   int64_t steps = cdiv64(span, kStep) + 1;                     // the first step need not start at the first row
   a.chunks = 1;
   if (a.tiles * heads > 0 && a.tiles * heads < want && steps > 2) {
-    int64_t n = (want + a.tiles * heads / 2) / (a.tiles * heads);
+    // on average, half of the chunks of a causal sequence without a window have no rows
+    const int64_t groups = a.causal && span == rows ? cdiv64(a.tiles * heads, 2) : a.tiles * heads;
+    int64_t n = (want + groups / 2) / groups;
     if (n > steps / 2) n = steps / 2;
     a.chunks = (int)n;
     steps = cdiv64(steps, n);
@@ -541,10 +556,9 @@ int launch(AttentionArgs a, hipStream_t stream) {
   chunk_plan(a);
   const int64_t pieces = key_pieces(a) * heads;
   const int64_t joined = (int64_t)(a.chunks > 1 ? a.tiles : a.sink_tiles) * kTileKeys * heads;
-  // tiles of 128 rows, or of 64 where these give no more than two workgroups per CU: see the forward pass
   const int64_t rows = (int64_t)a.rows * a.group;
-  const bool share = cdiv64(rows, 32 * kWaves) * heads < 2 * device_cu_count();
-  const int64_t row_tiles = cdiv64(rows, 32 * kWaves / (share ? 2 : 1));
+  const bool share = waves_per_row(rows, heads, a.slots) == 2;
+  const int64_t row_tiles = cdiv64(rows, share ? 64 : 128);
   if (!grid_fits(row_tiles * heads) || !grid_fits(pieces) || !grid_fits(joined)) return AT_ERR_DIM;
   int rc = AT_OK;
   if (a.rows > 0) {

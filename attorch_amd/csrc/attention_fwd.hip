@@ -299,15 +299,13 @@ __global__ __launch_bounds__(256) void attention_join_kernel(AttentionArgs a) {
     for (int r = all_rows + (threadIdx.x & 31); r < a.row_pitch; r += 32) lse[r] = INFINITY;
 }
 
-// How the work is cut.  Tiles of 128 rows leave a wave 32 rows and all keys of a tile; where they give no
-// more than two workgroups per CU, tiles of 64 rows whose waves share rows in pairs give twice as many
-// waves the same work; and where these still do not give every CU two workgroups, the keys are split among
-// several with at least four tiles of keys each, which another launch of 4 us joins (a tile takes a
-// workgroup about 1).
+// How the work is cut: into tiles of 128 rows, or of 64 whose waves share rows in pairs (waves_per_row), and
+// where these do not fill the GPU, the keys are split among several workgroups with at least four tiles of
+// keys each, which another launch of 4 us joins (a tile takes a workgroup about 1).
 void plan(AttentionArgs& a) {
   const int64_t heads = (int64_t)a.batch * a.kv_heads, rows = (int64_t)a.rows * a.group;
-  const int64_t want = 2 * device_cu_count();
-  a.waves_per_row = cdiv64(rows, 32 * kWaves) * heads < want ? 2 : 1;
+  const int64_t want = a.slots;
+  a.waves_per_row = waves_per_row(rows, heads, a.slots);
   const int64_t tile_rows = 32 * kWaves / a.waves_per_row;
   a.tiles = (int)cdiv64(rows, tile_rows);
   a.splits = 1;

@@ -174,18 +174,22 @@ __global__ __launch_bounds__(256) void rotary_kernel(RotaryArgs a) {
   }
 }
 
-template <typename T>
-int launch(const RotaryArgs& a, bool adjacent, bool vector, hipStream_t stream) {
-  constexpr int VEC = 16 / (int)sizeof(T);
+template <typename T, int VEC>
+int launch(const RotaryArgs& a, bool adjacent, hipStream_t stream) {
   const dim3 grid((unsigned)cdiv64(a.tokens, a.group)), block(256);
-  if (adjacent) {
-    if (vector) hipLaunchKernelGGL((rotary_kernel<T, true, VEC>), grid, block, 0, stream, a);
-    else hipLaunchKernelGGL((rotary_kernel<T, true, 1>), grid, block, 0, stream, a);
-  } else {
-    if (vector) hipLaunchKernelGGL((rotary_kernel<T, false, VEC>), grid, block, 0, stream, a);
-    else hipLaunchKernelGGL((rotary_kernel<T, false, 1>), grid, block, 0, stream, a);
-  }
+  if (adjacent) hipLaunchKernelGGL((rotary_kernel<T, true, VEC>), grid, block, 0, stream, a);
+  else hipLaunchKernelGGL((rotary_kernel<T, false, VEC>), grid, block, 0, stream, a);
   return launch_status();
+}
+
+template <typename T>
+int launch_width(const RotaryArgs& a, bool adjacent, int width, hipStream_t stream) {
+  if constexpr (sizeof(T) == 2) {
+    if (width == 8) return launch<T, 8>(a, adjacent, stream);
+  }
+  if (width >= 4) return launch<T, 4>(a, adjacent, stream);
+  if (width >= 2) return launch<T, 2>(a, adjacent, stream);
+  return launch<T, 1>(a, adjacent, stream);
 }
 
 }  // namespace
@@ -214,18 +218,21 @@ int at_rotary(const at_rotary_t* s, const void* q, const void* k, void* q_out, v
   RotaryArgs a = {};
   a.in[0] = (const char*)q; a.in[1] = (const char*)k;
   a.out[0] = (char*)q_out; a.out[1] = (char*)k_out;
-  bool vector = s->dim * size % 16 == 0;
+  // features of an access: the largest power of two that the pairs (both halves of them, or adjacent
+  // ones), the head, the strides and the addresses are multiples of, up to 16 bytes
+  int64_t common = (s->adjacent ? 2 * s->pairs : s->pairs) | s->dim | 16 / size;
+  int64_t bytes = 16;
   for (int n = 0; n < 2; ++n) {
     if ((n == 0 ? s->q_heads : s->k_heads) == 0) continue;
-    vector = vector && aligned16(a.in[n]) && aligned16(a.out[n]);
+    bytes |= (int64_t)(uintptr_t)a.in[n] | (int64_t)(uintptr_t)a.out[n];
     for (int j = 0; j < 3; ++j) {
       a.in_stride[n][j] = s->strides[n][j] * size;
       a.out_stride[n][j] = s->strides[2 + n][j] * size;
-      vector = vector && a.in_stride[n][j] % 16 == 0 && a.out_stride[n][j] % 16 == 0;
+      bytes |= a.in_stride[n][j] | a.out_stride[n][j];
     }
   }
-  // whole vectors of pairs, and of features in adjacent pairs
-  vector = vector && (s->adjacent ? 2 : 1) * s->pairs * size % 16 == 0;
+  common |= (bytes & -bytes) / size;
+  const int width = (int)(common & -common);
   a.positions = positions;
   a.inv_freq = inv_freq;
   a.pair_axis = pair_axis;
@@ -245,9 +252,9 @@ int at_rotary(const at_rotary_t* s, const void* q, const void* k, void* q_out, v
   while (group > 1 && a.tokens / group < 4 * (int64_t)device_cu_count()) group /= 2;
   a.group = group < 1 ? 1 : group;
   if (cdiv64(a.tokens, a.group) >= ((int64_t)1 << 24)) return AT_ERR_DIM;
-  if (s->dtype == AT_DTYPE_F32) return launch<float>(a, s->adjacent != 0, vector, (hipStream_t)stream);
-  if (s->dtype == AT_DTYPE_F16) return launch<f16_t>(a, s->adjacent != 0, vector, (hipStream_t)stream);
-  return launch<bf16_t>(a, s->adjacent != 0, vector, (hipStream_t)stream);
+  if (s->dtype == AT_DTYPE_F32) return launch_width<float>(a, s->adjacent != 0, width, (hipStream_t)stream);
+  if (s->dtype == AT_DTYPE_F16) return launch_width<f16_t>(a, s->adjacent != 0, width, (hipStream_t)stream);
+  return launch_width<bf16_t>(a, s->adjacent != 0, width, (hipStream_t)stream);
 }
 
 }  // extern "C"
