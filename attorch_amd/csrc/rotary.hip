@@ -5,8 +5,19 @@
 // Bound by memory: every feature is read and written once.  A workgroup takes a few tokens, forms the
 // cosines and sines of their angles and the tokens' addresses once in LDS (all heads of a token share
 // them) and then streams the heads of q and k.  A lane keeps its place in a head and goes from head to
-// head, two at a time, so that it has four vectors in flight.  The angles are formed in 64 bits and
-// reduced by whole turns there: at position 2^20 an fp32 product would already be off by 0.06 radians.
+// head, two at a time, so that it has four vectors in flight; lanes that only copy run along with those
+// that turn, and select instead of branching (a branch holds the loads of the tables back until those
+// of the features are there: 51 instead of 31 us for 8 x 4096 tokens of 24 heads of 64 features).  The
+// angles are formed in 64 bits and reduced by whole turns there: at position 2^20 an fp32 product would
+// already be off by 0.06 radians.  Results are rounded once, to the type of the inputs.
+//
+// 8 x 4096 tokens, 24 heads of 128 features, bf16: 75 us (5.4 TB/s); fp32 147 us (5.5 TB/s); a quarter of
+// the features turned 79 us; 5 or 37 pairs of 80 features, whose halves start anywhere, 40 us (6.3 TB/s, in
+// part from the last level cache).  One token of 128 sequences: 8 us, the latency of the launch, of the
+// angles' and then of the features' loads.
+#include <algorithm>
+#include <type_traits>
+
 #include "at_common.h"
 
 namespace at_hip {
@@ -15,6 +26,8 @@ namespace {
 constexpr int kMaxPairs = 512;
 constexpr int kTable = 1024;           // cosines and sines in LDS
 constexpr int kMaxTokens = 8;          // of a workgroup
+
+template <int W> using Width = std::integral_constant<int, W>;
 
 struct RotaryArgs {
   const char* in[2];                   // q, k
@@ -26,6 +39,7 @@ struct RotaryArgs {
   int64_t position_strides[3];
   int64_t tokens;                      // batch * rows
   int rows, heads, q_heads, dim, pairs, axes, position_type, inverse, group;
+  int turn_span, turn_width, copy_span, copy_width;   // see cut()
 };
 
 __device__ __forceinline__ double position_of(const RotaryArgs& a, int axis, int64_t b, int t) {
@@ -36,59 +50,41 @@ __device__ __forceinline__ double position_of(const RotaryArgs& a, int axis, int
   return (double)reinterpret_cast<const float*>(a.positions)[at];
 }
 
-// What a lane turns or copies at a time: VEC features (1: any size and alignment) of either half of the
-// pairs, or of adjacent pairs, or of the rest.
-template <typename T, bool ADJACENT, int VEC> struct Item {
-  static constexpr int kWidth = VEC > 1 || !ADJACENT ? VEC : 2;    // features an adjacent item covers
-  static constexpr bool kTwo = !ADJACENT;                          // two places in a head
-  float u[kWidth], w[kTwo ? VEC : 1];
+// What a lane takes of a head at a time: W features in two places, either half of pairs or features that
+// are only copied; with adjacent pairs in one place.  Lanes that turn and lanes that copy go together.
+// Accesses assume no more than an element's alignment: the hardware takes a vector from any address at
+// full speed, so odd sizes and strides do not make accesses narrow.
+template <typename T, bool ADJACENT, int W> struct Item {
+  T u[W], w[ADJACENT ? 1 : W];
 
-  static __device__ __forceinline__ void read(const T* p, float (&v)[kWidth]) {
-    if constexpr (VEC > 1 || kWidth == 1) {
-      load_f32<T, kWidth>(p, v);
-    } else {
-      v[0] = to_f32(p[0]);
-      v[1] = to_f32(p[1]);
-    }
+  __device__ __forceinline__ void load(const T* head, int d0, int d1) {
+    __builtin_memcpy(u, head + d0, W * sizeof(T));
+    if constexpr (!ADJACENT) __builtin_memcpy(w, head + d1, W * sizeof(T));
   }
-  static __device__ __forceinline__ void write(T* p, const float (&v)[kWidth]) {
-    if constexpr (VEC > 1 || kWidth == 1) {
-      store_f32<T, kWidth>(p, v);
-    } else {
-      p[0] = from_f32<T>(v[0]);
-      p[1] = from_f32<T>(v[1]);
-    }
+  static __device__ __forceinline__ void turn(T& p, T& q, float c, float s, bool turns) {
+    const float x = to_f32(p), y = to_f32(q);
+    p = turns ? from_f32<T>(__builtin_fmaf(-y, s, x * c)) : p;     // one order of roundings in all lanes
+    q = turns ? from_f32<T>(__builtin_fmaf(y, c, x * s)) : q;
   }
-  __device__ __forceinline__ void load(const T* head, int d, int pairs) {
-    read(head + d, u);
-    if constexpr (kTwo) load_f32<T, VEC>(head + d + pairs, w);
-  }
-  __device__ __forceinline__ void turn(const float* cs, const float* sn, int d) {
-    if constexpr (kTwo) {
+  __device__ __forceinline__ void turn(const float* cs, const float* sn, bool turns) {
+    if constexpr (!ADJACENT) {
 #pragma unroll
-      for (int j = 0; j < VEC; ++j) {
-        const float c = cs[d + j], s = sn[d + j], x = u[j], y = w[j];
-        u[j] = x * c - y * s;
-        w[j] = x * s + y * c;
-      }
-    } else {
+      for (int j = 0; j < W; ++j) turn(u[j], w[j], cs[j], sn[j], turns);
+    } else if constexpr (W > 1) {          // single features are only copied
 #pragma unroll
-      for (int j = 0; j < kWidth; j += 2) {
-        const float c = cs[(d + j) >> 1], s = sn[(d + j) >> 1], x = u[j], y = u[j + 1];
-        u[j] = x * c - y * s;
-        u[j + 1] = x * s + y * c;
-      }
+      for (int j = 0; j < W; j += 2) turn(u[j], u[j + 1], cs[j >> 1], sn[j >> 1], turns);
     }
   }
-  __device__ __forceinline__ void store(T* head, int d, int pairs) const {
-    write(head + d, u);
-    if constexpr (kTwo) store_f32<T, VEC>(head + d + pairs, w);
+  __device__ __forceinline__ void store(T* head, int d0, int d1) const {
+    __builtin_memcpy(head + d0, u, W * sizeof(T));
+    if constexpr (!ADJACENT) __builtin_memcpy(head + d1, w, W * sizeof(T));
   }
 };
 
-template <typename T, bool ADJACENT, int VEC>
-__global__ __launch_bounds__(256) void rotary_kernel(RotaryArgs a) {
-  typedef Item<T, ADJACENT, VEC> I;
+__host__ __device__ __forceinline__ int items(int span, int width) { return (span + width - 1) / width; }
+
+template <typename T, bool ADJACENT>
+__global__ __launch_bounds__(256, 6) void rotary_kernel(RotaryArgs a) {
   __shared__ float table_cos[kTable], table_sin[kTable];
   __shared__ int64_t base[kMaxTokens][4];      // token's offsets in q, k, q_out, k_out
   const int64_t first = (int64_t)blockIdx.x * a.group;
@@ -115,9 +111,7 @@ __global__ __launch_bounds__(256) void rotary_kernel(RotaryArgs a) {
   }
   __syncthreads();
 
-  // places of a head: items of pairs, then vectors of the features that are only copied
-  const int turned = ADJACENT ? 2 * a.pairs / I::kWidth : a.pairs / VEC;
-  const int places = turned + (a.dim - 2 * a.pairs) / VEC;
+  const int turned = items(a.turn_span, a.turn_width), places = turned + items(a.copy_span, a.copy_width);
   const int across = places < 256 ? places : 256, step = 256 / across;
   const int mine = (int)threadIdx.x / across;
   if (mine >= step) return;
@@ -131,65 +125,79 @@ __global__ __launch_bounds__(256) void rotary_kernel(RotaryArgs a) {
     x = reinterpret_cast<const T*>(a.in[which] + base[local][which] + head * a.in_stride[which][1]);
     y = reinterpret_cast<T*>(a.out[which] + base[local][2 + which] + head * a.out_stride[which][1]);
   };
-  for (int place = (int)threadIdx.x - mine * across; place < places; place += across) {
-    if (place < turned) {
-      const int d = place * I::kWidth;
-      int n = mine;
-      for (; n + step < heads; n += 2 * step) {
-        const T *x0, *x1;
-        T *y0, *y1;
-        int t0, t1;
-        find(n, x0, y0, t0);
-        find(n + step, x1, y1, t1);
-        I i0, i1;
-        i0.load(x0, d, a.pairs);
-        i1.load(x1, d, a.pairs);
-        i0.turn(table_cos + t0 * a.pairs, table_sin + t0 * a.pairs, d);
-        i0.store(y0, d, a.pairs);
-        i1.turn(table_cos + t1 * a.pairs, table_sin + t1 * a.pairs, d);
-        i1.store(y1, d, a.pairs);
-      }
-      if (n < heads) {
-        const T* x;
-        T* y;
-        int t;
-        find(n, x, y, t);
-        I i;
-        i.load(x, d, a.pairs);
-        i.turn(table_cos + t * a.pairs, table_sin + t * a.pairs, d);
-        i.store(y, d, a.pairs);
-      }
-    } else {
-      const int d = 2 * a.pairs + (place - turned) * VEC;
-      for (int n = mine; n < heads; n += step) {
-        const T* x;
-        T* y;
-        int t;
-        find(n, x, y, t);
-        float v[VEC];
-        load_f32<T, VEC>(x + d, v);
-        store_f32<T, VEC>(y + d, v);
-      }
+  auto go = [&](auto width, bool turns, int d0, int d1) {
+    typedef Item<T, ADJACENT, decltype(width)::value> I;
+    const int angle = turns ? (ADJACENT ? d0 / 2 : d0) : 0;
+    const float *cs = table_cos + angle, *sn = table_sin + angle;
+    int n = mine;
+    for (; n + step < heads; n += 2 * step) {
+      const T *x0, *x1;
+      T *y0, *y1;
+      int t0, t1;
+      find(n, x0, y0, t0);
+      find(n + step, x1, y1, t1);
+      I i0, i1;
+      i0.load(x0, d0, d1);
+      i1.load(x1, d0, d1);
+      i0.turn(cs + t0 * a.pairs, sn + t0 * a.pairs, turns);
+      i0.store(y0, d0, d1);
+      i1.turn(cs + t1 * a.pairs, sn + t1 * a.pairs, turns);
+      i1.store(y1, d0, d1);
     }
+    if (n < heads) {
+      const T* x;
+      T* y;
+      int t;
+      find(n, x, y, t);
+      I i;
+      i.load(x, d0, d1);
+      i.turn(cs + t * a.pairs, sn + t * a.pairs, turns);
+      i.store(y, d0, d1);
+    }
+  };
+  for (int place = (int)threadIdx.x - mine * across; place < places; place += across) {
+    const bool turns = place < turned;
+    const int width = turns ? a.turn_width : a.copy_width;
+    const int at = turns ? min(place * width, a.turn_span - width) : min((place - turned) * width, a.copy_span - width);
+    const int d0 = turns ? at : 2 * a.pairs + at, d1 = turns ? at + a.pairs : a.dim - a.copy_span + at;
+    if (width == 16 / (int)sizeof(T)) go(Width<16 / (int)sizeof(T)>(), turns, d0, d1);
+    else if (sizeof(T) == 2 && width == 4) go(Width<4>(), turns, d0, d1);
+    else if (width == 2) go(Width<2>(), turns, d0, d1);
+    else if (!ADJACENT || !turns) go(Width<1>(), turns, d0, d1);
   }
-}
-
-template <typename T, int VEC>
-int launch(const RotaryArgs& a, bool adjacent, hipStream_t stream) {
-  const dim3 grid((unsigned)cdiv64(a.tokens, a.group)), block(256);
-  if (adjacent) hipLaunchKernelGGL((rotary_kernel<T, true, VEC>), grid, block, 0, stream, a);
-  else hipLaunchKernelGGL((rotary_kernel<T, false, VEC>), grid, block, 0, stream, a);
-  return launch_status();
 }
 
 template <typename T>
-int launch_width(const RotaryArgs& a, bool adjacent, int width, hipStream_t stream) {
-  if constexpr (sizeof(T) == 2) {
-    if (width == 8) return launch<T, 8>(a, adjacent, stream);
+int launch(const RotaryArgs& a, bool adjacent, hipStream_t stream) {
+  const dim3 grid((unsigned)cdiv64(a.tokens, a.group)), block(256);
+  if (adjacent) hipLaunchKernelGGL((rotary_kernel<T, true>), grid, block, 0, stream, a);
+  else hipLaunchKernelGGL((rotary_kernel<T, false>), grid, block, 0, stream, a);
+  return launch_status();
+}
+
+// Cuts a head into items.  Those of pairs cover turn_span features from 0 (the first half of the pairs: an
+// item's second place lies `pairs` behind; or all adjacent ones), those of the rest copy_span features from
+// 2 * pairs (second places end with the head).  The last item of either ends with the span, so it may cover
+// features that others cover too: all write the same.  Only where pairs are turned in place does each
+// belong to one item.  Lanes with items of two widths take turns, so both get the smaller one where that
+// makes fewer than twice the items (5 pairs and 70 more features: 11 items of 4 instead of 2 of 4 and 5
+// of 8, 68 -> 40 us for 8 x 4096 tokens of 24 heads).
+void cut(RotaryArgs& a, int most, bool adjacent, bool in_place) {
+  const int copied = a.dim - 2 * a.pairs;
+  a.turn_span = adjacent ? 2 * a.pairs : a.pairs;
+  a.turn_width = a.copy_width = most;
+  while (a.turn_width > 1 && (a.turn_width > a.turn_span || (in_place && a.turn_span % a.turn_width != 0)))
+    a.turn_width /= 2;
+  while (a.copy_width > 1 && a.copy_width > copied) a.copy_width /= 2;
+  auto span = [&](int width) { return adjacent || copied == 0 ? copied : std::max((copied + 1) / 2, width); };
+  a.copy_span = span(a.copy_width);
+  const int least = std::min(a.turn_width, a.copy_width);
+  if (a.turn_span == 0 || copied == 0 || (adjacent && least < 2)) return;
+  if (items(a.turn_span, least) + items(span(least), least) <
+      2 * (items(a.turn_span, a.turn_width) + items(a.copy_span, a.copy_width))) {
+    a.turn_width = a.copy_width = least;
+    a.copy_span = span(least);
   }
-  if (width >= 4) return launch<T, 4>(a, adjacent, stream);
-  if (width >= 2) return launch<T, 2>(a, adjacent, stream);
-  return launch<T, 1>(a, adjacent, stream);
 }
 
 }  // namespace
@@ -218,21 +226,12 @@ int at_rotary(const at_rotary_t* s, const void* q, const void* k, void* q_out, v
   RotaryArgs a = {};
   a.in[0] = (const char*)q; a.in[1] = (const char*)k;
   a.out[0] = (char*)q_out; a.out[1] = (char*)k_out;
-  // features of an access: the largest power of two that the pairs (both halves of them, or adjacent
-  // ones), the head, the strides and the addresses are multiples of, up to 16 bytes
-  int64_t common = (s->adjacent ? 2 * s->pairs : s->pairs) | s->dim | 16 / size;
-  int64_t bytes = 16;
   for (int n = 0; n < 2; ++n) {
-    if ((n == 0 ? s->q_heads : s->k_heads) == 0) continue;
-    bytes |= (int64_t)(uintptr_t)a.in[n] | (int64_t)(uintptr_t)a.out[n];
     for (int j = 0; j < 3; ++j) {
       a.in_stride[n][j] = s->strides[n][j] * size;
       a.out_stride[n][j] = s->strides[2 + n][j] * size;
-      bytes |= a.in_stride[n][j] | a.out_stride[n][j];
     }
   }
-  common |= (bytes & -bytes) / size;
-  const int width = (int)(common & -common);
   a.positions = positions;
   a.inv_freq = inv_freq;
   a.pair_axis = pair_axis;
@@ -246,15 +245,16 @@ int at_rotary(const at_rotary_t* s, const void* q, const void* k, void* q_out, v
   a.axes = (int)s->axes;
   a.position_type = s->position_type;
   a.inverse = s->inverse != 0;
+  cut(a, 16 / size, s->adjacent != 0, (q && q == q_out) || (k && k == k_out));
   // tokens of a workgroup: as many as fill its lanes with angles, as long as every CU keeps several workgroups
   int group = a.pairs > 0 ? 256 / a.pairs : 4;
   if (group > kMaxTokens) group = kMaxTokens;
   while (group > 1 && a.tokens / group < 4 * (int64_t)device_cu_count()) group /= 2;
   a.group = group < 1 ? 1 : group;
   if (cdiv64(a.tokens, a.group) >= ((int64_t)1 << 24)) return AT_ERR_DIM;
-  if (s->dtype == AT_DTYPE_F32) return launch_width<float>(a, s->adjacent != 0, width, (hipStream_t)stream);
-  if (s->dtype == AT_DTYPE_F16) return launch_width<f16_t>(a, s->adjacent != 0, width, (hipStream_t)stream);
-  return launch_width<bf16_t>(a, s->adjacent != 0, width, (hipStream_t)stream);
+  if (s->dtype == AT_DTYPE_F32) return launch<float>(a, s->adjacent != 0, (hipStream_t)stream);
+  if (s->dtype == AT_DTYPE_F16) return launch<f16_t>(a, s->adjacent != 0, (hipStream_t)stream);
+  return launch<bf16_t>(a, s->adjacent != 0, (hipStream_t)stream);
 }
 
 }  // extern "C"

@@ -2,6 +2,8 @@
 GPU parity tests of rotary positions against the float64 oracle, whose error bounds are the tolerances.
 """
 
+import ctypes
+
 import pytest
 import torch
 
@@ -47,6 +49,33 @@ def test_sizes(dim, sections, adjacent, dtype) -> None:
     inv_freq, pair_axis = tables(sections)
     q, k = randn((3, 5, 7, dim), 1, dtype), randn((3, 2, 7, dim), 2, dtype)
     check(q, k, positions_of((axes, 3, 7), 3), inv_freq, pair_axis, adjacent)
+
+
+# numbers of pairs and of features behind them that no vector divides; more places than a workgroup has lanes
+@pytest.mark.parametrize('dtype', DTYPES)
+@pytest.mark.parametrize('adjacent', [False, True])
+@pytest.mark.parametrize('dim, pairs', [(80, 5), (80, 37), (72, 27), (24, 7), (31, 11), (3, 1), (1, 0), (127, 1), (129, 63),
+                                        (2100, 512), (2100, 3), (4099, 0)])
+def test_uneven_sizes(dim, pairs, adjacent, dtype) -> None:
+    inv_freq, pair_axis = tables((pairs,))
+    q, k = randn((2, 3, 5, dim), 1, dtype), randn((2, 2, 5, dim), 2, dtype)
+    check(q, k, positions_of((1, 2, 5), 3), inv_freq, pair_axis, adjacent)
+
+
+# at the C entry an output may be the input itself
+@pytest.mark.parametrize('dtype', DTYPES)
+@pytest.mark.parametrize('adjacent', [False, True])
+@pytest.mark.parametrize('dim, pairs', [(80, 5), (80, 37), (72, 27), (31, 11), (3, 1), (127, 1), (128, 64), (2100, 509)])
+def test_in_place(dim, pairs, adjacent, dtype) -> None:
+    inv_freq = tables((pairs,))[0].cuda()
+    q, k = (randn((9, heads, 70, dim), heads, dtype).cuda() for heads in (3, 2))
+    expected = attorch_amd.RotaryAutoGrad.apply(q, k, None, inv_freq, None, adjacent)
+    layouts = [attorch_amd.rotary._layout(t) for t in (q, k)]
+    shape = attorch_amd.rotary._plan(*layouts, None, attorch_amd.rotary._layout(inv_freq), None, adjacent, False)
+    stream = attorch_amd._lib.stream_of(q)
+    assert attorch_amd._lib.load().at_rotary(ctypes.byref(shape), q.data_ptr(), k.data_ptr(), q.data_ptr(), k.data_ptr(),
+                                             None, inv_freq.data_ptr(), None, stream) == 0
+    assert torch.equal(q, expected[0]) and torch.equal(k, expected[1])
 
 
 @pytest.mark.parametrize('dtype', DTYPES)
