@@ -226,16 +226,18 @@ typedef __attribute__((address_space(3))) float lds_float;
 typedef __attribute__((address_space(3))) i32x4 lds_i32x4;
 
 // [ROWS][dim] tile, dim padded with zeros to DT * 32 elements, rows of 64 (DT <= 2) or 128 elements.
-// The 16-byte chunks of a row are permuted by an XOR with spread(row) so that both kinds of
-// fragment reads touch all banks: 8 consecutive rows at one chunk (row order) as well as 4
-// consecutive rows at two neighbouring chunks (transposed reads).
+// The 16-byte chunks of a row are permuted by an XOR with spread(row) so that both kinds of fragment
+// reads touch each of the 64 banks once per pass: 16 consecutive rows at one chunk (row order), and 4
+// consecutive rows at four neighbouring chunks (transposed reads).  Counted over whole passes, no cycle
+// is lost to conflicts; it was a third of the forward pass's reads where only two neighbouring chunks of
+// the four were apart (window of 1024 over 8192 tokens: the three kernels 1467 -> 1448 us).
 template <typename T, int DT> struct Tile {
   static constexpr int kPitch = (DT <= 2 ? 64 : 128) * (int)sizeof(T);
   static constexpr int kChunks = kPitch / 16;
   static constexpr int kSteps = 2 * DT;             // contraction steps of 16 over dim
 
   static __device__ __forceinline__ int spread(int row) {
-    return ((row & 3) << 1) | ((row >> 2) & 1) | (kChunks >= 16 ? (row & 8) : 0);
+    return kChunks >= 16 ? ((row & 3) << 2) | ((row >> 2) & 3) : (((row >> 1) & 1) << 2) | ((row >> 2) & 3);
   }
   // Where a lane reads: byte addresses in LDS of its first fragments of a tile.  Tiles start at multiples of
   // kPitch, so a step along dim is an XOR with a constant, and rows further down are immediate offsets:
