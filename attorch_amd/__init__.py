@@ -4,7 +4,8 @@ MI355X-native implementation of attorch's layer-kernel hot path.
 The public names match attorch's (Linear, LayerNorm, RMSNorm, Softmax, LogSoftmax, Softmin,
 CrossEntropyLoss, NLLLoss, the p-norm losses, GLU, Conv2d, BatchNorm2d, AvgPool, the activation layers
 with fused dropout, Dropout, and their autograd Functions), so
-`import attorch_amd as attorch` is a drop-in for that path.  All compute happens in
+`import attorch_amd as attorch` is a drop-in for that path.  WindowAttention and Rotary add what a
+GPT block has between its projections.  All compute happens in
 hand-written gfx950 HIP kernels behind the C ABI declared in include/attorch_hip.h.
 """
 

@@ -11,7 +11,18 @@
 //
 // delta is taken from the output before its rounding (the forward pass keeps what the rounding left
 // over): an error of delta is common to a whole row of ds, and with the rounded output it was the largest
-// one in dq and dk (bf16, 512 tokens: 2.0e-3 of them against 1.7e-3 for rounding ds).
+// one in dq and dk (bf16, 512 tokens: 2.0e-3 of them against 1.7e-3 for rounding ds).  p and ds are rounded
+// to the inputs' type, as operands of the matrix cores, and ds without scale, which the sums get in fp32.
+// ds of fp16 inputs has output_grad's magnitude, so it is no larger than what the caller's loss scaling
+// already keeps in range, and its small values lose what gradients stored in fp16 lose.
+//
+// Both kernels are built as the forward kernel is: a lane holds a row (first) or a key (second) of each
+// result, which then is the next product's operand as it stands.  They are bound by the matrix cores, three
+// and four products per tile, at the clock that their power leaves (1.7 to 2.0 GHz).  4 x 32 heads, 4096
+// tokens, causal, 128 features, bf16: dq 0.82 ms and dk, dv 1.15 ms, 1000 and 960 TFLOP/s; window of 1024
+// over 2 x 8192 tokens, 32 heads on 8: 0.47 and 0.59 ms, 820 and 880 TFLOP/s.  fp32, 777 patches: 50 and
+// 57 us, 74 and 86 of the 139 TFLOP/s that a large product reaches.  (One launch that adds dq with atomics
+// would save a product of the scores and lose the fixed order.)
 #include "attention.h"
 
 namespace at_hip {
