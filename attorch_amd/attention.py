@@ -74,10 +74,13 @@ def _strides(shape: Sequence[int], stride: Sequence[int]) -> Tuple[int, int, int
 
 
 def _check(query: Layout, key: Layout, value: Layout, lengths: Optional[Layout], query_lengths: Optional[Layout],
-           window: Optional[int], num_sinks: int, scale: Optional[float]) -> None:
+           causal: bool, window: Optional[int], num_sinks: int, scale: Optional[float]) -> None:
     """
     Refuses what the kernels do not compute, before anything is launched.
     """
+    for name, option in (('causal', causal), ('window', window), ('num_sinks', num_sinks), ('scale', scale)):
+        if isinstance(option, Tensor):      # its value could change behind the layers' back
+            raise RuntimeError(f'{name} must be a plain value, received a tensor')
     (q, _, dtype, _), (k, _, k_dtype, _), (v, _, v_dtype, _) = query, key, value
     assert len(q) == 4 and len(k) == 4 and len(v) == 4, \
         f'Query, key and value must be [batch, heads, tokens, head_dim], received {tuple(q)}, {tuple(k)} and {tuple(v)}'
@@ -111,7 +114,7 @@ class _Plan:
     """
     What a forward call of given layouts and options passes on: nothing in it belongs to a tensor.
     """
-    __slots__ = ('direct', 'shape', 'ref', 'group', 'scale', 'output_shape', 'rest_bytes', 'kept_bytes',
+    __slots__ = ('direct', 'shape', 'ref', 'group', 'scale', 'output_shape', 'output_stride', 'rest_bytes', 'kept_bytes',
                  'workspace_bytes', 'like_inputs', 'grad_strides')
 
 
@@ -124,7 +127,7 @@ def _forward_plan(query: Layout, key: Layout, value: Layout, lengths: Optional[L
     depends on the device.  Remembered by layouts and options, since a program repeats few of them and
     the description takes longer than a small call's kernels.
     """
-    _check(query, key, value, lengths, query_lengths, window, num_sinks, scale)
+    _check(query, key, value, lengths, query_lengths, causal, window, num_sinks, scale)
     batch, heads, rows, dim = query[0]
     kv_heads, keys = key[0][1:3]
     plan = _Plan()
@@ -135,8 +138,8 @@ def _forward_plan(query: Layout, key: Layout, value: Layout, lengths: Optional[L
                    all(c[1] == (1,) or batch <= 1 for c in counts) and len({c[2] for c in counts}) <= 1)
     if not plan.direct:
         return plan
-    plan.output_shape = (batch, rows, heads, dim)
-    strides = [*_strides(*query[:2]), *_strides(*key[:2]), *_strides(*value[:2]), rows * heads * dim, dim, heads * dim]
+    plan.output_shape, plan.output_stride = (batch, heads, rows, dim), (rows * heads * dim, dim, heads * dim, 1)
+    strides = [*_strides(*query[:2]), *_strides(*key[:2]), *_strides(*value[:2]), *plan.output_stride[:3]]
     plan.shape = _Shape(batch, heads, kv_heads, rows, keys, dim, min(window or 0, 1 << 40), min(num_sinks, 1 << 40),
                         (ctypes.c_int64 * 24)(*strides), plan.scale, bool(causal), _lib.dtype_id(dtype),
                         int(bool(counts) and counts[0][2] is torch.int64))
@@ -240,7 +243,8 @@ class WindowAttentionAutoGrad(torch.autograd.Function):
             plan = _forward_plan(_layout(query), _layout(key), _layout(value), *counts, *options, plan.scale, output_dtype,
                                  device)
 
-        output = torch.empty(plan.output_shape, device=query.device, dtype=output_dtype)
+        # not as a view: autograd refuses to change those of a Function in place
+        output = torch.empty_strided(plan.output_shape, plan.output_stride, device=query.device, dtype=output_dtype)
         kept = rest = lse = workspace = None
         needs_grad = ctx.needs_input_grad
         if needs_grad[0] or needs_grad[1] or needs_grad[2]:
@@ -257,12 +261,16 @@ class WindowAttentionAutoGrad(torch.autograd.Function):
                 None if workspace is None else workspace.data_ptr(), plan.workspace_bytes, _lib.stream_of(query)),
                 'at_attention_fwd')
 
-        output = output.transpose(1, 2)
         if kept is not None:
             ctx.plan = plan
             ctx.head_dim = head_dim
             ctx.save_for_backward(query, key, value, output, kept, lengths, query_lengths)
-        return output if output.shape[3] == head_dim else output[..., :head_dim]
+        if output.shape[3] == head_dim:
+            return output
+        batch, heads, rows, _ = plan.output_shape
+        narrow = torch.empty_strided((batch, heads, rows, head_dim), (rows * heads * head_dim, head_dim, heads * head_dim, 1),
+                                     device=query.device, dtype=output_dtype)
+        return narrow.copy_(output[..., :head_dim])
 
     @staticmethod
     def backward(

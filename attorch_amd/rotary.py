@@ -180,6 +180,8 @@ class RotaryAutoGrad(torch.autograd.Function):
         Returns:
             Turned queries and keys (None without keys), of the dtypes of the inputs.
         """
+        if ctx.needs_input_grad[2] or ctx.needs_input_grad[3]:
+            raise RuntimeError('Rotary has no gradients of positions and inv_freq; detach them')
         if not inv_freq.is_contiguous():
             inv_freq = inv_freq.contiguous()
         if pair_axis is not None and not pair_axis.is_contiguous():

@@ -46,6 +46,10 @@ def test_attention_arguments() -> None:
                            ((True, 4, 0, float('inf')), 'scale'), ((True, 4, 0, float('nan')), 'scale')):
         with pytest.raises(RuntimeError, match=match):
             apply(*qkv(), None, None, *options)
+    for options, match in (((torch.tensor(True),), 'causal'), ((True, torch.tensor(3)), 'window'),
+                           ((True, 3, torch.tensor(1)), 'num_sinks'), ((True, 3, 1, torch.tensor(0.5)), 'scale')):
+        with pytest.raises(RuntimeError, match=f'{match} must be a plain value'):
+            apply(*qkv(), None, None, *options)
     with pytest.raises(RuntimeError, match='int32 or int64'):
         apply(*qkv(), torch.zeros(2))
     with pytest.raises(AssertionError):
@@ -70,6 +74,9 @@ def test_rotary_arguments() -> None:
                  (q, k, positions, freq, axis[:4]), (q, k, None, freq, axis), (q, k, positions[0, 0], freq, axis),
                  (q, k, positions[:, :, :4], freq, axis), (q, k, positions[:, :1], freq), (q, k, positions[0, 0, :4], freq)):
         with pytest.raises(AssertionError):
+            apply(*args)
+    for args in ((q, k, torch.zeros(5, requires_grad=True), freq), (q, k, None, freq.clone().requires_grad_())):
+        with pytest.raises(RuntimeError, match='no gradients of positions and inv_freq'):
             apply(*args)
     for args, match in (((q.half(), k, None, freq), 'same dtype'), ((q, k, None, freq.float()), 'float64'),
                         ((q, k, positions, freq, axis.long()), 'int32')):

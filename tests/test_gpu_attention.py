@@ -81,6 +81,15 @@ def test_windows(window, sinks, causal, dtype) -> None:
 
 @pytest.mark.parametrize('dtype', DTYPES)
 @pytest.mark.parametrize('causal', [True, False])
+@pytest.mark.parametrize('heads, kv_heads, window, sinks', [(3, 1, 100, 0), (5, 1, 37, 3), (4, 4, 65, 0), (24, 3, 129, 1)])
+def test_windows_over_many_tiles(heads, kv_heads, window, sinks, causal, dtype) -> None:
+    """Tiles of keys whose rows are several windows away from the first one, in whole and padded batches."""
+    check(*inputs(2, heads, kv_heads, 1100, 1100, 24, dtype), lengths=torch.tensor([1100, 777]), causal=causal, window=window,
+          sinks=sinks)
+
+
+@pytest.mark.parametrize('dtype', DTYPES)
+@pytest.mark.parametrize('causal', [True, False])
 @pytest.mark.parametrize('window, sinks', [(20, 1), (20, 33), (20, 64), (33, 65), (20, 129), (100, 140), (20, 300), (1, 700)])
 def test_sinks_far_from_their_readers(window, sinks, causal, dtype) -> None:
     """
@@ -256,6 +265,26 @@ def test_frozen_inputs_and_no_grad() -> None:
     (grad,) = torch.autograd.grad(out, leaves[0], dout, create_graph=True)
     with pytest.raises(RuntimeError):
         grad.sum().backward()          # no second derivatives
+
+
+@pytest.mark.parametrize('dim', [32, 20])
+def test_outputs_changed_in_place(dim) -> None:
+    """Outputs are no views, so they may be changed in place where no backward pass needs them."""
+    q, k, v, dout = (t.cuda() for t in inputs(1, 2, 2, 40, 40, dim, torch.float16))
+    expected = attorch_amd.WindowAttention()(q, k, v)
+    leaves = [t.detach().requires_grad_() for t in (q, k, v)]
+    out = attorch_amd.WindowAttention()(*leaves)
+    assert torch.equal(out, expected) and out.stride() == expected.stride() and not out._is_view()
+    out.mul_(2.0)
+    assert torch.equal(out, 2.0 * expected)
+    with torch.inference_mode():
+        out = attorch_amd.WindowAttention()(*leaves)
+        assert torch.equal(out.mul_(2.0), 2.0 * expected)
+    if dim % 8:                        # a copy of what the backward pass needs
+        out = attorch_amd.WindowAttention()(*leaves)
+        got = torch.autograd.grad(out.mul_(2.0), leaves, dout)
+        for a, b in zip(got, torch.autograd.grad(attorch_amd.WindowAttention()(*leaves), leaves, 2.0 * dout)):
+            assert torch.equal(a, b)
 
 
 def test_other_stream_and_graph() -> None:
