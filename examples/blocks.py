@@ -251,9 +251,13 @@ class TinyGPT(nn.Module):
     def extend(self, tokens: Tensor, cache: List[Tuple[Tensor, Tensor]], lengths: Tensor) -> Tensor:
         """
         Logits of new tokens (a prompt, a part of one or single tokens), which are the last ones of
-        sequences that have `lengths` tokens with them; their keys and values go into the cache.
-        For the fused backend with rotary.
+        sequences that have `lengths` tokens with them; their keys and values go into the cache,
+        which must have room for them.  For the fused backend with rotary.
         """
+        if self.pos_embed is not None or not all(block.fused for block in self.blocks):
+            raise RuntimeError('Sequences are continued on attorch_amd.nn and with rotary positions only')
+        if tokens.shape[1] > cache[0][0].shape[2]:
+            raise RuntimeError(f'The cache has room for {cache[0][0].shape[2]} tokens, received {tokens.shape[1]} new ones')
         output = self.tok_embed(tokens)
         for block, stored in zip(self.blocks, cache):
             output = block(output, stored, lengths)

@@ -12,6 +12,7 @@ import attorch_amd
 from attorch_amd import _lib
 from attorch_amd.attention import _Shape as AttentionShape
 from attorch_amd.rotary import _Shape as RotaryShape
+from examples.blocks import TinyGPT
 
 
 def qkv(batch=2, heads=4, kv_heads=2, rows=5, keys=5, dim=16, dtype=torch.float32):
@@ -62,6 +63,14 @@ def test_attention_arguments() -> None:
         attorch_amd.WindowAttention(window=0)
     with pytest.raises(RuntimeError, match='sinks'):
         attorch_amd.WindowAttention(num_sinks=-1)
+
+
+def test_continued_sequences_of_other_models() -> None:
+    tokens, lengths = torch.zeros(1, 3, dtype=torch.int64), torch.tensor([3])
+    for options in ({'rotary': True}, {}, {'window': 4}):
+        model = TinyGPT(torch.nn, 20, 1, 32, 2, 8, **options)
+        with pytest.raises(RuntimeError, match='continued'):
+            model.extend(tokens, model.new_cache(1, 8), lengths)
 
 
 def test_rotary_arguments() -> None:
