@@ -38,6 +38,7 @@ struct AttentionArgs {
   int lengths64, causal;
   int batch, kv_heads, group, rows, keys, dim;
   int row_pitch, tiles, splits, waves_per_row, slots;
+  int narrow;                          // forward: tiles of 32 keys (see plan)
   int sink_tiles, far_chunks, far_steps, chunks, chunk_steps;   // dk and dv: see chunk_plan
   int left, right, sinks;
   float scale, scale_log2;

@@ -24,12 +24,13 @@
 // keys with up to five on their way read 4.5 TB/s: fewer, larger loads keep memory busier.  For many rows
 // they leave room for three workgroups per CU: window 1024 358 -> 341 us, but 346 -> 360 us for causal
 // rows of 64 features and 70 -> 84 us for fewer workgroups than that fills.)
+#include <algorithm>
+
 #include "attention.h"
 
 namespace at_hip {
 namespace {
 
-constexpr int kKeys = 64;        // keys of a tile
 constexpr int kWaves = 4;
 constexpr int kMaxSplits = 128;
 
@@ -47,13 +48,13 @@ __device__ __forceinline__ void store_output(const AttentionArgs& a, int64_t to,
   }
 }
 
-// WK waves share 32 rows and halve each tile of keys among them (1 or 2); they join at the end.
-template <typename T, int DT, int WK>
-__global__ __launch_bounds__(kWaves * 64, (kPerCu<T, DT>)) void attention_fwd_kernel(AttentionArgs a) {
+// WK waves share 32 rows and halve each tile of KEYS keys among them (1 or 2); they join at the end.
+template <typename T, int DT, int WK, int KEYS>
+__global__ __launch_bounds__(kWaves * 64, (KEYS == 32 ? 2 : kPerCu<T, DT>)) void attention_fwd_kernel(AttentionArgs a) {
   typedef Tile<T, DT> L;
   typedef typename Frag<T>::type F;
-  constexpr int kTileBytes = kKeys * L::kPitch;
-  constexpr int kRows = 32 * kWaves / WK, kMine = kKeys / WK, NS = kMine / 32;
+  constexpr int kTileBytes = KEYS * L::kPitch;
+  constexpr int kRows = 32 * kWaves / WK, kMine = KEYS / WK, NS = kMine / 32;
   __shared__ __attribute__((aligned(1024))) char lds[4 * kTileBytes];   // two stages of keys | values
 
   const int lane = threadIdx.x & 63, half = lane >> 5;
@@ -99,8 +100,8 @@ __global__ __launch_bounds__(kWaves * 64, (kPerCu<T, DT>)) void attention_fwd_ke
   KeyRange range = {0, 0, 0};
   if (row0 < live_rows)
     range = keys_of(a, seq, seq.start + row0 / a.group, seq.start + (min(row0 + kRows, live_rows) - 1) / a.group);
-  const KeyWalk walk(range, max(a.k.token, a.v.token), kKeys);
-  if (row0 < live_rows) tiles = (walk.end + kKeys - 1) / kKeys;
+  const KeyWalk walk(range, max(a.k.token, a.v.token), KEYS);
+  if (row0 < live_rows) tiles = (walk.end + KEYS - 1) / KEYS;
   const int split = blockIdx.y;
   const int t_begin = (int)((int64_t)tiles * split / a.splits), t_end = (int)((int64_t)tiles * (split + 1) / a.splits);
 
@@ -113,14 +114,14 @@ __global__ __launch_bounds__(kWaves * 64, (kPerCu<T, DT>)) void attention_fwd_ke
   const int val_offs[2] = {L::template lane_offset<kWaves>(val_off, dim_bytes, 0),
                            L::template lane_offset<kWaves>(val_off, dim_bytes, 1)};
   auto fetch = [&](int t, char* stage) {
-    const int v0 = t * kKeys, k0 = walk.first_key(v0);
+    const int v0 = t * KEYS, k0 = walk.first_key(v0);
     const i32x4 kr = open_rsrc(kb + k0 * a.k.token), vr = open_rsrc(vb + k0 * a.v.token);
-    if (v0 >= walk.begin && v0 + kKeys <= walk.end) {
-      L::template fetch_all<kKeys, kWaves>(kr, key_offs, kWaves * L::kLoadRows * (int)a.k.token, stage);
-      L::template fetch_all<kKeys, kWaves>(vr, val_offs, kWaves * L::kLoadRows * (int)a.v.token, stage + kTileBytes);
+    if (v0 >= walk.begin && v0 + KEYS <= walk.end) {
+      L::template fetch_all<KEYS, kWaves>(kr, key_offs, kWaves * L::kLoadRows * (int)a.k.token, stage);
+      L::template fetch_all<KEYS, kWaves>(vr, val_offs, kWaves * L::kLoadRows * (int)a.v.token, stage + kTileBytes);
     } else {
-      L::template fetch<kKeys, kWaves>(kr, dim_bytes, stage, [&](int r) { return walk.offset(v0, r, (int)a.k.token); });
-      L::template fetch<kKeys, kWaves>(vr, dim_bytes, stage + kTileBytes,
+      L::template fetch<KEYS, kWaves>(kr, dim_bytes, stage, [&](int r) { return walk.offset(v0, r, (int)a.k.token); });
+      L::template fetch<KEYS, kWaves>(vr, dim_bytes, stage + kTileBytes,
                                       [&](int r) { return walk.offset(v0, r, (int)a.v.token); });
     }
   };
@@ -132,8 +133,8 @@ __global__ __launch_bounds__(kWaves * 64, (kPerCu<T, DT>)) void attention_fwd_ke
     __syncthreads();     // tile t is everybody's, and nobody reads the other stage any more
     if (t + 1 < t_end) fetch(t + 1, lds + ((t - t_begin + 1) & 1) * 2 * kTileBytes);
     // the wave's part of the tile: places v0 ..; behind the sinks these are the keys k0 ..
-    const int v0 = t * kKeys + wave_key, k0 = v0 + walk.shift;
-    const bool mixed = t * kKeys < walk.begin;
+    const int v0 = t * KEYS + wave_key, k0 = v0 + walk.shift;
+    const bool mixed = t * KEYS < walk.begin;
     if (last < first || !(mixed || (k0 < mine.hi && k0 + kMine > mine.lo) || k0 < mine.sinks)) continue;
 
     const typename L::Reader lr = L::reader(stage + wave_key * L::kPitch);
@@ -321,18 +322,32 @@ __global__ __launch_bounds__(256) void attention_join_kernel(AttentionArgs a) {
 // How the work is cut: into tiles of 128 rows, or of 64 whose waves share rows in pairs (waves_per_row), and
 // where these do not fill the GPU, the keys are split among several workgroups with at least four tiles of
 // keys each, which another launch of 4 us joins (a tile takes a workgroup about 1).
+//
+// fp32 heads of more than 64 features fill LDS with one workgroup's tiles of 64 keys.  Tiles of 32 let a CU
+// hold two workgroups, which pays where there are several for each place, and for single tokens where the
+// splits fill them all: window of 512 over 4096 tokens, 32 heads on 8 of 128: 344 -> 287 us; single tokens
+// over 64 x 600: 198 -> 102 us, 16 x 4096: 201 -> 172 us, 32768: 97 -> 89 us.  Elsewhere waves that share
+// rows, or workgroups that follow each other, do better: causal, 2 x 2048 tokens, 16 heads: 307 against 372
+// us; single tokens over 5 x 2359, 4 heads: 37 against 50 us.
 void plan(AttentionArgs& a) {
   const int64_t heads = (int64_t)a.batch * a.kv_heads, rows = (int64_t)a.rows * a.group;
-  const int64_t want = a.slots;
-  a.waves_per_row = waves_per_row(rows, heads, a.slots);
+  // keys that one tile of rows can see
+  auto tiles_seen = [&](int64_t tile_rows) {
+    const int64_t span = (int64_t)a.left + a.right + cdiv64(tile_rows, a.group) + a.sinks;
+    return cdiv64(span < a.keys ? span : a.keys, 64);
+  };
+  const int64_t two_per_cu = 2 * (int64_t)device_cu_count();
+  const int64_t whole = cdiv64(rows, 32 * kWaves) * heads;
+  a.narrow = a.slots < two_per_cu &&
+             (whole >= 2 * two_per_cu || (rows <= 32 && heads * std::max<int64_t>(tiles_seen(32 * kWaves) / 4, 1) >= two_per_cu));
+  const int64_t want = a.narrow ? two_per_cu : a.slots;
+  a.waves_per_row = a.narrow ? 1 : waves_per_row(rows, heads, a.slots);
   const int64_t tile_rows = 32 * kWaves / a.waves_per_row;
   a.tiles = (int)cdiv64(rows, tile_rows);
   a.splits = 1;
   const int64_t groups = a.tiles * heads;
   if (groups >= want || groups == 0) return;
-  // keys that one tile of rows can see
-  const int64_t span = (int64_t)a.left + a.right + cdiv64(tile_rows, a.group) + a.sinks;
-  const int64_t tiles = cdiv64(span < a.keys ? span : a.keys, kKeys);
+  const int64_t tiles = tiles_seen(tile_rows);
   int64_t n = want / groups;           // rounded up, a few workgroups would run after all the others
   if (n > tiles / 4) n = tiles / 4;
   a.splits = (int)(n < 1 ? 1 : n > kMaxSplits ? kMaxSplits : n);
@@ -340,8 +355,15 @@ void plan(AttentionArgs& a) {
 
 template <typename T, int DT>
 void launch(const AttentionArgs& a, const dim3& grid, hipStream_t stream) {
-  if (a.waves_per_row == 1) hipLaunchKernelGGL((attention_fwd_kernel<T, DT, 1>), grid, dim3(kWaves * 64), 0, stream, a);
-  else hipLaunchKernelGGL((attention_fwd_kernel<T, DT, 2>), grid, dim3(kWaves * 64), 0, stream, a);
+  const dim3 block(kWaves * 64);
+  if constexpr (kPerCu<T, DT> == 1) {
+    if (a.narrow) {
+      hipLaunchKernelGGL((attention_fwd_kernel<T, DT, 1, 32>), grid, block, 0, stream, a);
+      return;
+    }
+  }
+  if (a.waves_per_row == 1) hipLaunchKernelGGL((attention_fwd_kernel<T, DT, 1, 64>), grid, block, 0, stream, a);
+  else hipLaunchKernelGGL((attention_fwd_kernel<T, DT, 2, 64>), grid, block, 0, stream, a);
 }
 
 template <typename T>

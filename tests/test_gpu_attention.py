@@ -342,3 +342,13 @@ def test_long_cache_offsets() -> None:
         q = randn((1, 4, rows, dim), 3, torch.bfloat16)
         out = attorch_amd.WindowAttention(window=100, num_sinks=4)(q.cuda(), k, v)
         assert_within(out, attention(q, tail_k, tail_v, window=100, sinks=4)['out'], f'{rows} rows')
+
+
+# fp32 heads of more than 64 features, in workgroups of few keys: many rows, and many splits of single tokens
+@pytest.mark.parametrize('batch, heads, kv_heads, rows, keys, dim, window, lengths', [
+    (4, 32, 8, 1030, 1030, 72, 70, [1030, 0, 517, 1]), (4, 64, 64, 515, 515, 104, None, None),
+    (64, 8, 8, 1, 1400, 128, None, list(range(1, 1400, 22))), (3, 4, 2, 5, 60000, 80, None, [60000, 33333, 7]),
+    (2, 24, 8, 2, 20000, 120, 9000, None)])
+def test_wide_heads_in_full_precision(batch, heads, kv_heads, rows, keys, dim, window, lengths) -> None:
+    tensors = inputs(batch, heads, kv_heads, rows, keys, dim, torch.float32)
+    check(*tensors, lengths=None if lengths is None else torch.tensor(lengths[:batch]), window=window, sinks=3)
