@@ -76,6 +76,18 @@ __device__ __forceinline__ KeyRange keys_of(const AttentionArgs& a, const Sequen
   return r;
 }
 
+// How many of the first rows see at most `most` keys each: all of them, those of the first tokens of a causal
+// sequence, or none that is known to.
+__device__ __forceinline__ int rows_that_see(const AttentionArgs& a, const Sequence& s, int most) {
+  if (s.len <= most || a.left + a.right + a.sinks < most) return a.rows * a.group;
+  return a.causal ? max(most - s.start, 0) * a.group : 0;
+}
+// Rows that see no more keys than this form their output without rounding the probabilities: the sum
+// of few roundings does not average out, and through delta it reaches all of a row's gradients (13 tokens in
+// bf16: dq 2.0 times as far off as its own rounding alone, 1.4 times with exact outputs; 512 tokens 1.52 and
+// 1.44 times).  Beyond it, a second product for all keys would cost a third of the forward pass.
+constexpr int kFewKeys = 128;
+
 // The keys of a range as one list, which is walked over in tiles: place v of the list is key v for the
 // sinks (v < sinks) and key v + shift for the others (v >= begin).  The two parts follow each other
 // without a gap, so that a few sinks cost no tile of their own and the first tile of a window starts at
@@ -184,6 +196,15 @@ template <> struct Frag<float> {
       for (int n = 0; n < N; ++n) c[n] = __builtin_amdgcn_mfma_f32_32x32x2f32(f[n].e[j], y.e[j], c[n], 0, 0, 0);
   }
 };
+
+// What the rounding in pack(f) leaves over.
+template <typename T> __device__ __forceinline__ typename Frag<T>::type low_part(const float (&f)[8]) {
+  float r[8];
+  Frag<T>::unpack(Frag<T>::pack(f), r);
+#pragma unroll
+  for (int e = 0; e < 8; ++e) r[e] = f[e] - r[e];
+  return Frag<T>::pack(r);
+}
 
 // Probabilities of fp16 inputs are multiplied by 2^value before they are rounded to fp16: without it
 // those of a long flat row would be subnormal numbers.  In the backward pass they are at most 1, in the

@@ -14,7 +14,8 @@
 // one in dq and dk (bf16, 512 tokens: 2.0e-3 of them against 1.7e-3 for rounding ds).  p and ds are rounded
 // to the inputs' type, as operands of the matrix cores, and ds without scale, which the sums get in fp32.
 // ds of fp16 inputs has output_grad's magnitude, so it is no larger than what the caller's loss scaling
-// already keeps in range, and its small values lose what gradients stored in fp16 lose.
+// already keeps in range, and its small values lose what gradients stored in fp16 lose.  Rows that see a
+// single key have zeros as ds by definition, not what p and delta's roundings would leave.
 //
 // Both kernels are built as the forward kernel is: a lane holds a row (first) or a key (second) of each
 // result, which then is the next product's operand as it stands.  They are bound by the matrix cores, three
@@ -187,6 +188,10 @@ __global__ __launch_bounds__(kWaves * 64, (kPerCu<T, DT>)) void attention_dq_ker
       for (int e = 0; e < 16; ++e) dq[dt][e] += X::get(room, dt * 16 + e);
   }
   if (row >= all_rows) return;
+  if (row < rows_that_see(a, seq, 1)) {   // the only key's probability is 1, whatever the query
+#pragma unroll
+    for (int dt = 0; dt < DT; ++dt) dq[dt] = zero_acc();
+  }
   char* gp = a.dq.p + b * a.dq.batch + head * a.dq.head + i * a.dq.token;
 #pragma unroll
   for (int dt = 0; dt < DT; ++dt)
@@ -363,6 +368,7 @@ __global__ __launch_bounds__(kWaves * 64, (kPerCu<T, DT>)) void attention_dkv_ke
   };
 
   const int start = __builtin_amdgcn_readfirstlane(first_step(a, steps)), count = end - begin;
+  const int single = __builtin_amdgcn_readfirstlane(rows_that_see(a, seq, 1));
   if (count > 0) fetch(start, lds);
   for (int u = 0, t = start, next; u < count; ++u, t = next) {
     char* stage = lds + (u & 1) * kStage;
@@ -403,6 +409,10 @@ __global__ __launch_bounds__(kWaves * 64, (kPerCu<T, DT>)) void attention_dkv_ke
           const bool seen = acc_row(e, 0) >= lo && acc_row(e, 0) <= hi;
           s[e] = seen ? s[e] : 0.f;
           dp[e] = seen ? dp[e] : 0.f;
+        }
+        if (r0 < single) {               // probabilities of 1, whatever the key
+#pragma unroll
+          for (int e = 0; e < 16; ++e) dp[e] = row + acc_row(e, 0) < single ? 0.f : dp[e];
         }
       }
 #pragma unroll

@@ -6,7 +6,8 @@
 // was summed before is rescaled when the maximum grows (exponentials in base 2, fp32 throughout).  The
 // probabilities are rounded to the inputs' type for the second product only, since the matrix cores take
 // 16-bit operands of one type: 2^-9 (bf16) or 2^-12 (fp16) of each on average, as much again as rounding
-// the output leaves (bf16: 2.3e-3 of the output's norm with both, 1.7e-3 with the output's alone).
+// the output leaves (bf16: 2.3e-3 of the output's norm with both, 1.7e-3 with the output's alone).  Where
+// rows see few keys, what that rounding leaves over takes part in a product of its own (kFewKeys).
 //
 // The product is formed as keys x rows, so that a lane holds one row: the maximum and the sum need one
 // exchange between the two halves of a wave, and the probabilities leave the matrix cores as the second
@@ -25,6 +26,7 @@
 // they leave room for three workgroups per CU: window 1024 358 -> 341 us, but 346 -> 360 us for causal
 // rows of 64 features and 70 -> 84 us for fewer workgroups than that fills.)
 #include <algorithm>
+#include <type_traits>
 
 #include "attention.h"
 
@@ -127,71 +129,82 @@ __global__ __launch_bounds__(kWaves * 64, (KEYS == 32 ? 2 : kPerCu<T, DT>)) void
   };
 
   if (t_begin < t_end) fetch(t_begin, lds);
-  for (int t = t_begin; t < t_end; ++t) {
-    char* stage = lds + ((t - t_begin) & 1) * 2 * kTileBytes;
-    lds_dma_wait_all();
-    __syncthreads();     // tile t is everybody's, and nobody reads the other stage any more
-    if (t + 1 < t_end) fetch(t + 1, lds + ((t - t_begin + 1) & 1) * 2 * kTileBytes);
-    // the wave's part of the tile: places v0 ..; behind the sinks these are the keys k0 ..
-    const int v0 = t * KEYS + wave_key, k0 = v0 + walk.shift;
-    const bool mixed = t * KEYS < walk.begin;
-    if (last < first || !(mixed || (k0 < mine.hi && k0 + kMine > mine.lo) || k0 < mine.sinks)) continue;
+  // EXACT: the second product takes what the rounding of the probabilities leaves over as well (see kFewKeys)
+  auto walk_keys = [&](auto exact) {
+    for (int t = t_begin; t < t_end; ++t) {
+      char* stage = lds + ((t - t_begin) & 1) * 2 * kTileBytes;
+      lds_dma_wait_all();
+      __syncthreads();     // tile t is everybody's, and nobody reads the other stage any more
+      if (t + 1 < t_end) fetch(t + 1, lds + ((t - t_begin + 1) & 1) * 2 * kTileBytes);
+      // the wave's part of the tile: places v0 ..; behind the sinks these are the keys k0 ..
+      const int v0 = t * KEYS + wave_key, k0 = v0 + walk.shift;
+      const bool mixed = t * KEYS < walk.begin;
+      if (last < first || !(mixed || (k0 < mine.hi && k0 + kMine > mine.lo) || k0 < mine.sinks)) continue;
 
-    const typename L::Reader lr = L::reader(stage + wave_key * L::kPitch);
-    f32x16 s[NS];
+      const typename L::Reader lr = L::reader(stage + wave_key * L::kPitch);
+      f32x16 s[NS];
 #pragma unroll
-    for (int n = 0; n < NS; ++n) s[n] = zero_acc();
+      for (int n = 0; n < NS; ++n) s[n] = zero_acc();
 #pragma unroll
-    for (int ks = 0; ks < L::kSteps; ++ks)
-      Frag<T>::mma_all([&](int n) { return L::rows_frag(lr, 0, n * 32, ks); }, qf[ks], s);
-    // places of the lane relative to its first one are constants: 8 apart, 4 in a row
-    const bool whole = !mixed && k0 >= last - a.left && k0 + kMine - 1 <= min(first + a.right, seq.len - 1);
-    if (!whole) {
-      int v = v0 + half * 4;
-      asm volatile("" : "+v"(v));      // a branch: as selects the masks would be formed for every tile
-      const int lo = max(see_lo - walk.shift, walk.begin) - v, hi = see_hi - walk.shift - v, sinks = see_sinks - v;
+      for (int ks = 0; ks < L::kSteps; ++ks)
+        Frag<T>::mma_all([&](int n) { return L::rows_frag(lr, 0, n * 32, ks); }, qf[ks], s);
+      // places of the lane relative to its first one are constants: 8 apart, 4 in a row
+      const bool whole = !mixed && k0 >= last - a.left && k0 + kMine - 1 <= min(first + a.right, seq.len - 1);
+      if (!whole) {
+        int v = v0 + half * 4;
+        asm volatile("" : "+v"(v));      // a branch: as selects the masks would be formed for every tile
+        const int lo = max(see_lo - walk.shift, walk.begin) - v, hi = see_hi - walk.shift - v, sinks = see_sinks - v;
+#pragma unroll
+        for (int n = 0; n < NS; ++n)
+#pragma unroll
+          for (int e = 0; e < 16; ++e) {
+            const int c = n * 32 + acc_row(e, 0);
+            s[n][e] = (c >= lo && c <= hi) || c < sinks ? s[n][e] : -INFINITY;
+          }
+      }
+      float top = -INFINITY;
+#pragma unroll
+      for (int e = 0; e < 16; ++e) top = fmaxf(fmaxf(top, s[0][e]), s[NS - 1][e]);
+      top = half_max(top) * a.scale_log2;
+      // The exponentials are taken relative to a maximum that may lag behind by kSlack: any reference gives
+      // the same result, and moving it costs a pass over the output, which now is rare.
+      if (__any(top > m + kSlack)) {
+        const float old = m;
+        m = fmaxf(m, top);
+        const float shrink = m == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(old - m);
+        l *= shrink;
+#pragma unroll
+        for (int dt = 0; dt < DT; ++dt)
+#pragma unroll
+          for (int e = 0; e < 16; ++e) o[dt][e] *= shrink;
+      }
+      const float base = m == -INFINITY ? 0.f : ProbShift<T>::forward - m;   // -inf: the row has seen nothing yet
+      float sum[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
       for (int n = 0; n < NS; ++n)
 #pragma unroll
         for (int e = 0; e < 16; ++e) {
-          const int c = n * 32 + acc_row(e, 0);
-          s[n][e] = (c >= lo && c <= hi) || c < sinks ? s[n][e] : -INFINITY;
+          s[n][e] = __builtin_amdgcn_exp2f(fmaf(s[n][e], a.scale_log2, base));
+          sum[e & 3] += s[n][e];
         }
-    }
-    float top = -INFINITY;
+      l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
 #pragma unroll
-    for (int e = 0; e < 16; ++e) top = fmaxf(fmaxf(top, s[0][e]), s[NS - 1][e]);
-    top = half_max(top) * a.scale_log2;
-    // The exponentials are taken relative to a maximum that may lag behind by kSlack: any reference gives
-    // the same result, and moving it costs a pass over the output, which now is rare.
-    if (__any(top > m + kSlack)) {
-      const float old = m;
-      m = fmaxf(m, top);
-      const float shrink = m == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(old - m);
-      l *= shrink;
+      for (int ks = 0; ks < kMine / 16; ++ks) {
+        float pr[8];
 #pragma unroll
-      for (int dt = 0; dt < DT; ++dt)
-#pragma unroll
-        for (int e = 0; e < 16; ++e) o[dt][e] *= shrink;
-    }
-    const float base = m == -INFINITY ? 0.f : ProbShift<T>::forward - m;   // -inf: the row has seen nothing yet
-    float sum[4] = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-    for (int n = 0; n < NS; ++n)
-#pragma unroll
-      for (int e = 0; e < 16; ++e) {
-        s[n][e] = __builtin_amdgcn_exp2f(fmaf(s[n][e], a.scale_log2, base));
-        sum[e & 3] += s[n][e];
+        for (int e = 0; e < 8; ++e) pr[e] = s[ks >> 1][(ks & 1) * 8 + e];
+        const F pf = Frag<T>::pack(pr);
+        Frag<T>::mma_all([&](int dt) { return L::cols_frag(lr, kTileBytes, ks * 16, dt); }, pf, o);
+        if constexpr (decltype(exact)::value)
+          Frag<T>::mma_all([&](int dt) { return L::cols_frag(lr, kTileBytes, ks * 16, dt); }, low_part<T>(pr), o);
       }
-    l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
-#pragma unroll
-    for (int ks = 0; ks < kMine / 16; ++ks) {
-      float pr[8];
-#pragma unroll
-      for (int e = 0; e < 8; ++e) pr[e] = s[ks >> 1][(ks & 1) * 8 + e];
-      const F pf = Frag<T>::pack(pr);
-      Frag<T>::mma_all([&](int dt) { return L::cols_frag(lr, kTileBytes, ks * 16, dt); }, pf, o);
     }
+  };
+  if constexpr (sizeof(T) == 2) {
+    if (min(row0 + kRows, live_rows) <= rows_that_see(a, seq, kFewKeys)) walk_keys(std::true_type());
+    else walk_keys(std::false_type());
+  } else {
+    walk_keys(std::false_type());
   }
 
   l = half_sum(l);

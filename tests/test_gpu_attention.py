@@ -352,3 +352,47 @@ def test_long_cache_offsets() -> None:
 def test_wide_heads_in_full_precision(batch, heads, kv_heads, rows, keys, dim, window, lengths) -> None:
     tensors = inputs(batch, heads, kv_heads, rows, keys, dim, torch.float32)
     check(*tensors, lengths=None if lengths is None else torch.tensor(lengths[:batch]), window=window, sinks=3)
+
+
+@pytest.mark.parametrize('dtype', DTYPES)
+@pytest.mark.parametrize('tokens, causal, window, lengths', [(1, True, None, None), (1, False, 3, None), (300, True, 1, None),
+                                                             (300, False, 1, [300, 0, 77]), (70, False, None, [1, 0, 1])])
+def test_single_keys(tokens, causal, window, lengths, dtype) -> None:
+    """A token that sees one key has its value as output, whatever queries and keys are: their gradients are zeros."""
+    batch = 3 if lengths else 2
+    q, k, v, dout = (t.cuda() for t in inputs(batch, 6, 2, tokens, tokens, 40, dtype))
+    counts = torch.tensor(lengths or [tokens] * batch, device='cuda')
+    leaves = [t.requires_grad_() for t in (q, k, v)]
+    out = attorch_amd.WindowAttention(causal=causal, window=window)(*leaves, counts)
+    dq, dk, dv = torch.autograd.grad(out, leaves, dout)
+    live = (torch.arange(tokens, device='cuda') < counts[:, None])[:, None, :, None]
+    # the probability is within 2^-21 of 1, which is less than half a step of 16 bits and a few steps of 32
+    same = v.detach().repeat_interleave(3, 1).float() * live
+    steps = 0.5 if dtype is not torch.float32 else 8
+    assert ((out.float() - same).abs() <= steps * torch.finfo(dtype).eps * same.abs()).all()
+    assert not dq.any() and not dk.any()
+    summed = (dout.double() * live).unflatten(1, (2, 3))
+    error = (dv.double() - summed.sum(2)).abs()
+    # probabilities and the result are rounded, and three terms added in fp32
+    assert (error <= (torch.finfo(dtype).eps + 2.0 ** -20) * summed.abs().sum(2)).all()
+
+
+@pytest.mark.parametrize('dtype', [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize('batch, tokens, window', [(40, 13, None), (100, 4, 3), (4, 256, None), (2, 512, None), (2, 700, 20)])
+def test_gradients_of_rows_with_few_keys_keep_their_precision(batch, tokens, window, dtype) -> None:
+    """
+    Gradients of queries and keys are rounded twice, as ds and at the end: sqrt(2) times as far off as by
+    the last rounding alone, and up to 1.5 times where few large terms make up a sum.  An output of rounded
+    probabilities would add a third one through delta (1.5 to 2 times).
+    """
+    q, k, v, dout = inputs(batch, 4, 4, tokens, tokens, 64, dtype)
+    leaves = [t.double().requires_grad_() for t in (q, k, v)]
+    scores = leaves[0] @ leaves[1].transpose(2, 3) / 8.0
+    distance = torch.arange(tokens)[:, None] - torch.arange(tokens)
+    seen = (distance >= 0) & (distance < (window or tokens))
+    expected = torch.autograd.grad(scores.masked_fill(~seen, float('-inf')).softmax(-1) @ leaves[2], leaves, dout.double())
+    ours = [t.cuda().requires_grad_() for t in (q, k, v)]
+    got = torch.autograd.grad(attorch_amd.WindowAttention(window=window)(*ours), ours, dout.cuda())
+    for name, a, b in zip(('query', 'key'), got, expected):
+        once = (b.to(dtype).double() - b).norm()
+        assert (a.cpu().double() - b).norm() <= 1.5 * once, name
