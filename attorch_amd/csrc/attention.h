@@ -82,10 +82,11 @@ __device__ __forceinline__ int rows_that_see(const AttentionArgs& a, const Seque
   if (s.len <= most || a.left + a.right + a.sinks < most) return a.rows * a.group;
   return a.causal ? max(most - s.start, 0) * a.group : 0;
 }
-// Rows that see no more keys than this form their output without rounding the probabilities: the sum
-// of few roundings does not average out, and through delta it reaches all of a row's gradients (13 tokens in
-// bf16: dq 2.0 times as far off as its own rounding alone, 1.4 times with exact outputs; 512 tokens 1.52 and
-// 1.44 times).  Beyond it, a second product for all keys would cost a third of the forward pass.
+// Rows that see no more keys than this form their output and gradients without rounding the probabilities
+// and ds: the sum of few roundings does not average out, and an output's reaches all of a row's gradients
+// through delta (13 tokens in bf16: dq 2.0 times as far off as its own rounding alone, 512 tokens 1.52 times;
+// with exact outputs 1.4, with ds exact too 1.0 and 1.4 times).  Beyond it, second products for all keys would cost
+// a quarter of a step.  dk and dv go by the extents: all rows see few keys, or none is treated so.
 constexpr int kFewKeys = 128;
 
 // The keys of a range as one list, which is walked over in tiles: place v of the list is key v for the

@@ -24,6 +24,8 @@
 // over 2 x 8192 tokens, 32 heads on 8: 0.47 and 0.59 ms, 820 and 880 TFLOP/s.  fp32, 777 patches: 50 and
 // 57 us, 74 and 86 of the 139 TFLOP/s that a large product reaches.  (One launch that adds dq with atomics
 // would save a product of the scores and lose the fixed order.)
+#include <type_traits>
+
 #include "attention.h"
 
 namespace at_hip {
@@ -131,47 +133,58 @@ __global__ __launch_bounds__(kWaves * 64, (kPerCu<T, DT>)) void attention_dq_ker
   };
 
   if (tiles > 0) fetch(0, lds);
-  for (int t = 0; t < tiles; ++t) {
-    char* stage = lds + (t & 1) * 2 * kTileBytes;
-    lds_dma_wait_all();
-    __syncthreads();
-    if (t + 1 < tiles) fetch(t + 1, lds + ((t + 1) & 1) * 2 * kTileBytes);
-    // the wave's part of the tile: places v0 ..; behind the sinks these are the keys k0 ..
-    const int v0 = t * kStep + wave_key, k0 = v0 + walk.shift;
-    const bool mixed = t * kStep < walk.begin;
-    if (last < first || !(mixed || (k0 < mine.hi && k0 + kMine > mine.lo) || k0 < mine.sinks)) continue;
-    const bool whole = !mixed && k0 >= last - a.left && k0 + kMine - 1 <= min(first + a.right, seq.len - 1);
+  // exact: ds goes into the product with what its rounding leaves over (see kFewKeys)
+  auto go = [&](auto exact) {
+    for (int t = 0; t < tiles; ++t) {
+      char* stage = lds + (t & 1) * 2 * kTileBytes;
+      lds_dma_wait_all();
+      __syncthreads();
+      if (t + 1 < tiles) fetch(t + 1, lds + ((t + 1) & 1) * 2 * kTileBytes);
+      // the wave's part of the tile: places v0 ..; behind the sinks these are the keys k0 ..
+      const int v0 = t * kStep + wave_key, k0 = v0 + walk.shift;
+      const bool mixed = t * kStep < walk.begin;
+      if (last < first || !(mixed || (k0 < mine.hi && k0 + kMine > mine.lo) || k0 < mine.sinks)) continue;
+      const bool whole = !mixed && k0 >= last - a.left && k0 + kMine - 1 <= min(first + a.right, seq.len - 1);
 
-    const typename L::Reader lr = L::reader(stage + wave_key * L::kPitch);
+      const typename L::Reader lr = L::reader(stage + wave_key * L::kPitch);
 #pragma unroll
-    for (int n = 0; n < kMine / 32; ++n) {
-      f32x16 s = zero_acc(), dp = zero_acc();
+      for (int n = 0; n < kMine / 32; ++n) {
+        f32x16 s = zero_acc(), dp = zero_acc();
 #pragma unroll
-      for (int ks = 0; ks < L::kSteps; ++ks) {
-        Frag<T>::mma2(L::rows_frag(lr, 0, n * 32, ks), qf[ks], s, L::rows_frag(lr, kTileBytes, n * 32, ks), df[ks], dp);
-      }
+        for (int ks = 0; ks < L::kSteps; ++ks) {
+          Frag<T>::mma2(L::rows_frag(lr, 0, n * 32, ks), qf[ks], s, L::rows_frag(lr, kTileBytes, n * 32, ks), df[ks], dp);
+        }
 #pragma unroll
-      for (int e = 0; e < 16; ++e)
-        s[e] = __builtin_amdgcn_exp2f(fmaf(s[e], a.scale_log2, -lse)) * (dp[e] - delta);
-      if (!whole) {
-        int v = v0 + n * 32 + half * 4;
-        asm volatile("" : "+v"(v));      // a branch: as selects the masks would be formed for every tile
-        const int lo = max(see_lo - walk.shift, walk.begin) - v, hi = see_hi - walk.shift - v, sinks = see_sinks - v;
+        for (int e = 0; e < 16; ++e)
+          s[e] = __builtin_amdgcn_exp2f(fmaf(s[e], a.scale_log2, -lse)) * (dp[e] - delta);
+        if (!whole) {
+          int v = v0 + n * 32 + half * 4;
+          asm volatile("" : "+v"(v));      // a branch: as selects the masks would be formed for every tile
+          const int lo = max(see_lo - walk.shift, walk.begin) - v, hi = see_hi - walk.shift - v, sinks = see_sinks - v;
 #pragma unroll
-        for (int e = 0; e < 16; ++e) {
-          const int c = acc_row(e, 0);
-          s[e] = (c >= lo && c <= hi) || c < sinks ? s[e] : 0.f;
+          for (int e = 0; e < 16; ++e) {
+            const int c = acc_row(e, 0);
+            s[e] = (c >= lo && c <= hi) || c < sinks ? s[e] : 0.f;
+          }
+        }
+#pragma unroll
+        for (int t16 = 0; t16 < 2; ++t16) {
+          float x[8];
+#pragma unroll
+          for (int e = 0; e < 8; ++e) x[e] = s[t16 * 8 + e];
+          const F ds = Frag<T>::pack(x);
+          Frag<T>::mma_all([&](int dt) { return L::cols_frag(lr, 0, n * 32 + t16 * 16, dt); }, ds, dq);
+          if constexpr (decltype(exact)::value)
+            Frag<T>::mma_all([&](int dt) { return L::cols_frag(lr, 0, n * 32 + t16 * 16, dt); }, low_part<T>(x), dq);
         }
       }
-#pragma unroll
-      for (int t16 = 0; t16 < 2; ++t16) {
-        float x[8];
-#pragma unroll
-        for (int e = 0; e < 8; ++e) x[e] = s[t16 * 8 + e];
-        const F ds = Frag<T>::pack(x);
-        Frag<T>::mma_all([&](int dt) { return L::cols_frag(lr, 0, n * 32 + t16 * 16, dt); }, ds, dq);
-      }
     }
+  };
+  if constexpr (sizeof(T) == 2) {
+    if (min(row0 + kRows, live_rows) <= rows_that_see(a, seq, kFewKeys)) go(std::true_type());
+    else go(std::false_type());
+  } else {
+    go(std::false_type());
   }
 
   if constexpr (WK > 1) {              // join the two halves of the keys
@@ -276,7 +289,8 @@ __device__ __forceinline__ int wave_min(int v) {
 // A wave owns 32 keys, whose keys and values stay in registers as operands, and walks over the rows that
 // see them.  Of the rows that see sinks only, the waves of a workgroup share the walk instead: those with
 // the same 32 keys take every second or fourth 32 rows (see chunk_plan for how the results are summed).
-template <typename T, int DT>
+// EXACT: ds goes into the product with what its rounding leaves over (see kFewKeys).
+template <typename T, int DT, bool EXACT>
 __global__ __launch_bounds__(kWaves * 64, (kPerCu<T, DT>)) void attention_dkv_kernel(AttentionArgs a) {
   typedef Tile<T, DT> L;
   typedef typename Frag<T>::type F;
@@ -430,6 +444,8 @@ __global__ __launch_bounds__(kWaves * 64, (kPerCu<T, DT>)) void attention_dkv_ke
           Frag<T>::mma2(L::cols_frag(lr, kTileBytes, n * 32 + t16 * 16, dt), pf, dv[dt],
                         L::cols_frag(lr, 0, n * 32 + t16 * 16, dt), df, dk[dt]);
         }
+        if constexpr (EXACT)
+          Frag<T>::mma_all([&](int dt) { return L::cols_frag(lr, 0, n * 32 + t16 * 16, dt); }, low_part<T>(y), dk);
       }
     }
   }
@@ -604,7 +620,14 @@ int launch(AttentionArgs a, hipStream_t stream) {
     rc = launch_status();
     if (rc != AT_OK) return rc;
   }
-  hipLaunchKernelGGL((attention_dkv_kernel<T, DT>), dim3((unsigned)pieces), dim3(kWaves * 64), 0, stream, a);
+  if constexpr (sizeof(T) == 2) {        // kernels of their own: with both in one the registers do not suffice
+    if (a.keys <= kFewKeys || a.left + a.right + a.sinks < kFewKeys)
+      hipLaunchKernelGGL((attention_dkv_kernel<T, DT, true>), dim3((unsigned)pieces), dim3(kWaves * 64), 0, stream, a);
+    else
+      hipLaunchKernelGGL((attention_dkv_kernel<T, DT, false>), dim3((unsigned)pieces), dim3(kWaves * 64), 0, stream, a);
+  } else {
+    hipLaunchKernelGGL((attention_dkv_kernel<T, DT, false>), dim3((unsigned)pieces), dim3(kWaves * 64), 0, stream, a);
+  }
   rc = launch_status();
   if (rc != AT_OK || joined == 0) return rc;
   if (a.chunks > 1)                    // whole tiles of keys: a multiple of 8 of them

@@ -129,7 +129,7 @@ __global__ __launch_bounds__(kWaves * 64, (KEYS == 32 ? 2 : kPerCu<T, DT>)) void
   };
 
   if (t_begin < t_end) fetch(t_begin, lds);
-  // EXACT: the second product takes what the rounding of the probabilities leaves over as well (see kFewKeys)
+  // exact: the second product takes what the rounding of the probabilities leaves over as well (see kFewKeys)
   auto walk_keys = [&](auto exact) {
     for (int t = t_begin; t < t_end; ++t) {
       char* stage = lds + ((t - t_begin) & 1) * 2 * kTileBytes;
