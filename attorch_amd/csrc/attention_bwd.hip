@@ -15,7 +15,8 @@
 // to the inputs' type, as operands of the matrix cores, and ds without scale, which the sums get in fp32.
 // ds of fp16 inputs has output_grad's magnitude, so it is no larger than what the caller's loss scaling
 // already keeps in range, and its small values lose what gradients stored in fp16 lose.  Rows that see a
-// single key have zeros as ds by definition, not what p and delta's roundings would leave.
+// single key have zeros as ds by definition, not what p and delta's roundings would leave (dq: all such rows;
+// dk: where all rows see few keys, so that nothing larger is added).
 //
 // Both kernels are built as the forward kernel is: a lane holds a row (first) or a key (second) of each
 // result, which then is the next product's operand as it stands.  They are bound by the matrix cores, three
@@ -289,7 +290,8 @@ __device__ __forceinline__ int wave_min(int v) {
 // A wave owns 32 keys, whose keys and values stay in registers as operands, and walks over the rows that
 // see them.  Of the rows that see sinks only, the waves of a workgroup share the walk instead: those with
 // the same 32 keys take every second or fourth 32 rows (see chunk_plan for how the results are summed).
-// EXACT: ds goes into the product with what its rounding leaves over (see kFewKeys).
+// EXACT: ds goes into the product with what its rounding leaves over (see kFewKeys), and is zero for rows that see
+// a single key.
 template <typename T, int DT, bool EXACT>
 __global__ __launch_bounds__(kWaves * 64, (kPerCu<T, DT>)) void attention_dkv_kernel(AttentionArgs a) {
   typedef Tile<T, DT> L;
@@ -424,7 +426,7 @@ __global__ __launch_bounds__(kWaves * 64, (kPerCu<T, DT>)) void attention_dkv_ke
           s[e] = seen ? s[e] : 0.f;
           dp[e] = seen ? dp[e] : 0.f;
         }
-        if (r0 < single) {               // probabilities of 1, whatever the key
+        if (EXACT && r0 < single) {      // probabilities of 1, whatever the key
 #pragma unroll
           for (int e = 0; e < 16; ++e) dp[e] = row + acc_row(e, 0) < single ? 0.f : dp[e];
         }
@@ -444,7 +446,7 @@ __global__ __launch_bounds__(kWaves * 64, (kPerCu<T, DT>)) void attention_dkv_ke
           Frag<T>::mma2(L::cols_frag(lr, kTileBytes, n * 32 + t16 * 16, dt), pf, dv[dt],
                         L::cols_frag(lr, 0, n * 32 + t16 * 16, dt), df, dk[dt]);
         }
-        if constexpr (EXACT)
+        if constexpr (EXACT && sizeof(T) == 2)
           Frag<T>::mma_all([&](int dt) { return L::cols_frag(lr, 0, n * 32 + t16 * 16, dt); }, low_part<T>(y), dk);
       }
     }
@@ -620,14 +622,11 @@ int launch(AttentionArgs a, hipStream_t stream) {
     rc = launch_status();
     if (rc != AT_OK) return rc;
   }
-  if constexpr (sizeof(T) == 2) {        // kernels of their own: with both in one the registers do not suffice
-    if (a.keys <= kFewKeys || a.left + a.right + a.sinks < kFewKeys)
-      hipLaunchKernelGGL((attention_dkv_kernel<T, DT, true>), dim3((unsigned)pieces), dim3(kWaves * 64), 0, stream, a);
-    else
-      hipLaunchKernelGGL((attention_dkv_kernel<T, DT, false>), dim3((unsigned)pieces), dim3(kWaves * 64), 0, stream, a);
-  } else {
+  // kernels of their own: with both in one the registers do not suffice
+  if (a.keys <= kFewKeys || a.left + a.right + a.sinks < kFewKeys)
+    hipLaunchKernelGGL((attention_dkv_kernel<T, DT, true>), dim3((unsigned)pieces), dim3(kWaves * 64), 0, stream, a);
+  else
     hipLaunchKernelGGL((attention_dkv_kernel<T, DT, false>), dim3((unsigned)pieces), dim3(kWaves * 64), 0, stream, a);
-  }
   rc = launch_status();
   if (rc != AT_OK || joined == 0) return rc;
   if (a.chunks > 1)                    // whole tiles of keys: a multiple of 8 of them
