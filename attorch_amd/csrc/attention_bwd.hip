@@ -586,7 +586,7 @@ void chunk_plan(AttentionArgs& a) {
   }
   a.chunk_steps = (int)steps;
   const int64_t far = cdiv64(rows, kStep) + 1 - steps * a.chunks;
-  a.sink_tiles = a.sinks > 0 && far > 0 ? (int)cdiv64(a.sinks, kTileKeys) : 0;
+  a.sink_tiles = a.sinks > 0 && far > 0 && heads > 0 ? (int)cdiv64(a.sinks, kTileKeys) : 0;   // no heads: an empty batch
   a.far_chunks = a.far_steps = 0;
   if (a.sink_tiles > 0) {
     int64_t n = cdiv64(want, a.sink_tiles * heads);
@@ -655,7 +655,7 @@ extern "C" {
 
 int64_t at_attention_bwd_workspace_bytes(const at_attention_t* shape) {
   AttentionArgs a;
-  if (attention_args(shape, a) != AT_OK || a.keys == 0) return 0;
+  if (attention_args(shape, a) != AT_OK || a.batch == 0 || a.keys == 0) return 0;
   chunk_plan(a);
   return delta_bytes(a) + part_bytes(a);
 }

@@ -145,6 +145,18 @@ def test_attention_codes() -> None:
     assert lib.at_attention_row_pitch(33, 4, 3) == 0
 
 
+@pytest.mark.parametrize('causal', [0, 1])
+@pytest.mark.parametrize('window, sinks', [(0, 0), (20, 0), (20, 4), (20, 300), (0, 4)])
+def test_attention_codes_of_empty_batches(window, sinks, causal) -> None:
+    """No sequence, but rows that reach beyond the window: nothing to do, and no workspace to do it in."""
+    lib = _lib.load()
+    shape = ctypes.byref(attention_shape(batch=0, rows=700, keys=700, window=window, sinks=sinks, causal=causal,
+                                         strides=[11200, 11200, 16] * 8))
+    assert lib.at_attention_fwd_workspace_bytes(shape) == 0 and lib.at_attention_bwd_workspace_bytes(shape) == 0
+    assert lib.at_attention_fwd(shape, *[None] * 9, 0, None) == 0
+    assert lib.at_attention_bwd(shape, *[None] * 13, 0, None) == 0
+
+
 def test_rotary_codes() -> None:
     lib = _lib.load()
     p = ctypes.addressof(ctypes.create_string_buffer(4096))

@@ -236,6 +236,14 @@ def test_empty_calls() -> None:
             assert grad.shape == leaf.shape and not grad.any()
 
 
+@pytest.mark.parametrize('causal', [True, False])
+def test_empty_batches_with_sinks_beyond_the_window(causal) -> None:
+    q, k, v, dout = (t.cuda().requires_grad_() for t in inputs(0, 4, 2, 700, 700, 32, torch.bfloat16))
+    out = attorch_amd.WindowAttention(causal=causal, window=20, num_sinks=4)(q, k, v)
+    for grad, leaf in zip(torch.autograd.grad(out, (q, k, v), dout), (q, k, v)):
+        assert grad.shape == leaf.shape
+
+
 def test_autocast() -> None:
     q, k, v, dout = (t.cuda() for t in inputs(2, 4, 2, 60, 60, 64, torch.float32))
     leaves = [t.requires_grad_() for t in (q, k, v)]
