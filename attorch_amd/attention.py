@@ -114,8 +114,8 @@ class _Plan:
     """
     What a forward call of given layouts and options passes on: nothing in it belongs to a tensor.
     """
-    __slots__ = ('direct', 'shape', 'ref', 'group', 'scale', 'output_shape', 'output_stride', 'rest_bytes', 'kept_bytes',
-                 'workspace_bytes', 'like_inputs', 'grad_strides')
+    __slots__ = ('direct', 'options', 'dtype', 'shape', 'ref', 'group', 'scale', 'output_shape', 'output_stride', 'rest_bytes',
+                 'kept_bytes', 'workspace_bytes', 'like_inputs', 'grad_strides')
 
 
 @functools.lru_cache(maxsize=4096)
@@ -131,6 +131,7 @@ def _forward_plan(query: Layout, key: Layout, value: Layout, lengths: Optional[L
     batch, heads, rows, dim = query[0]
     kv_heads, keys = key[0][1:3]
     plan = _Plan()
+    plan.options, plan.dtype = (causal, window, num_sinks, scale), dtype
     plan.group = heads // kv_heads
     plan.scale = dim ** -0.5 if scale is None else scale
     counts = [c for c in (lengths, query_lengths) if c is not None]
@@ -160,6 +161,28 @@ def _forward_plan(query: Layout, key: Layout, value: Layout, lengths: Optional[L
     return plan
 
 
+def _planned(what: str, query: Tensor, key: Tensor, value: Tensor, lengths: Optional[Tensor],
+             query_lengths: Optional[Tensor], causal: bool, window: Optional[int], num_sinks: int, scale: Optional[float],
+             dtype: torch.dtype) -> Tuple[_Plan, Tensor, Tensor, Tensor, Optional[Tensor], Optional[Tensor]]:
+    """
+    Description of a call and the tensors that it is of: copies of those that the kernels cannot read
+    where they lie.
+    """
+    device = query.get_device()
+    counts = (None if lengths is None else _layout(lengths), None if query_lengths is None else _layout(query_lengths))
+    plan = _forward_plan(_layout(query), _layout(key), _layout(value), *counts, causal, window, num_sinks, scale, dtype, device)
+    _lib.require_same_device(what, query, key, value, lengths, query_lengths)
+    if not plan.direct:
+        query, key, value = (_for_kernel(t, dtype, g) for t, g in ((query, plan.group), (key, 1), (value, 1)))
+        lengths, query_lengths = (None if c is None else c.long().contiguous() for c in (lengths, query_lengths))
+        counts = (None if lengths is None else _layout(lengths), None if query_lengths is None else _layout(query_lengths))
+        plan = _forward_plan(_layout(query), _layout(key), _layout(value), *counts, causal, window, num_sinks, plan.scale, dtype,
+                             device)
+        if not plan.direct:
+            raise RuntimeError(f'{what}: a tile of {query.shape[1]} heads is more than the kernels can address')
+    return plan, query, key, value, lengths, query_lengths
+
+
 @functools.lru_cache(maxsize=4096)
 def _backward_plan(forward: _Plan, output_grad: Layout, dtype: torch.dtype, device: int) -> Optional[Tuple[_Shape, int]]:
     """
@@ -171,6 +194,20 @@ def _backward_plan(forward: _Plan, output_grad: Layout, dtype: torch.dtype, devi
     shape = _Shape.from_buffer_copy(forward.shape)
     shape.strides = (ctypes.c_int64 * 24)(*shape.strides[:12], *_strides(*output_grad[:2]), *forward.grad_strides)
     return shape, _lib.load().at_attention_bwd_workspace_bytes(ctypes.byref(shape))
+
+
+def _stored_output(plan: _Plan, query: Tensor, output: Tensor, kept: Tensor) -> Tuple[Tensor, Tensor]:
+    """
+    The output and what was kept beside it as the forward call stored them.
+    """
+    if (output.device != query.device or kept.device != query.device or output.shape != plan.output_shape or
+            kept.shape != (plan.kept_bytes,) or kept.dtype is not torch.uint8):
+        raise RuntimeError('WindowAttention backward: saved tensors came back on another device or in another shape')
+    if output.stride() != plan.output_stride or output.dtype is not plan.dtype or output.data_ptr() % 16 != 0:
+        output = torch.empty_strided(plan.output_shape, plan.output_stride, device=query.device, dtype=plan.dtype).copy_(output)
+    if kept.stride() != (1,) or kept.data_ptr() % 16 != 0:
+        kept = kept.clone(memory_format=torch.contiguous_format)
+    return output, kept
 
 
 def _gradient_of(tensor: Tensor, like: bool) -> Tensor:
@@ -229,19 +266,9 @@ class WindowAttentionAutoGrad(torch.autograd.Function):
             Output of shape [batch, heads, rows, head_dim], laid out as [batch, rows, heads, head_dim].
         """
         output_dtype = get_output_dtype(query.dtype, autocast='fp16')
-        device = query.get_device()
-        options = (causal, window, num_sinks)
-        counts = (None if lengths is None else _layout(lengths), None if query_lengths is None else _layout(query_lengths))
-        plan = _forward_plan(_layout(query), _layout(key), _layout(value), *counts, *options, scale, output_dtype, device)
-        _lib.require_same_device('WindowAttention', query, key, value, lengths, query_lengths)
-        head_dim = query.shape[3]
-        if not plan.direct:
-            query, key, value = (_for_kernel(t, output_dtype, g) for t, g in ((query, plan.group), (key, 1), (value, 1)))
-            lengths, query_lengths = (None if c is None else c.long().contiguous() for c in (lengths, query_lengths))
-            counts = (None if lengths is None else _layout(lengths),
-                      None if query_lengths is None else _layout(query_lengths))
-            plan = _forward_plan(_layout(query), _layout(key), _layout(value), *counts, *options, plan.scale, output_dtype,
-                                 device)
+        head_dim = query.shape[-1]
+        plan, query, key, value, lengths, query_lengths = _planned(
+            'WindowAttention', query, key, value, lengths, query_lengths, causal, window, num_sinks, scale, output_dtype)
 
         # not as a view: autograd refuses to change those of a Function in place
         output = torch.empty_strided(plan.output_shape, plan.output_stride, device=query.device, dtype=output_dtype)
@@ -286,7 +313,11 @@ class WindowAttentionAutoGrad(torch.autograd.Function):
 
 def _backward(ctx: Any, output_grad: Tensor) -> Tuple[Optional[Tensor], ...]:
     query, key, value, output, kept, lengths, query_lengths = ctx.saved_tensors
+    # hooks may return saved tensors in other layouts than they were saved in
     forward = ctx.plan
+    forward, query, key, value, lengths, query_lengths = _planned(
+        'WindowAttention backward', query, key, value, lengths, query_lengths, *forward.options, forward.dtype)
+    output, kept = _stored_output(forward, query, output, kept)
     device = query.get_device()
     if output_grad.get_device() != device:
         _lib.require_same_device('WindowAttention backward', query, output_grad)
@@ -294,6 +325,8 @@ def _backward(ctx: Any, output_grad: Tensor) -> Tuple[Optional[Tensor], ...]:
     if plan is None:
         output_grad = _for_kernel(output_grad, query.dtype, forward.group)
         plan = _backward_plan(forward, _layout(output_grad), query.dtype, device)
+        if plan is None:
+            raise RuntimeError(f'WindowAttention backward: a tile of {query.shape[1]} heads is more than the kernels can address')
     shape, workspace_bytes = plan
     like = forward.like_inputs
     query_grad, key_grad, value_grad = \

@@ -258,6 +258,35 @@ def test_autocast() -> None:
         assert grad.dtype is torch.float32 and torch.equal(grad, other.float())
 
 
+def laid_out_anew(tensor):
+    """Equal values, contiguous and then in every second place."""
+    return torch.stack([tensor, torch.zeros_like(tensor)], -1).contiguous()[..., 0]
+
+
+@pytest.mark.parametrize('dtype', DTYPES)
+@pytest.mark.parametrize('dim', [32, 20])
+@pytest.mark.parametrize('hook', [
+    lambda: torch.autograd.graph.save_on_cpu(), lambda: torch.autograd.graph.save_on_cpu(pin_memory=True),
+    lambda: torch.autograd.graph.saved_tensors_hooks(lambda t: t.detach().clone(memory_format=torch.contiguous_format),
+                                                     lambda t: t),
+    lambda: torch.autograd.graph.saved_tensors_hooks(lambda t: t.detach(), laid_out_anew)])
+def test_saved_tensors_in_another_layout(hook, dim, dtype) -> None:
+    """Saved tensors that hooks return with other strides (as offloading them does) give the same gradients."""
+    q, k, v, dout = inputs(2, 4, 2, 70, 70, dim, dtype)
+    packed = torch.cat([t.transpose(1, 2).flatten(2) for t in (q, k, v)], -1).cuda()
+    views = [t.unflatten(2, (-1, dim)).transpose(1, 2) for t in packed.split([4 * dim, 2 * dim, 2 * dim], -1)]
+    lengths = torch.tensor([70, 33], device='cuda')
+    layer = attorch_amd.WindowAttention(window=20, num_sinks=2)
+    for variant in (views, [t.cuda() for t in (q, k, v)], [t.contiguous().cuda() for t in (q, k, v)]):
+        leaves = [t.detach().requires_grad_() for t in variant]
+        out = layer(*leaves, lengths)
+        expected = torch.autograd.grad(out, leaves, dout.cuda())
+        with hook():
+            out = layer(*leaves, lengths)
+        for got, want in zip(torch.autograd.grad(out, leaves, dout.cuda()), expected):
+            assert torch.equal(got, want)
+
+
 def test_frozen_inputs_and_no_grad() -> None:
     q, k, v, dout = (t.cuda() for t in inputs(1, 2, 2, 40, 40, 32, torch.float16))
     leaves = [t.detach().requires_grad_() for t in (q, k, v)]
