@@ -129,6 +129,10 @@ def _rotate(query: Optional[Tensor], key: Optional[Tensor], positions: Optional[
     """
     Turns the queries and keys (either may be absent) by their positions' angles, or back.
     """
+    if not inv_freq.is_contiguous():
+        inv_freq = inv_freq.contiguous()
+    if pair_axis is not None and not pair_axis.is_contiguous():
+        pair_axis = pair_axis.contiguous()
     tables = (None if positions is None else _layout(positions), _layout(inv_freq),
               None if pair_axis is None else _layout(pair_axis), adjacent, inverse)
     shape = _plan(None if query is None else _layout(query), None if key is None else _layout(key), *tables)
@@ -182,11 +186,6 @@ class RotaryAutoGrad(torch.autograd.Function):
         """
         if ctx.needs_input_grad[2] or ctx.needs_input_grad[3]:
             raise RuntimeError('Rotary has no gradients of positions and inv_freq; detach them')
-        if not inv_freq.is_contiguous():
-            inv_freq = inv_freq.contiguous()
-        if pair_axis is not None and not pair_axis.is_contiguous():
-            pair_axis = pair_axis.contiguous()
-
         adjacent = bool(adjacent)
         outputs = _rotate(query, key, positions, inv_freq, pair_axis, adjacent, False)
         ctx.adjacent = adjacent

@@ -1,5 +1,5 @@
 """
-CPU-only tests of what the attention layer passes to the C entry points when saved tensors
+CPU-only tests of what the attention and rotary layers pass to the C entry points when saved tensors
 come back in another layout than they were saved in, as saved-tensor hooks may return them: the entry
 points are replaced by ones that follow every stride on the host.
 """
@@ -30,6 +30,9 @@ class Recorder:
     def at_attention_fwd(self, shape, q, k, v, lengths, query_lengths, out, *_):
         values = torch.randn(BATCH * HEADS * TOKENS * DIM, generator=torch.Generator().manual_seed(2)).to(self.dtype)
         ctypes.memmove(out, values.data_ptr(), values.nbytes)
+        return 0
+
+    def at_rotary(self, *_):
         return 0
 
 
@@ -142,3 +145,31 @@ def test_attention_follows_the_layouts_that_come_back(relay, packed, dtype, reco
     grads = torch.autograd.grad(out, leaves, dout)
     for grad, leaf, value in zip(grads, leaves, (1.0, 2.0, 3.0)):
         assert grad.shape == leaf.shape and (grad == value).all()
+
+
+@pytest.mark.parametrize('relay', [contiguous, spread])
+def test_rotary_follows_the_layouts_that_come_back(relay, recorder) -> None:
+    q, k, _ = projections(torch.float32, True)
+    inv_freq = torch.rand(8, dtype=torch.float64)
+    pair_axis = torch.arange(8, dtype=torch.int32) % 2
+    positions = torch.arange(2 * BATCH * TOKENS).view(2, BATCH, TOKENS)
+    alive = Kept()
+    with hooks(alive.unpack(relay)):
+        outs = attorch_amd.RotaryAutoGrad.apply(q, k, positions, inv_freq, pair_axis)
+    seen = []
+
+    def inverse(shape, *args):
+        shape = shape._obj
+        assert shape.inverse
+        _, _, _, _, at, freq, axis, _ = args
+        read = [[[ctypes.c_int64.from_address(at + 8 * sum(i * s for i, s in zip((x, b, t), shape.position_strides))).value
+                  for t in range(TOKENS)] for b in range(BATCH)] for x in range(2)]
+        assert read == positions.tolist()
+        assert list((ctypes.c_double * 8).from_address(freq)) == inv_freq.tolist()
+        assert list((ctypes.c_int32 * 8).from_address(axis)) == pair_axis.tolist()
+        seen.append(True)
+        return 0
+
+    recorder.at_rotary = inverse
+    torch.autograd.grad(outs, (q, k), [torch.ones_like(t) for t in outs])
+    assert seen
