@@ -202,7 +202,8 @@ __global__ __launch_bounds__(kWaves * 64, (kPerCu<T, DT>)) void attention_dq_ker
       for (int e = 0; e < 16; ++e) dq[dt][e] += X::get(room, dt * 16 + e);
   }
   if (row >= all_rows) return;
-  if (row < rows_that_see(a, seq, 1)) {   // the only key's probability is 1, whatever the query
+  // the only key's probability is 1, whatever the query; and beside a padded row whole tiles were not masked
+  if (!valid || row < rows_that_see(a, seq, 1)) {
 #pragma unroll
     for (int dt = 0; dt < DT; ++dt) dq[dt] = zero_acc();
   }

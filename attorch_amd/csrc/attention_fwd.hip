@@ -230,12 +230,12 @@ __global__ __launch_bounds__(kWaves * 64, (KEYS == 32 ? 2 : kPerCu<T, DT>)) void
 #pragma unroll
       for (int e = 0; e < 16; ++e) o[dt][e] = o[dt][e] * w0 + X::get(room, 2 + dt * 16 + e) * w1;
   }
-  const float inv = l > 0.f ? 1.f / l : l == 0.f ? 0.f : l;
-  if (!valid) {          // a padded row, beside which whole tiles were not masked
+  if (!valid) {          // a padded row, beside which whole tiles were not masked: anything, NaN where keys are not finite
     l = 0.f;
 #pragma unroll
     for (int dt = 0; dt < DT; ++dt) o[dt] = zero_acc();
   }
+  const float inv = l > 0.f ? 1.f / l : l == 0.f ? 0.f : l;
   const float lse = valid ? m + __builtin_amdgcn_logf(l) - ProbShift<T>::forward : INFINITY;
   if (a.splits > 1) {
     if (row >= all_rows) return;
