@@ -476,6 +476,7 @@ __global__ __launch_bounds__(kWaves * 64, (kPerCu<T, DT>)) void attention_dkv_ke
     if (share > 0) return;
   }
 
+  const bool seen = row_lo <= row_hi;  // otherwise the sums hold 0 times rows, NaN where these are not finite
   const float dv_scale = ProbShift<T>::backward != 0.f ? 1.f / 32768.f : 1.f;
   const bool partial = a.chunks > 1 || (piece.tile < a.sink_tiles && subtile * 32 < far_keys(a, piece.tile));
   float* part = a.part + (int64_t)(wave * 32 + (lane & 31)) * a.dim +
@@ -491,8 +492,8 @@ __global__ __launch_bounds__(kWaves * 64, (kPerCu<T, DT>)) void attention_dkv_ke
       float x[4], y[4];
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
-        x[j] = dk[dt][q * 4 + j] * a.scale;
-        y[j] = dv[dt][q * 4 + j] * dv_scale;
+        x[j] = seen ? dk[dt][q * 4 + j] * a.scale : 0.f;
+        y[j] = seen ? dv[dt][q * 4 + j] * dv_scale : 0.f;
       }
       if (d >= a.dim) continue;
       if (partial) {                   // one of several partial sums

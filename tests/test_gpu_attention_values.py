@@ -39,3 +39,32 @@ def test_padded_rows_beside_keys_and_values_that_are_not_finite(bad, rows, keys,
             x = x.detach().cpu().transpose(1, 2)
             assert (x[padded] == 0).all(), (name, place)
             assert not torch.isfinite(x[~padded]).all()
+
+
+@pytest.mark.parametrize('dtype', DTYPES)
+@pytest.mark.parametrize('causal', [True, False])
+@pytest.mark.parametrize('heads, kv_heads', [(3, 1), (24, 24)])
+@pytest.mark.parametrize('rows, keys, lengths, query_lengths', PADDED)
+@pytest.mark.parametrize('window, sinks', [(None, 0), (40, 3)])
+@pytest.mark.parametrize('bad', [NAN, INF])
+def test_unseen_keys_beside_rows_that_are_not_finite(bad, window, sinks, rows, keys, lengths, query_lengths, heads, kv_heads, causal,
+                                                     dtype) -> None:
+    counts = torch.tensor(lengths)
+    query_counts = torch.tensor(query_lengths) if query_lengths else counts.clamp(max=rows)
+    start = (counts - query_counts).clamp(min=0)
+    key = torch.arange(keys)
+    unseen = key >= counts[:, None]
+    if window:
+        unseen |= (key >= sinks) & (key <= (start - window)[:, None])
+    for place in (0, 3):
+        tensors = list(inputs(3, heads, kv_heads, rows, keys, 64, dtype))
+        tensors[place][:, :, 0] = bad       # a row of every sequence that is a token
+        q, k, v, dout = (t.cuda() for t in tensors)
+        leaves = [t.requires_grad_() for t in (q, k, v)]
+        out = attorch_amd.WindowAttention(causal=causal, window=window, num_sinks=sinks)(
+            *leaves, counts.cuda(), query_counts.cuda() if query_lengths else None)
+        _, dk, dv = torch.autograd.grad(out, leaves, dout)
+        for name, x in (('key gradient', dk), ('value gradient', dv)):
+            x = x.cpu().transpose(1, 2)
+            assert (x[unseen] == 0).all(), (name, place)
+        assert not torch.isfinite(x[~unseen]).all()
