@@ -215,6 +215,32 @@ constexpr float kSlack = 8.f;
 template <typename T> struct ProbShift { static constexpr float forward = 0.f, backward = 0.f; };
 template <> struct ProbShift<f16_t> { static constexpr float forward = 15.f - kSlack, backward = 15.f; };
 
+// ds of fp16 inputs carries a factor of its own into its rounding, the same power of two for all terms of a sum (a
+// row's of dq, a key's of dk), which leaves the sum in fp32: 2^ProbShift::backward at first, lowered where a
+// term would leave fp16's range, so neither small output gradients over many keys (ds is their size
+// times a probability) nor large ones are lost while the sums themselves fit fp16.  As it stands, ds would be subnormal
+// below 6e-5: dq of 4096 tokens was 3 to 7 times as far off as its last rounding alone with output gradients of 1e-3,
+// and infinite where ds passed 65504.  Looking for the largest term costs up to 2 % of a step (8 x 512 tokens, 16 heads of
+// 64: 77.2 -> 78.5 us; 4 x 4096, 32 heads of 64: 1486 -> 1508 us; of 128: none).
+// The factor that brings terms of magnitude `top` > kDsLimit down to [2^12, 2^13), and its exponent.
+constexpr float kDsLimit = 32768.f;
+struct DsFactor {
+  float value, log2;
+};
+__device__ __forceinline__ DsFactor ds_factor(float top) {
+  if (!(top > kDsLimit)) return {1.f, 0.f};
+  const int exponent = 12 + 127 - (int)(__float_as_uint(top) >> 23);    // -116 for infinity
+  return {__uint_as_float((unsigned)(exponent + 127) << 23), (float)exponent};
+}
+__device__ __forceinline__ float largest(const f32x16& v) {
+  float top = 0.f;
+#pragma unroll
+  for (int e = 0; e < 16; e += 2) top = fmaxf(fmaxf(top, fabsf(v[e])), fabsf(v[e + 1]));
+  return top;
+}
+// 1 / x of a power of two
+__device__ __forceinline__ float inverse_power(float x) { return __uint_as_float((254u << 23) - __float_as_uint(x)); }
+
 __device__ __forceinline__ f32x16 zero_acc() {
   f32x16 z;
 #pragma unroll

@@ -13,8 +13,7 @@
 // over): an error of delta is common to a whole row of ds, and with the rounded output it was the largest
 // one in dq and dk (bf16, 512 tokens: 2.0e-3 of them against 1.7e-3 for rounding ds).  p and ds are rounded
 // to the inputs' type, as operands of the matrix cores, and ds without scale, which the sums get in fp32.
-// ds of fp16 inputs has output_grad's magnitude, so it is no larger than what the caller's loss scaling
-// already keeps in range, and its small values lose what gradients stored in fp16 lose.  Rows that see a
+// ds of fp16 inputs is multiplied by a power of two before it is rounded (ds_factor).  Rows that see a
 // single key have zeros as ds by definition, not what p and delta's roundings would leave (dq: all such rows;
 // dk: where all rows see few keys, so that nothing larger is added).
 //
@@ -97,6 +96,8 @@ __global__ __launch_bounds__(kWaves * 64, (kPerCu<T, DT>)) void attention_dq_ker
   f32x16 dq[DT];
 #pragma unroll
   for (int dt = 0; dt < DT; ++dt) dq[dt] = zero_acc();
+  constexpr bool kFactor = ProbShift<T>::backward != 0.f;
+  float base = ProbShift<T>::backward - lse, undo = kFactor ? 1.f / 32768.f : 1.f;   // of the row's ds, see ds_factor
 
   const int p = seq.start + i;
   const int see_lo = valid ? p - a.left : 1, see_hi = valid ? min(p + a.right, seq.len - 1) : 0;
@@ -157,7 +158,7 @@ __global__ __launch_bounds__(kWaves * 64, (kPerCu<T, DT>)) void attention_dq_ker
         }
 #pragma unroll
         for (int e = 0; e < 16; ++e)
-          s[e] = __builtin_amdgcn_exp2f(fmaf(s[e], a.scale_log2, -lse)) * (dp[e] - delta);
+          s[e] = __builtin_amdgcn_exp2f(fmaf(s[e], a.scale_log2, base)) * (dp[e] - delta);
         if (!whole) {
           int v = v0 + n * 32 + half * 4;
           asm volatile("" : "+v"(v));      // a branch: as selects the masks would be formed for every tile
@@ -166,6 +167,20 @@ __global__ __launch_bounds__(kWaves * 64, (kPerCu<T, DT>)) void attention_dq_ker
           for (int e = 0; e < 16; ++e) {
             const int c = acc_row(e, 0);
             s[e] = (c >= lo && c <= hi) || c < sinks ? s[e] : 0.f;
+          }
+        }
+        if constexpr (kFactor) {
+          const float top = largest(s);
+          if (__any(top > kDsLimit)) {
+            const DsFactor f = ds_factor(half_max(top));   // both halves of the wave add to a sum
+            base += f.log2;
+            undo *= inverse_power(f.value);
+#pragma unroll
+            for (int e = 0; e < 16; ++e) s[e] *= f.value;
+#pragma unroll
+            for (int dt = 0; dt < DT; ++dt)
+#pragma unroll
+              for (int e = 0; e < 16; ++e) dq[dt][e] *= f.value;
           }
         }
 #pragma unroll
@@ -186,6 +201,12 @@ __global__ __launch_bounds__(kWaves * 64, (kPerCu<T, DT>)) void attention_dq_ker
     else go(std::false_type());
   } else {
     go(std::false_type());
+  }
+  if constexpr (kFactor) {
+#pragma unroll
+    for (int dt = 0; dt < DT; ++dt)
+#pragma unroll
+      for (int e = 0; e < 16; ++e) dq[dt][e] *= undo;
   }
 
   if constexpr (WK > 1) {              // join the two halves of the keys
@@ -345,6 +366,8 @@ __global__ __launch_bounds__(kWaves * 64, (kPerCu<T, DT>)) void attention_dkv_ke
   f32x16 dk[DT], dv[DT];
 #pragma unroll
   for (int dt = 0; dt < DT; ++dt) dk[dt] = dv[dt] = zero_acc();
+  constexpr bool kFactor = ProbShift<T>::backward != 0.f;
+  float factor = 1.f;                  // of the key's ds beside the probabilities' 2^backward, see ds_factor
 
   const char* qb = a.q.p + b * a.q.batch + (int64_t)h * a.group * a.q.head;
   const char* db = a.dout.p + b * a.dout.batch + (int64_t)h * a.group * a.dout.head;
@@ -432,6 +455,21 @@ __global__ __launch_bounds__(kWaves * 64, (kPerCu<T, DT>)) void attention_dkv_ke
           for (int e = 0; e < 16; ++e) dp[e] = row + acc_row(e, 0) < single ? 0.f : dp[e];
         }
       }
+      if constexpr (kFactor) {
+#pragma unroll
+        for (int e = 0; e < 16; ++e) dp[e] *= factor;
+        const float top = largest(dp);
+        if (__any(top > kDsLimit)) {
+          const DsFactor f = ds_factor(half_max(top));   // both halves of the wave add to a sum
+          factor *= f.value;
+#pragma unroll
+          for (int e = 0; e < 16; ++e) dp[e] *= f.value;
+#pragma unroll
+          for (int dt = 0; dt < DT; ++dt)
+#pragma unroll
+            for (int e = 0; e < 16; ++e) dk[dt][e] *= f.value;
+        }
+      }
 #pragma unroll
       for (int t16 = 0; t16 < 2; ++t16) {
         float x[8], y[8];
@@ -439,7 +477,6 @@ __global__ __launch_bounds__(kWaves * 64, (kPerCu<T, DT>)) void attention_dkv_ke
         for (int e = 0; e < 8; ++e) {
           x[e] = s[t16 * 8 + e];
           y[e] = dp[t16 * 8 + e];
-          if (ProbShift<T>::backward != 0.f) y[e] *= 1.f / 32768.f;
         }
         const F pf = Frag<T>::pack(x), df = Frag<T>::pack(y);
 #pragma unroll
@@ -451,6 +488,15 @@ __global__ __launch_bounds__(kWaves * 64, (kPerCu<T, DT>)) void attention_dkv_ke
           Frag<T>::mma_all([&](int dt) { return L::cols_frag(lr, 0, n * 32 + t16 * 16, dt); }, low_part<T>(y), dk);
       }
     }
+  }
+
+  const float dv_scale = kFactor ? 1.f / 32768.f : 1.f;
+  if constexpr (kFactor) {
+    const float undo = dv_scale * inverse_power(factor);
+#pragma unroll
+    for (int dt = 0; dt < DT; ++dt)
+#pragma unroll
+      for (int e = 0; e < 16; ++e) dk[dt][e] *= undo;
   }
 
   if (sharers > 1) {                   // the first wave of each 32 keys takes the others' sums over
@@ -477,7 +523,6 @@ __global__ __launch_bounds__(kWaves * 64, (kPerCu<T, DT>)) void attention_dkv_ke
   }
 
   const bool seen = row_lo <= row_hi;  // otherwise the sums hold 0 times rows, NaN where these are not finite
-  const float dv_scale = ProbShift<T>::backward != 0.f ? 1.f / 32768.f : 1.f;
   const bool partial = a.chunks > 1 || (piece.tile < a.sink_tiles && subtile * 32 < far_keys(a, piece.tile));
   float* part = a.part + (int64_t)(wave * 32 + (lane & 31)) * a.dim +
                 (bh * first_part(a, a.tiles) + first_part(a, piece.tile) + (piece.far ? a.chunks : 0) + piece.chunk) *

@@ -99,7 +99,7 @@ def attention(q: Tensor, k: Tensor, v: Tensor, dout: Optional[Tensor] = None, le
             delta = (D * out).sum(-1, keepdim=True)
             ds = p * (dp - delta)
             d_err = (D.abs() * out_err).sum(-1, keepdim=True) + (dim + 2) * e * (D.abs() * out.abs()).sum(-1, keepdim=True)
-            # a rounded ds is off by half a step; in fp16 small ones are subnormal
+            # a rounded ds is off by half a step, or less than the type's smallest number
             x = (u + eps) * ds.abs() + p * (d_err + (dim + 2) * e * (D.abs() @ V.abs().T)) + seen * _tiny(dtype) + \
                 z * (dp.abs() + delta.abs())
             c = seen.sum(0).double()[:, None]
