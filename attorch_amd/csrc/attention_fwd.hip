@@ -434,7 +434,9 @@ int at_attention_fwd(const at_attention_t* shape, const void* q, const void* k, 
   if (rc != AT_OK) return rc;
   if (a.batch == 0 || a.rows == 0) return AT_OK;
   if (!q || !out || (a.keys > 0 && (!k || !v))) return AT_ERR_NULL;
-  if (!aligned16(q) || !aligned16(k) || !aligned16(v) || !aligned16(out) || (lse && !aligned16(lse)) || !aligned16(out_rest)) return AT_ERR_ALIGN;
+  if (!aligned16(q) || !aligned16(k) || !aligned16(v) || !aligned16(out) || !aligned16(lse) || !aligned16(out_rest) ||
+      !aligned16(workspace))
+    return AT_ERR_ALIGN;
   a.q.p = (char*)q; a.k.p = (char*)k; a.v.p = (char*)v; a.out.p = (char*)out;
   a.lengths = lengths;
   a.query_lengths = query_lengths;

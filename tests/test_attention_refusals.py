@@ -145,6 +145,15 @@ def test_attention_codes() -> None:
     assert lib.at_attention_row_pitch(33, 4, 3) == 0
 
 
+def test_attention_codes_of_misaligned_workspaces() -> None:
+    lib = _lib.load()
+    p = (ctypes.addressof(ctypes.create_string_buffer(4096)) + 63) // 64 * 64
+    cache = ctypes.byref(attention_shape(rows=1, keys=100000))
+    size = lib.at_attention_fwd_workspace_bytes(cache)
+    assert lib.at_attention_fwd(cache, p, p, p, None, None, p, None, None, p + 8, size, None) == -6
+    assert lib.at_attention_bwd(ctypes.byref(attention_shape()), *[p] * 12, p + 8, 1 << 20, None) == -6
+
+
 @pytest.mark.parametrize('causal', [0, 1])
 @pytest.mark.parametrize('window, sinks', [(0, 0), (20, 0), (20, 4), (20, 300), (0, 4)])
 def test_attention_codes_of_empty_batches(window, sinks, causal) -> None:
