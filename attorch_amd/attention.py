@@ -247,7 +247,8 @@ class WindowAttentionAutoGrad(torch.autograd.Function):
         values hold where no query of their sequence sees them reaches no result, NaN included.
 
         Args:
-            query: Queries of shape [batch, heads, rows, head_dim], the last tokens of their sequences.
+            query: Queries of shape [batch, heads, rows, head_dim], the last tokens of their sequences. They,
+                the keys and the values must have one dtype; autocast casts them to its own.
             key: Keys of shape [batch, kv_heads, tokens, head_dim]; kv_heads divides heads, and
                 query head n reads key head n // (heads // kv_heads).
             value: Values, shaped like the keys.
@@ -266,6 +267,8 @@ class WindowAttentionAutoGrad(torch.autograd.Function):
             Output of shape [batch, heads, rows, head_dim], laid out as [batch, rows, heads, head_dim].
         """
         output_dtype = get_output_dtype(query.dtype, autocast='fp16')
+        if not query.dtype is key.dtype is value.dtype is output_dtype and torch.is_autocast_enabled('cuda'):
+            query, key, value = (t.to(output_dtype) for t in (query, key, value))
         head_dim = query.shape[-1]
         plan, query, key, value, lengths, query_lengths = _planned(
             'WindowAttention', query, key, value, lengths, query_lengths, causal, window, num_sinks, scale, output_dtype)

@@ -258,6 +258,24 @@ def test_autocast() -> None:
         assert grad.dtype is torch.float32 and torch.equal(grad, other.float())
 
 
+@pytest.mark.parametrize('dtype', [torch.float16, torch.bfloat16])
+@pytest.mark.parametrize('others', [(torch.float32, torch.float32), (torch.bfloat16, torch.float16),
+                                    (torch.float16, torch.float32)])
+def test_autocast_of_inputs_of_different_types(others, dtype) -> None:
+    """Queries of a projection beside a cache in the weights' type: all are cast, and gradients cast back."""
+    q, k, v, dout = (t.cuda() for t in inputs(2, 4, 2, 60, 60, 64, torch.float32))
+    leaves = [t.to(d).requires_grad_() for t, d in zip((q, k, v), (dtype, *others))]
+    with torch.autocast('cuda', dtype=dtype):
+        out = attorch_amd.WindowAttention(window=30)(*leaves)
+    assert out.dtype is dtype
+    plain = [t.detach().to(dtype).requires_grad_() for t in leaves]
+    same = attorch_amd.WindowAttention(window=30)(*plain)
+    assert torch.equal(out, same)
+    expected = torch.autograd.grad(same, plain, dout.to(dtype))
+    for grad, leaf, other in zip(torch.autograd.grad(out, leaves, dout.to(dtype)), leaves, expected):
+        assert grad.dtype is leaf.dtype and torch.equal(grad, other.to(leaf.dtype))
+
+
 def laid_out_anew(tensor):
     """Equal values, contiguous and then in every second place."""
     return torch.stack([tensor, torch.zeros_like(tensor)], -1).contiguous()[..., 0]
