@@ -13,7 +13,7 @@ pre_act_add of BatchNorm2d) are spelled out as separate torch layers for the lat
 `load_from` copies the parameters of one variant into the other so the two can be compared.
 """
 
-from typing import List, Optional, Tuple
+from typing import List, NamedTuple, Optional, Tuple
 
 import torch
 from torch import Tensor
@@ -123,6 +123,31 @@ class BasicBlock(nn.Module):
             self.downsample.load_from(other.downsample)
 
 
+class NewTokens(NamedTuple):
+    """
+    Where the tokens of a call that continues sequences belong.
+    """
+    positions: Tensor       # [batch, chunk]
+    slots: Tensor           # [batch, chunk] places in the cache, no two of a sequence the same
+    live: Tensor            # [batch, chunk] the others are padding
+    lengths: Tensor
+    query_lengths: Tensor
+
+
+def new_tokens(lengths: Tensor, query_lengths: Optional[Tensor], chunk: int, room: int) -> NewTokens:
+    """
+    The first `query_lengths` of a sequence's `chunk` tokens (None: as many as it has tokens for) are its last
+    ones, the others are padding.  Nothing here waits for the device.
+    """
+    lengths = lengths.long()
+    new = chunk if query_lengths is None else query_lengths.long().clamp(0, chunk)
+    start = (lengths - new).clamp(min=0)
+    new = (lengths - start).clamp(min=0)
+    step = torch.arange(chunk, device=lengths.device)
+    positions = start[:, None] + step
+    return NewTokens(positions, positions % room, step < new[:, None], start + new, new)
+
+
 class TransformerBlock(nn.Module):
     """
     Pre-norm block: x + attention(LN(x)), then + MLP(LN(.)) with a fused Linear+GELU.
@@ -174,7 +199,8 @@ class TransformerBlock(nn.Module):
                                               attn_mask=seen)
 
     def attention(self, input: Tensor, cache: Optional[Tuple[Tensor, Tensor]] = None,
-                  lengths: Optional[Tensor] = None) -> Tensor:
+                  lengths: Optional[Tensor] = None, query_lengths: Optional[Tensor] = None,
+                  new: Optional[NewTokens] = None) -> Tensor:
         batch, seq, dim = input.shape
         if self.plain and cache is None:
             qkv = self.qkv(input).view(batch, seq, 3, self.num_heads, dim // self.num_heads)
@@ -186,22 +212,23 @@ class TransformerBlock(nn.Module):
         if not self.fused:
             out = self._spelled_out(q, k, v)
         else:
-            positions = None
-            if cache is not None:          # the new tokens are the last of each sequence
-                positions = (lengths - seq)[:, None] + torch.arange(seq, device=input.device)
+            if cache is not None and new is None:
+                new = new_tokens(lengths, query_lengths, seq, cache[0].shape[2])
             if self.turn is not None:
-                q, k = self.turn(q, k, positions)
+                q, k = self.turn(q, k, None if cache is None else new.positions)
             if cache is not None:
                 rows = torch.arange(batch, device=input.device)[:, None]
-                for stored, new in zip(cache, (k, v)):
-                    stored[rows, :, positions] = new.transpose(1, 2)
+                for stored, fresh in zip(cache, (k, v)):     # padding rewrites what is there
+                    stored[rows, :, new.slots] = torch.where(new.live[..., None, None], fresh.transpose(1, 2),
+                                                             stored[rows, :, new.slots])
                 k, v = cache
-            out = self.core(q, k, v, lengths)
+                lengths, query_lengths = new.lengths, new.query_lengths
+            out = self.core(q, k, v, lengths, query_lengths)
         return self.proj(out.transpose(1, 2).reshape(batch, seq, dim))
 
-    def forward(self, input: Tensor, cache: Optional[Tuple[Tensor, Tensor]] = None,
-                lengths: Optional[Tensor] = None) -> Tensor:
-        output = input + self.attention(self.ln1(input), cache, lengths)
+    def forward(self, input: Tensor, cache: Optional[Tuple[Tensor, Tensor]] = None, lengths: Optional[Tensor] = None,
+                query_lengths: Optional[Tensor] = None, new: Optional[NewTokens] = None) -> Tensor:
+        output = input + self.attention(self.ln1(input), cache, lengths, query_lengths, new)
         return output + self.fc2(self.fc1(self.ln2(output)))
 
     def load_from(self, other: 'TransformerBlock') -> None:
@@ -248,19 +275,23 @@ class TinyGPT(nn.Module):
         return [tuple(torch.empty(batch, block.kv_heads, max_tokens, block.head_dim, device=weight.device, dtype=weight.dtype)
                       for _ in range(2)) for block in self.blocks]
 
-    def extend(self, tokens: Tensor, cache: List[Tuple[Tensor, Tensor]], lengths: Tensor) -> Tensor:
+    def extend(self, tokens: Tensor, cache: List[Tuple[Tensor, Tensor]], lengths: Tensor,
+               query_lengths: Optional[Tensor] = None) -> Tensor:
         """
-        Logits of new tokens (a prompt, a part of one or single tokens), which are the last ones of
+        Logits of new tokens (prompts, parts of them or single tokens), which are the last ones of
         sequences that have `lengths` tokens with them; their keys and values go into the cache,
-        which must have room for them.  For the fused backend with rotary.
+        which must have room for them.  Of a sequence's row of tokens the first `query_lengths` are
+        new (None: all, or as many as it has tokens in all), the others are padding: they leave
+        the cache as it is, and their logits mean nothing.  For the fused backend with rotary.
         """
         if self.pos_embed is not None or not all(block.fused for block in self.blocks):
             raise RuntimeError('Sequences are continued on attorch_amd.nn and with rotary positions only')
         if tokens.shape[1] > cache[0][0].shape[2]:
             raise RuntimeError(f'The cache has room for {cache[0][0].shape[2]} tokens, received {tokens.shape[1]} new ones')
+        new = new_tokens(lengths, query_lengths, tokens.shape[1], cache[0][0].shape[2])
         output = self.tok_embed(tokens)
         for block, stored in zip(self.blocks, cache):
-            output = block(output, stored, lengths)
+            output = block(output, stored, lengths, query_lengths, new)
         return self.head(self.norm(output))
 
     def load_from(self, other: 'TinyGPT') -> None:

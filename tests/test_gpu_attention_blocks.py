@@ -100,3 +100,42 @@ def test_rotary_and_attention_layers(dtype) -> None:
         assert_within(grad, expected[name], name)
     for grad, inner, name in zip(grads[2:4], grads[:2], ('query', 'key')):
         assert_within(grad, rotary(inner.cpu(), *tables, inverse=True), f'{name} gradient')
+
+
+@pytest.mark.parametrize('int_type', [torch.int32, torch.int64])
+def test_prompts_of_different_lengths(int_type) -> None:
+    """
+    Padded prompts, chunks and single tokens of sequences that all grow at a pace of their own, one of them
+    empty at first, give the logits of the whole sequences, and padding leaves the cache as it is: what was
+    not written is still NaN, and the rest does not change.
+    """
+    torch.manual_seed(3)
+    model = TinyGPT(fused_nn, 500, 2, 128, 4, **OPTIONS).to('cuda')
+    room = 50
+    tokens = torch.randint(0, 500, (4, room), device='cuda')
+    done = [0, 0, 0, 0]
+    with torch.no_grad():
+        whole = model(tokens)
+        cache = model.new_cache(4, room)
+        for pair in cache:
+            for t in pair:
+                t.fill_(float('nan'))
+        # new tokens of each sequence, and whether their numbers are given (otherwise a sequence's length says)
+        for step, counted in (((33, 5, 0, 20), False), ((2, 0, 7, 9), True), ((1, 0, 1, 0), True), ((1, 1, 1, 1), False),
+                              ((0, 40, 3, 12), True), ((13, 4, 1, 8), True)):
+            before = [[t.clone() for t in pair] for pair in cache]
+            chunk = torch.full((4, max(step)), 499, device='cuda')
+            for b, n in enumerate(step):
+                chunk[b, :n] = tokens[b, done[b]:done[b] + n]
+            done = [d + n for d, n in zip(done, step)]
+            lengths = torch.tensor(done, device='cuda', dtype=int_type)
+            logits = model.extend(chunk, cache, lengths,
+                                  torch.tensor(step, device='cuda', dtype=int_type) if counted else None)
+            for b, n in enumerate(step):
+                torch.testing.assert_close(logits[b, :n], whole[b, done[b] - n:done[b]], rtol=1e-4, atol=1e-4)
+            for pair, old in zip(cache, before):
+                for t, o in zip(pair, old):
+                    for b, n in enumerate(step):
+                        assert torch.isfinite(t[b, :, :done[b]]).all() and torch.isnan(t[b, :, done[b]:]).all()
+                        assert torch.equal(t[b, :, :done[b] - n], o[b, :, :done[b] - n])
+    assert done == [50, 50, 13, 50]
