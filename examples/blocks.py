@@ -137,12 +137,12 @@ class NewTokens(NamedTuple):
 def new_tokens(lengths: Tensor, query_lengths: Optional[Tensor], chunk: int, room: int) -> NewTokens:
     """
     The first `query_lengths` of a sequence's `chunk` tokens (None: as many as it has tokens for) are its last
-    ones, the others are padding.  Nothing here waits for the device.
+    ones, the others are padding, and so are tokens that find no room.  Nothing here waits for the device.
     """
     lengths = lengths.long()
     new = chunk if query_lengths is None else query_lengths.long().clamp(0, chunk)
     start = (lengths - new).clamp(min=0)
-    new = (lengths - start).clamp(min=0)
+    new = (lengths.clamp(max=room) - start).clamp(min=0)
     step = torch.arange(chunk, device=lengths.device)
     positions = start[:, None] + step
     return NewTokens(positions, positions % room, step < new[:, None], start + new, new)
@@ -279,10 +279,11 @@ class TinyGPT(nn.Module):
                query_lengths: Optional[Tensor] = None) -> Tensor:
         """
         Logits of new tokens (prompts, parts of them or single tokens), which are the last ones of
-        sequences that have `lengths` tokens with them; their keys and values go into the cache,
-        which must have room for them.  Of a sequence's row of tokens the first `query_lengths` are
-        new (None: all, or as many as it has tokens in all), the others are padding: they leave
-        the cache as it is, and their logits mean nothing.  For the fused backend with rotary.
+        sequences that have `lengths` tokens with them; their keys and values go into the cache.
+        Of a sequence's row of tokens the first `query_lengths` are new (None: all, or as many as it
+        has tokens in all), the others are padding: they leave the cache as it is, and their logits
+        mean nothing.  So do tokens for which the cache has no room left.  For the fused
+        backend with rotary.
         """
         if self.pos_embed is not None or not all(block.fused for block in self.blocks):
             raise RuntimeError('Sequences are continued on attorch_amd.nn and with rotary positions only')

@@ -12,7 +12,7 @@ import attorch_amd
 from attorch_amd import _lib
 from attorch_amd.attention import _Shape as AttentionShape
 from attorch_amd.rotary import _Shape as RotaryShape
-from examples.blocks import TinyGPT
+from examples.blocks import TinyGPT, new_tokens
 
 
 def qkv(batch=2, heads=4, kv_heads=2, rows=5, keys=5, dim=16, dtype=torch.float32):
@@ -71,6 +71,30 @@ def test_continued_sequences_of_other_models() -> None:
         model = TinyGPT(torch.nn, 20, 1, 32, 2, 8, **options)
         with pytest.raises(RuntimeError, match='continued'):
             model.extend(tokens, model.new_cache(1, 8), lengths)
+
+
+@pytest.mark.parametrize('int_type', [torch.int32, torch.int64])
+def test_places_of_new_tokens(int_type) -> None:
+    """
+    Tokens of continued sequences are counted from their starts and stored where the cache has room; the slots of
+    padding are places of the cache too, and a sequence's are all different.
+    """
+    room, chunk = 12, 5
+    lengths = torch.tensor([0, 3, 5, 9, 12, 13, 14, 17, 18, 40, -2], dtype=int_type)
+    for given in (None, 0, 2, 5, 9):
+        counts = None if given is None else torch.full_like(lengths, given)
+        new = new_tokens(lengths, counts, chunk, room)
+        wanted = chunk if given is None else min(given, chunk)
+        for b, length in enumerate(lengths.tolist()):
+            start = max(length - wanted, 0)
+            live = [start + i for i in range(wanted) if start + i < min(length, room)]
+            assert new.positions[b].tolist() == list(range(start, start + chunk))
+            assert new.live[b].tolist() == [i < len(live) for i in range(chunk)]
+            assert new.slots[b][new.live[b]].tolist() == live
+            assert len(set(new.slots[b].tolist())) == chunk and all(0 <= s < room for s in new.slots[b].tolist())
+            assert new.query_lengths[b] == len(live)
+            # as attention places its rows
+            assert not live or (new.lengths[b] - new.query_lengths[b] == start and new.lengths[b] <= room)
 
 
 def test_rotary_arguments() -> None:

@@ -139,3 +139,23 @@ def test_prompts_of_different_lengths(int_type) -> None:
                         assert torch.isfinite(t[b, :, :done[b]]).all() and torch.isnan(t[b, :, done[b]:]).all()
                         assert torch.equal(t[b, :, :done[b] - n], o[b, :, :done[b] - n])
     assert done == [50, 50, 13, 50]
+
+
+def test_sequences_that_fill_the_cache() -> None:
+    """Tokens that find no room change nothing: neither what is stored nor the logits of those that do."""
+    torch.manual_seed(3)
+    model = TinyGPT(fused_nn, 500, 2, 128, 4, **OPTIONS).to('cuda')
+    tokens = torch.randint(0, 500, (3, 40), device='cuda')
+    with torch.no_grad():
+        whole = model(tokens)
+        cache = model.new_cache(3, 32)
+        model.extend(tokens[:, :28], cache, torch.full((3,), 28, device='cuda'))
+        logits = model.extend(tokens[:, 28:36], cache, torch.tensor([36, 32, 30], device='cuda'),
+                              torch.tensor([8, 4, 2], device='cuda'))
+        for b, n in enumerate((4, 4, 2)):
+            torch.testing.assert_close(logits[b, :n], whole[b, 28:28 + n], rtol=1e-4, atol=1e-4)
+        before = [[t.clone() for t in pair] for pair in cache]
+        model.extend(tokens[:, 36:37], cache, torch.tensor([37, 33, 40], device='cuda'))
+        for pair, old in zip(cache, before):
+            for t, o in zip(pair, old):
+                assert torch.equal(t[:2], o[:2]) and torch.equal(t[2, :, :30], o[2, :, :30])
