@@ -219,7 +219,7 @@ class TransformerBlock(nn.Module):
             if cache is not None:
                 rows = torch.arange(batch, device=input.device)[:, None]
                 for stored, fresh in zip(cache, (k, v)):     # padding rewrites what is there
-                    stored[rows, :, new.slots] = torch.where(new.live[..., None, None], fresh.transpose(1, 2),
+                    stored[rows, :, new.slots] = torch.where(new.live[..., None, None], fresh.transpose(1, 2).to(stored.dtype),
                                                              stored[rows, :, new.slots])
                 k, v = cache
                 lengths, query_lengths = new.lengths, new.query_lengths

@@ -159,3 +159,20 @@ def test_sequences_that_fill_the_cache() -> None:
         for pair, old in zip(cache, before):
             for t, o in zip(pair, old):
                 assert torch.equal(t[:2], o[:2]) and torch.equal(t[2, :, :30], o[2, :, :30])
+
+
+@pytest.mark.parametrize('amp_dtype, rtol, atol', AMP_CASES)
+@pytest.mark.parametrize('cache_dtype', [torch.float32, torch.float16, torch.bfloat16])
+def test_continued_sequences_under_autocast(cache_dtype, amp_dtype, rtol, atol) -> None:
+    """The cache may be of the weights' type or of a smaller one."""
+    torch.manual_seed(3)
+    model = TinyGPT(fused_nn, 500, 2, 128, 4, **OPTIONS).to('cuda')
+    tokens = torch.randint(0, 500, (2, 40), device='cuda')
+    with torch.no_grad(), torch.autocast('cuda', dtype=amp_dtype):
+        whole = model(tokens)
+        cache = [tuple(t.to(cache_dtype) for t in pair) for pair in model.new_cache(2, 40)]
+        done = 0
+        for step in (33, 1, 6):
+            logits = model.extend(tokens[:, done:done + step], cache, torch.full((2,), done + step, device='cuda'))
+            torch.testing.assert_close(logits.float(), whole[:, done:done + step].float(), rtol=rtol, atol=atol)
+            done += step
