@@ -114,8 +114,8 @@ class _Plan:
     """
     What a forward call of given layouts and options passes on: nothing in it belongs to a tensor.
     """
-    __slots__ = ('direct', 'options', 'dtype', 'shape', 'ref', 'group', 'scale', 'output_shape', 'output_stride', 'rest_bytes',
-                 'kept_bytes', 'workspace_bytes', 'like_inputs', 'grad_strides')
+    __slots__ = ('direct', 'options', 'dtype', 'shape', 'ref', 'group', 'scale', 'output_shape', 'output_stride', 'saved',
+                 'rest_bytes', 'kept_bytes', 'workspace_bytes', 'like_inputs', 'grad_strides')
 
 
 @functools.lru_cache(maxsize=4096)
@@ -150,6 +150,8 @@ def _forward_plan(query: Layout, key: Layout, value: Layout, lengths: Optional[L
     # what the backward pass needs, in one tensor: what the output's rounding leaves over, and the rows' sums
     plan.rest_bytes = 0 if dtype is torch.float32 else (batch * rows * heads * dim * dtype.itemsize + 255) // 256 * 256
     plan.kept_bytes = plan.rest_bytes + 4 * batch * kv_heads * lib.at_attention_row_pitch(rows, heads, kv_heads)
+    plan.saved = (query, key, value, (plan.output_shape, plan.output_stride, dtype, True),
+                  ((plan.kept_bytes,), (1,), torch.uint8, True), *counts)
     # gradients take the inputs' layouts where these are dense and [batch, tokens, heads, dim] otherwise
     plan.like_inputs, plan.grad_strides = [], []
     for shape, stride, _, _ in (query, key, value):
@@ -318,9 +320,11 @@ def _backward(ctx: Any, output_grad: Tensor) -> Tuple[Optional[Tensor], ...]:
     query, key, value, output, kept, lengths, query_lengths = ctx.saved_tensors
     # hooks may return saved tensors in other layouts than they were saved in
     forward = ctx.plan
-    forward, query, key, value, lengths, query_lengths = _planned(
-        'WindowAttention backward', query, key, value, lengths, query_lengths, *forward.options, forward.dtype)
-    output, kept = _stored_output(forward, query, output, kept)
+    saved = [t for t in (query, key, value, output, kept, lengths, query_lengths) if t is not None]
+    if tuple(map(_layout, saved)) != forward.saved or len({t.get_device() for t in saved}) != 1:
+        forward, query, key, value, lengths, query_lengths = _planned(
+            'WindowAttention backward', query, key, value, lengths, query_lengths, *forward.options, forward.dtype)
+        output, kept = _stored_output(forward, query, output, kept)
     device = query.get_device()
     if output_grad.get_device() != device:
         _lib.require_same_device('WindowAttention backward', query, output_grad)

@@ -217,10 +217,9 @@ class TransformerBlock(nn.Module):
             if self.turn is not None:
                 q, k = self.turn(q, k, None if cache is None else new.positions)
             if cache is not None:
-                rows = torch.arange(batch, device=input.device)[:, None]
+                live, slots = new.live[:, None, :, None], new.slots[:, None, :, None].expand(k.shape)
                 for stored, fresh in zip(cache, (k, v)):     # padding rewrites what is there
-                    stored[rows, :, new.slots] = torch.where(new.live[..., None, None], fresh.transpose(1, 2).to(stored.dtype),
-                                                             stored[rows, :, new.slots])
+                    stored.scatter_(2, slots, torch.where(live, fresh.to(stored.dtype), stored.gather(2, slots)))
                 k, v = cache
                 lengths, query_lengths = new.lengths, new.query_lengths
             out = self.core(q, k, v, lengths, query_lengths)
