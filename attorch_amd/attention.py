@@ -115,7 +115,7 @@ class _Plan:
     What a forward call of given layouts and options passes on: nothing in it belongs to a tensor.
     """
     __slots__ = ('direct', 'options', 'dtype', 'shape', 'ref', 'group', 'scale', 'output_shape', 'output_stride', 'saved',
-                 'rest_bytes', 'kept_bytes', 'workspace_bytes', 'like_inputs', 'grad_strides')
+                 'counts_dtype', 'rest_bytes', 'kept_bytes', 'workspace_bytes', 'like_inputs', 'grad_strides')
 
 
 @functools.lru_cache(maxsize=4096)
@@ -150,8 +150,9 @@ def _forward_plan(query: Layout, key: Layout, value: Layout, lengths: Optional[L
     # what the backward pass needs, in one tensor: what the output's rounding leaves over, and the rows' sums
     plan.rest_bytes = 0 if dtype is torch.float32 else (batch * rows * heads * dim * dtype.itemsize + 255) // 256 * 256
     plan.kept_bytes = plan.rest_bytes + 4 * batch * kv_heads * lib.at_attention_row_pitch(rows, heads, kv_heads)
-    plan.saved = (query, key, value, (plan.output_shape, plan.output_stride, dtype, True),
-                  ((plan.kept_bytes,), (1,), torch.uint8, True), *counts)
+    plan.counts_dtype = counts[0][2] if counts else None
+    plan.saved = ((query[0], key[0], value[0], plan.output_shape, (plan.kept_bytes,)),
+                  (query[1], key[1], value[1], plan.output_stride, (1,)))
     # gradients take the inputs' layouts where these are dense and [batch, tokens, heads, dim] otherwise
     plan.like_inputs, plan.grad_strides = [], []
     for shape, stride, _, _ in (query, key, value):
@@ -196,6 +197,23 @@ def _backward_plan(forward: _Plan, output_grad: Layout, dtype: torch.dtype, devi
     shape = _Shape.from_buffer_copy(forward.shape)
     shape.strides = (ctypes.c_int64 * 24)(*shape.strides[:12], *_strides(*output_grad[:2]), *forward.grad_strides)
     return shape, _lib.load().at_attention_bwd_workspace_bytes(ctypes.byref(shape))
+
+
+def _as_saved(plan: _Plan, query: Tensor, key: Tensor, value: Tensor, output: Tensor, kept: Tensor,
+              lengths: Optional[Tensor], query_lengths: Optional[Tensor]) -> bool:
+    """
+    Whether saved tensors are laid out as the plan has them.
+    """
+    device = query.get_device()
+    for counts in (lengths, query_lengths):
+        if counts is not None and not (counts.is_contiguous() and counts.get_device() == device and
+                                       counts.dtype is plan.counts_dtype):
+            return False
+    return (((query.shape, key.shape, value.shape, output.shape, kept.shape),
+             (query.stride(), key.stride(), value.stride(), output.stride(), kept.stride())) == plan.saved and
+            query.dtype is key.dtype is value.dtype is output.dtype is plan.dtype and
+            device == key.get_device() == value.get_device() == output.get_device() == kept.get_device() and
+            (query.data_ptr() | key.data_ptr() | value.data_ptr() | output.data_ptr() | kept.data_ptr()) % 16 == 0)
 
 
 def _stored_output(plan: _Plan, query: Tensor, output: Tensor, kept: Tensor) -> Tuple[Tensor, Tensor]:
@@ -320,8 +338,7 @@ def _backward(ctx: Any, output_grad: Tensor) -> Tuple[Optional[Tensor], ...]:
     query, key, value, output, kept, lengths, query_lengths = ctx.saved_tensors
     # hooks may return saved tensors in other layouts than they were saved in
     forward = ctx.plan
-    saved = [t for t in (query, key, value, output, kept, lengths, query_lengths) if t is not None]
-    if tuple(map(_layout, saved)) != forward.saved or len({t.get_device() for t in saved}) != 1:
+    if not _as_saved(forward, query, key, value, output, kept, lengths, query_lengths):
         forward, query, key, value, lengths, query_lengths = _planned(
             'WindowAttention backward', query, key, value, lengths, query_lengths, *forward.options, forward.dtype)
         output, kept = _stored_output(forward, query, output, kept)
