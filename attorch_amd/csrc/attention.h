@@ -216,13 +216,16 @@ template <typename T> struct ProbShift { static constexpr float forward = 0.f, b
 template <> struct ProbShift<f16_t> { static constexpr float forward = 15.f - kSlack, backward = 15.f; };
 
 // ds of fp16 inputs carries a factor of its own into its rounding, the same power of two for all terms of a sum (a
-// row's of dq, a key's of dk), which leaves the sum in fp32: 2^ProbShift::backward at first, lowered where a
-// term would leave fp16's range, so neither small output gradients over many keys (ds is their size
-// times a probability) nor large ones are lost while the sums themselves fit fp16.  As it stands, ds would be subnormal
+// row's of dq, a key's of dk), which leaves the sum in fp32: 2^kDsShift at first, lowered where a term would
+// leave fp16's range, so neither small output gradients over many keys (ds is their size times a probability)
+// nor large ones are lost while the sums themselves fit fp16.  As it stands, ds would be subnormal
 // below 6e-5: dq of 4096 tokens was 3 to 7 times as far off as its last rounding alone with output gradients of 1e-3,
-// and infinite where ds passed 65504.  Looking for the largest term costs up to 2 % of a step (8 x 512 tokens, 16 heads of
-// 64: 77.2 -> 78.5 us; 4 x 4096, 32 heads of 64: 1486 -> 1508 us; of 128: none).
-// The factor that brings terms of magnitude `top` > kDsLimit down to [2^12, 2^13), and its exponent.
+// and infinite where ds passed 65504.  With 2^11 a small term loses at most 2^-36: 2^12 of them, all
+// off to the same side, make up a gradient's own smallest step.  Looking for the largest term takes 2 us of the
+// 75 of a ragged batch's two kernels (6 x 1537 tokens, 12 heads on 4 of 80); with 2^15 at first, which lowers
+// factors in most walks, 5 us.
+// ds_factor: what brings terms of magnitude `top` > kDsLimit down to [2^12, 2^13), and its exponent.
+constexpr float kDsShift = 11.f, kDsStart = 2048.f;
 constexpr float kDsLimit = 32768.f;
 struct DsFactor {
   float value, log2;

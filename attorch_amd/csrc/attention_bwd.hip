@@ -13,7 +13,7 @@
 // over): an error of delta is common to a whole row of ds, and with the rounded output it was the largest
 // one in dq and dk (bf16, 512 tokens: 2.0e-3 of them against 1.7e-3 for rounding ds).  p and ds are rounded
 // to the inputs' type, as operands of the matrix cores, and ds without scale, which the sums get in fp32.
-// ds of fp16 inputs is multiplied by a power of two before it is rounded (ds_factor).  Rows that see a
+// ds of fp16 inputs is multiplied by a power of two before it is rounded (kDsShift).  Rows that see a
 // single key have zeros as ds by definition, not what p and delta's roundings would leave (dq: all such rows;
 // dk: where all rows see few keys, so that nothing larger is added).
 //
@@ -97,7 +97,7 @@ __global__ __launch_bounds__(kWaves * 64, (kPerCu<T, DT>)) void attention_dq_ker
 #pragma unroll
   for (int dt = 0; dt < DT; ++dt) dq[dt] = zero_acc();
   constexpr bool kFactor = ProbShift<T>::backward != 0.f;
-  float base = ProbShift<T>::backward - lse, undo = kFactor ? 1.f / 32768.f : 1.f;   // of the row's ds, see ds_factor
+  float base = (kFactor ? kDsShift : 0.f) - lse, undo = kFactor ? 1.f / kDsStart : 1.f;   // of the row's ds, see kDsShift
 
   const int p = seq.start + i;
   const int see_lo = valid ? p - a.left : 1, see_hi = valid ? min(p + a.right, seq.len - 1) : 0;
@@ -367,7 +367,7 @@ __global__ __launch_bounds__(kWaves * 64, (kPerCu<T, DT>)) void attention_dkv_ke
 #pragma unroll
   for (int dt = 0; dt < DT; ++dt) dk[dt] = dv[dt] = zero_acc();
   constexpr bool kFactor = ProbShift<T>::backward != 0.f;
-  float factor = 1.f;                  // of the key's ds beside the probabilities' 2^backward, see ds_factor
+  float factor = kDsStart / 32768.f;   // of the key's ds beside the probabilities' own
 
   const char* qb = a.q.p + b * a.q.batch + (int64_t)h * a.group * a.q.head;
   const char* db = a.dout.p + b * a.dout.batch + (int64_t)h * a.group * a.dout.head;

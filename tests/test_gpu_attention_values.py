@@ -9,7 +9,7 @@ import torch
 import attorch_amd
 from oracle.attention import attention_visible
 from .helpers import DTYPES
-from .test_gpu_attention import inputs
+from .test_gpu_attention import check, inputs
 
 pytestmark = pytest.mark.gpu
 NAN, INF = float('nan'), float('inf')
@@ -110,3 +110,16 @@ def test_gradients_of_any_size(tokens, size, heads, kv_heads, dim, causal, windo
             x, y = a[:, :, part].double(), b[:, :, part]
             once = (y.to(dtype).double() - y).norm()
             assert (x - y).norm() <= (2.75 if name == 'value' else 1.5) * once, name
+
+
+@pytest.mark.parametrize('dtype', [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize('causal', [True, False])
+@pytest.mark.parametrize('batch, heads, kv_heads, rows, keys, dim, window, sinks', [
+    (2, 4, 2, 300, 300, 64, None, 0), (1, 4, 2, 700, 700, 32, 20, 33), (1, 4, 2, 700, 700, 32, 20, 300), (2, 2, 1, 70, 1111, 128, None, 0),
+    (3, 6, 2, 100, 100, 80, 30, 2), (8, 32, 32, 150, 150, 40, None, 0)])
+def test_output_gradients_of_mixed_sizes(batch, heads, kv_heads, rows, keys, dim, window, sinks, causal, dtype) -> None:
+    """Rows whose output gradients are eight orders of magnitude apart, large ones behind small ones and in front of them."""
+    q, k, v, dout = inputs(batch, heads, kv_heads, rows, keys, dim, dtype)
+    size = 10.0 ** ((torch.arange(rows) * 7 // 40) * 5 % 9 - 5.0)       # 1e-5 to 1e3, another one every six rows
+    check(q, k, v, (dout * size[:, None]).to(dtype), causal=causal, window=window, sinks=sinks)
+    check(q, k, v, (dout * size.flip(0)[:, None]).to(dtype), causal=causal, window=window, sinks=sinks)
