@@ -20,10 +20,10 @@
 // Both kernels are built as the forward kernel is: a lane holds a row (first) or a key (second) of each
 // result, which then is the next product's operand as it stands.  They are bound by the matrix cores, three
 // and four products per tile, at the clock that their power leaves (1.7 to 2.0 GHz).  4 x 32 heads, 4096
-// tokens, causal, 128 features, bf16: dq 0.82 ms and dk, dv 1.15 ms, 1000 and 960 TFLOP/s; window of 1024
-// over 2 x 8192 tokens, 32 heads on 8: 0.47 and 0.59 ms, 820 and 880 TFLOP/s.  fp32, 777 patches: 50 and
-// 57 us, 74 and 86 of the 139 TFLOP/s that a large product reaches.  (One launch that adds dq with atomics
-// would save a product of the scores and lose the fixed order.)
+// tokens, causal, 128 features, bf16: dq 0.81 to 0.86 ms and dk, dv 1.15 to 1.22 ms, 960 to 1020 and 900 to 960 TFLOP/s;
+// window of 1024 over 2 x 8192 tokens, 32 heads on 8: 0.48 to 0.50 and 0.59 to 0.63 ms, 770 to 810 and 820 to 870
+// TFLOP/s.  fp32, 777 patches: 50 to 53 and 57 to 62 us, 70 to 74 and 79 to 86 of the 139 TFLOP/s that a large product
+// reaches.  (One launch that adds dq with atomics would save a product of the scores and lose the fixed order.)
 #include <type_traits>
 
 #include "attention.h"

@@ -17,9 +17,9 @@
 //
 // Many rows: bound by the matrix cores and the exponentials, 16 of which take as long as half of the 16
 // products of a 32 x 32 tile of 128 features, and by the power of both: the clock falls to 1.75 GHz.  4 x 32
-// heads, 4096 tokens, causal, 128 features, bf16: 0.69 ms, 800 TFLOP/s; window of 1024 over 2 x 8192 tokens,
-// 32 heads on 8: 0.36 ms, 720 TFLOP/s; a chunk of 1024 tokens over 16384 with a window of 4096: 88 us,
-// 780 TFLOP/s.  fp32, 777 patches: 36 us, 68 TFLOP/s.
+// heads, 4096 tokens, causal, 128 features, bf16: 0.68 to 0.72 ms, 770 to 810 TFLOP/s; window of 1024 over 2 x
+// 8192 tokens, 32 heads on 8: 0.36 to 0.38 ms, 680 to 715 TFLOP/s; a chunk of 1024 tokens over 16384 with a window of
+// 4096: 87 to 91 us, 750 to 790 TFLOP/s.  fp32, 777 patches: 37 us, 66 TFLOP/s.
 // Single tokens: bound by reading the keys and values once.  64 conversations of 4096 to 8192 tokens, 32
 // heads on 8, bf16: 319 us, 5.0 TB/s; one of 131072: 97 us and 6 us for the join, 5.4 TB/s.  (Tiles of 32
 // keys with up to five on their way read 4.5 TB/s: fewer, larger loads keep memory busier.  For many rows
