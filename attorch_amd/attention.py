@@ -289,9 +289,11 @@ class WindowAttentionAutoGrad(torch.autograd.Function):
         output_dtype = get_output_dtype(query.dtype, autocast='fp16')
         if not query.dtype is key.dtype is value.dtype is output_dtype and torch.is_autocast_enabled('cuda'):
             query, key, value = (t.to(output_dtype) for t in (query, key, value))
-        head_dim = query.shape[-1]
+        given = query.shape
         plan, query, key, value, lengths, query_lengths = _planned(
             'WindowAttention', query, key, value, lengths, query_lengths, causal, window, num_sinks, scale, output_dtype)
+
+        head_dim = given[3]
 
         # not as a view: autograd refuses to change those of a Function in place
         output = torch.empty_strided(plan.output_shape, plan.output_stride, device=query.device, dtype=output_dtype)
